@@ -1,0 +1,531 @@
+// Sliding-window attention, forward, for sm_100a (visibility rule: window.cuh). Persistent CTAs; an item of work is one or two
+// tiles of 128 query rows that walk the same list of key blocks, so a K / V block fetched once serves both tiles and the
+// softmax of one tile runs under the matrix products of the other:
+//   warp 0       TMA producer: the tiles' queries and a ring of K and V blocks,
+//   warp 1       issues S = Q K^T and O += P V as UMMAs; S, P and O stay in tensor memory (P overwrites the scores it came from),
+//   warps 4-7 and 8-11  one warpgroup per tile, a thread per query row: running maximum and sum, P in bf16, output.
+// The two tiles are two query heads of one key/value head on the same rows where the group is even, else neighbouring rows of
+// one head. O is rescaled only when a row's maximum has grown by more than 2^8 since the last rescale: P then stays below 2^8
+// and its bf16 rounding is relative, so nothing is lost, and after the first blocks the rescale hardly ever happens.
+#include "host.h"
+#include "ptx.cuh"
+#include "window.cuh"
+
+namespace mb {
+
+constexpr int kWfThreads = 384;
+constexpr int kWfStages = 5;                       // K and V blocks in flight
+// registers: the launch gives 168 x 384 = 64512; after the split 128 x 56 + 256 x 224 = 64512
+constexpr int kWfLaunchRegs = 168, kWfOtherRegs = 56, kWfSoftmaxRegs = 224;
+static_assert(128 * kWfOtherRegs + 256 * kWfSoftmaxRegs <= kWfThreads * kWfLaunchRegs, "register split exceeds the launch");
+constexpr float kWfLog2e = 1.4426950408889634f, kWfLn2 = 0.6931471805599453f;
+constexpr float kWfGrowth = 8.f;                   // log2 of how far P may exceed 1 before O is rescaled
+
+struct WindowFwdArgs {
+  __nv_bfloat16* out;       // [B, Sq, Hq, D]
+  float* lse;               // [B, Hq, Sq]
+  WindowRule rule;
+  int B, Sq, Sk, Hq, Hkv;
+  int pair;                 // tiles of an item: 0 one tile, 1 two heads of a group, 2 two neighbouring row tiles
+  int row_units, head_units, items;
+  float scale_log2;
+  int* status;
+};
+
+__device__ __forceinline__ float wf_exp2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+struct WindowItem {
+  int batch, kv_head;
+  int head[2], q0[2];
+  WindowTile tile[2];
+  int a0, na, w0, n;        // union list: blocks a0 .. a0 + na, then w0 ..; n in all
+  __device__ __forceinline__ int block(int u) const { return u < na ? a0 + u : w0 + u - na; }
+};
+
+// Where the tiles of an item lie; late rows (long lists) first. `with_tiles`: also what they visit (warp-collective).
+__device__ __forceinline__ void window_item(const WindowFwdArgs& p, int item, WindowItem& it) {
+  const int hu = item % p.head_units;
+  const int rest = item / p.head_units;
+  const int ru = p.row_units - 1 - rest % p.row_units;
+  it.batch = rest / p.row_units;
+  const int head = p.pair == 1 ? 2 * hu : hu;
+  it.kv_head = head / (p.Hq / p.Hkv);
+  it.head[0] = head, it.head[1] = p.pair == 1 ? head + 1 : head;
+  it.q0[0] = ru * (p.pair == 2 ? 2 : 1) * kWinBlock;
+  it.q0[1] = p.pair == 0 ? p.Sq : p.pair == 1 ? it.q0[0] : it.q0[0] + kWinBlock;   // a tile from row Sq on is empty
+}
+
+__device__ __forceinline__ void window_item_blocks(const WindowFwdArgs& p, WindowItem& it) {
+  it.tile[0] = window_tile(p.rule, it.batch, p.Sq, p.Sk, it.q0[0]);
+  it.tile[1] = p.pair == 1 ? it.tile[0] : window_tile(p.rule, it.batch, p.Sq, p.Sk, it.q0[1]);
+  const WindowTile &x = it.tile[0], &y = it.tile[1];
+  it.a0 = it.na = it.w0 = it.n = 0;
+  const bool hx = x.b1 > x.b0, hy = y.b1 > y.b0;
+  if (!hx && !hy) return;
+  it.w0 = !hx ? y.b0 : !hy ? x.b0 : min(x.b0, y.b0);
+  const int w1 = max(x.b1, y.b1);
+  // first tokens before the union's window; a tile whose document starts later has its own inside it
+  int lo = kWinNone, hi = 0;
+  if (x.ea > x.sa) lo = x.sa, hi = x.ea;
+  if (y.ea > y.sa) lo = min(lo, y.sa), hi = max(hi, y.ea);
+  hi = min(hi, it.w0);
+  if (lo < hi) it.a0 = lo, it.na = hi - lo;
+  it.n = it.na + w1 - it.w0;
+}
+
+template <int D>
+__global__ void __launch_bounds__(kWfThreads, 1)
+window_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
+                  const __grid_constant__ CUtensorMap tmV, const WindowFwdArgs p) {
+  constexpr int ATOMS = D / 64;                    // 64-wide swizzle atoms along head_dim
+  constexpr int TILE_BYTES = kWinBlock * D * 2;
+  constexpr int ATOM_BYTES = kWinBlock * 128;
+  constexpr uint32_t TMEM_COLS = 512, O_COL = 0, S_COL = 256;   // O of tile t at t * 128, its scores at 256 + t * 128
+
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint8_t* sQ = smem;                              // 2 tiles
+  uint8_t* sKV = sQ + 2 * TILE_BYTES;              // kWfStages blocks
+  uint64_t* bars = reinterpret_cast<uint64_t*>(sKV + kWfStages * TILE_BYTES);
+  uint64_t* q_full = bars;                         // 2
+  uint64_t* q_empty = bars + 2;                    // 2
+  uint64_t* s_full = bars + 4;                     // 2
+  uint64_t* p_full = bars + 6;                     // 2
+  uint64_t* o_full = bars + 8;                     // 2
+  uint64_t* kv_full = bars + 10;                   // kWfStages
+  uint64_t* kv_empty = kv_full + kWfStages;        // kWfStages
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(kv_empty + kWfStages);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (threadIdx.x == 0) {
+    for (int t = 0; t < 2; ++t) {
+      mbar_init(&q_full[t], 1);
+      mbar_init(&q_empty[t], 1);
+      mbar_init(&s_full[t], 1);
+      mbar_init(&p_full[t], 4);
+      mbar_init(&o_full[t], 1);
+    }
+    for (int i = 0; i < kWfStages; ++i) {
+      mbar_init(&kv_full[i], 1);
+      mbar_init(&kv_empty[i], 1);
+    }
+    abort_flag[0] = 0;
+    abort_flag[1] = p.status[3];
+    fence_barrier_init();
+    prefetch_tmap(&tmQ);
+    prefetch_tmap(&tmK);
+    prefetch_tmap(&tmV);
+  }
+  if (warp == 1) {
+    tmem_alloc(tmem_slot, TMEM_COLS);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem_base = *tmem_slot;
+
+  if (warp < 4) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kWfOtherRegs));
+    if (warp == 0) {
+      // ---------------------------------------------------------------- TMA producer
+      int slot = 0, round = 0;                     // ring position and how often it has gone round
+      int q_uses[2] = {0, 0};
+      bool ok = true;
+      for (int item = blockIdx.x; item < p.items; item += gridDim.x) {
+        WindowItem it;
+        window_item(p, item, it);
+        window_item_blocks(p, it);
+        if (lane == 0) {
+#pragma unroll
+          for (int t = 0; t < 2; ++t) {
+            if (!ok || it.tile[t].count() == 0) continue;
+            ok = mbar_wait(&q_empty[t], (q_uses[t] & 1) ^ 1, abort_flag);
+            if (!ok) continue;
+            ++q_uses[t];
+            mbar_arrive_expect_tx(&q_full[t], TILE_BYTES);
+#pragma unroll
+            for (int a = 0; a < ATOMS; ++a)
+              tma_load_4d(sQ + t * TILE_BYTES + a * ATOM_BYTES, &tmQ, &q_full[t], a * 64, it.head[t], it.q0[t], it.batch);
+          }
+          for (int u = 0; ok && u < it.n; ++u) {
+            const int key0 = it.block(u) * kWinBlock;
+            for (int kv = 0; kv < 2; ++kv) {
+              ok = mbar_wait(&kv_empty[slot], (round & 1) ^ 1, abort_flag);
+              if (!ok) break;
+              mbar_arrive_expect_tx(&kv_full[slot], TILE_BYTES);
+#pragma unroll
+              for (int a = 0; a < ATOMS; ++a)
+                tma_load_4d(sKV + slot * TILE_BYTES + a * ATOM_BYTES, kv ? &tmV : &tmK, &kv_full[slot], a * 64, it.kv_head, key0, it.batch);
+              if (++slot == kWfStages) slot = 0, ++round;
+            }
+          }
+        }
+        ok = __shfl_sync(0xffffffffu, static_cast<int>(ok), 0) != 0;
+        if (!ok) break;
+      }
+    } else if (warp == 1) {
+      // ---------------------------------------------------------------- UMMA issuer
+      // Step u: for each tile first O += P V of its last block (u - 1), then its scores of block u over that P. The scores'
+      // commit therefore also says that the product before them is complete, which is what a rescale of O waits for.
+      const uint32_t idesc_qk = make_idesc_bf16(kWinBlock, kWinBlock, 0, 0);
+      const uint32_t idesc_pv = make_idesc_bf16(kWinBlock, D, 0, 1);
+      constexpr uint32_t hi = smem_desc_hi_sw128(1024);
+      int base = 0;                                // K / V blocks consumed before this item
+      int p_count[2] = {0, 0}, q_count[2] = {0, 0};
+      bool ok = true;
+      for (int item = blockIdx.x; item < p.items; item += gridDim.x) {
+        WindowItem it;
+        window_item(p, item, it);
+        window_item_blocks(p, it);
+        if (lane == 0) {
+          int left[2] = {it.tile[0].count(), it.tile[1].count()};   // blocks whose scores are not issued yet
+          bool pending[2] = {false, false}, begun[2] = {false, false}, has_o[2] = {false, false};
+          for (int u = 0; ok && u <= it.n; ++u) {
+            const int kc = base + 2 * u, vc = kc - 1;               // ring counts of K of block u and V of block u - 1
+            const int ks = kc % kWfStages, vs = (vc + kWfStages) % kWfStages;
+            const int blk = u < it.n ? it.block(u) : -1;
+#pragma unroll
+            for (int t = 0; t < 2; ++t) {
+              if (!ok) continue;
+              const uint32_t s_tmem = tmem_base + S_COL + static_cast<uint32_t>(t) * 128u;
+              if (pending[t]) {
+                ok = mbar_wait(&kv_full[vs], (vc / kWfStages) & 1, abort_flag) && mbar_wait(&p_full[t], p_count[t] & 1, abort_flag);
+                if (!ok) continue;
+                ++p_count[t];
+                tc_fence_after();
+                const uint32_t v_lo = smem_desc_lo(smem_u32(sKV + vs * TILE_BYTES), ATOM_BYTES);
+                const uint32_t o_tmem = tmem_base + O_COL + static_cast<uint32_t>(t) * 128u;
+                const uint32_t acc0 = has_o[t] ? 1u : 0u;
+#pragma unroll
+                for (int kk = 0; kk < kWinBlock / 16; ++kk)
+                  umma_bf16_ts_lh(o_tmem, s_tmem + static_cast<uint32_t>(kk * 8), v_lo + static_cast<uint32_t>(kk * 128), hi, idesc_pv,
+                                  kk != 0 ? 1u : acc0);
+                has_o[t] = true;
+                pending[t] = false;
+                if (left[t] == 0) umma_commit(&o_full[t]);
+              }
+              if (blk >= 0 && it.tile[t].has(blk)) {
+                if (!begun[t]) {
+                  ok = mbar_wait(&q_full[t], q_count[t] & 1, abort_flag);
+                  if (!ok) continue;
+                  ++q_count[t];
+                  begun[t] = true;
+                }
+                ok = mbar_wait(&kv_full[ks], (kc / kWfStages) & 1, abort_flag);
+                if (!ok) continue;
+                tc_fence_after();
+                const uint32_t q_lo = smem_desc_lo(smem_u32(sQ + t * TILE_BYTES), 16), k_lo = smem_desc_lo(smem_u32(sKV + ks * TILE_BYTES), 16);
+#pragma unroll
+                for (int kk = 0; kk < D / 16; ++kk) {
+                  const uint32_t off = static_cast<uint32_t>(((kk >> 2) * ATOM_BYTES + (kk & 3) * 32) >> 4);
+                  umma_bf16_ss_lh(s_tmem, q_lo + off, hi, k_lo + off, hi, idesc_qk, kk != 0 ? 1u : 0u);
+                }
+                umma_commit(&s_full[t]);
+                pending[t] = true;
+                if (--left[t] == 0) umma_commit(&q_empty[t]);
+              }
+            }
+            if (!ok) break;
+            // A block that no tile needed (a gap of the union) still has to have arrived before its slot is given back.
+            if (u > 0) {
+              ok = mbar_wait(&kv_full[vs], (vc / kWfStages) & 1, abort_flag);
+              if (!ok) break;
+              umma_commit(&kv_empty[vs]);
+            }
+            if (u < it.n) {
+              ok = mbar_wait(&kv_full[ks], (kc / kWfStages) & 1, abort_flag);
+              if (!ok) break;
+              umma_commit(&kv_empty[ks]);
+            }
+          }
+          base += 2 * it.n;
+        }
+        ok = __shfl_sync(0xffffffffu, static_cast<int>(ok), 0) != 0;
+        if (!ok) break;
+      }
+    }
+    __syncwarp();
+  } else {
+    // ------------------------------------------------------------------ softmax and output: a thread per query row
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kWfSoftmaxRegs));
+    const int t = (warp - 4) >> 2;
+    const int row = (warp & 3) * 32 + lane;
+    const uint32_t t_lane = static_cast<uint32_t>((warp & 3) * 32) << 16;
+    const uint32_t s_tmem = tmem_base + S_COL + static_cast<uint32_t>(t) * 128u + t_lane;
+    const uint32_t o_tmem = tmem_base + O_COL + static_cast<uint32_t>(t) * 128u + t_lane;
+    int s_count = 0, o_count = 0;
+    bool ok = true;
+    for (int item = blockIdx.x; item < p.items; item += gridDim.x) {
+      WindowItem it;
+      window_item(p, item, it);
+      const int q0 = it.q0[t], head = it.head[t];
+      if (q0 >= p.Sq) continue;                    // the missing second tile
+      const WindowTile tile = window_tile(p.rule, it.batch, p.Sq, p.Sk, q0);
+      const int n = tile.count();
+      const int qi = q0 + row;
+      const WindowRow w = window_row(p.rule, it.batch, p.Sk, qi + p.Sk - p.Sq, qi < p.Sq);
+      float m_run = -INFINITY, l_run = 0.f;        // maximum (exp2 domain) that P is relative to, sum of P
+      for (int j = 0; j < n; ++j) {
+        ok = mbar_wait(&s_full[t], s_count & 1, abort_flag);
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) break;
+        ++s_count;
+        tc_fence_after();
+        const int key0 = tile.block(j) * kWinBlock;
+        uint32_t s[128];
+#pragma unroll
+        for (int c = 0; c < 4; ++c) tmem_ld_32x32b_x32(s_tmem + c * 32, reinterpret_cast<uint32_t(&)[32]>(s[c * 32]));
+        tmem_ld_wait();
+        if (key0 < tile.full_lo || key0 + kWinBlock - 1 > tile.full_hi) {
+#pragma unroll
+          for (int c = 0; c < 4; ++c) {
+            const uint32_t seen = window_bits(w, key0 + c * 32);
+#pragma unroll
+            for (int i = 0; i < 32; ++i)
+              if (!((seen >> i) & 1u)) s[c * 32 + i] = __float_as_uint(-INFINITY);
+          }
+        }
+        float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+        for (int i = 0; i < 128; ++i) mx[i & 3] = fmaxf(mx[i & 3], __uint_as_float(s[i]));
+        const float m_blk = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * p.scale_log2;
+        if (__any_sync(0xffffffffu, m_blk > m_run + kWfGrowth)) {
+          const float m_new = fmaxf(m_run, m_blk);
+          const float alpha = m_run == -INFINITY ? 0.f : wf_exp2(m_run - m_new);
+          m_run = m_new;
+          l_run *= alpha;
+          if (j > 0) {
+#pragma unroll 1
+            for (int c = 0; c < D; c += 16) {
+              uint32_t r[16];
+              tmem_ld_32x32b_x16(o_tmem + c, r);
+              tmem_ld_wait();
+#pragma unroll
+              for (int i = 0; i < 16; ++i) r[i] = __float_as_uint(__uint_as_float(r[i]) * alpha);
+              tmem_st_32x32b_x16(o_tmem + c, r);
+            }
+          }
+        }
+        const float m_safe = m_run == -INFINITY ? 0.f : m_run;
+        float sum[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {              // 32 keys: 16 columns of packed P
+          uint32_t pk[16];
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            const float a = wf_exp2(fmaf(__uint_as_float(s[c * 32 + 2 * i]), p.scale_log2, -m_safe));
+            const float b = wf_exp2(fmaf(__uint_as_float(s[c * 32 + 2 * i + 1]), p.scale_log2, -m_safe));
+            sum[i & 3] += a + b;
+            pk[i] = pack_bf16x2(a, b);
+          }
+          tmem_st_32x32b_x16(s_tmem + c * 16, pk);
+        }
+        l_run += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+        tmem_st_wait();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&p_full[t]);
+      }
+      if (!ok) break;
+      // ---------------------------------------------------------------- output
+      if (n > 0) {
+        ok = mbar_wait(&o_full[t], o_count & 1, abort_flag);
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) break;
+        ++o_count;
+        tc_fence_after();
+      }
+      const float inv = l_run > 0.f ? 1.f / l_run : 0.f;
+      __nv_bfloat16* dst = p.out + ((static_cast<long long>(it.batch) * p.Sq + qi) * p.Hq + head) * D;
+#pragma unroll 1
+      for (int c = 0; c < D; c += 32) {
+        uint32_t r[32];
+        if (n > 0) {                               // warp-collective: every lane takes part, rows inside the sequence are stored
+          tmem_ld_32x32b_x32(o_tmem + c, r);
+          tmem_ld_wait();
+        } else {
+#pragma unroll
+          for (int i = 0; i < 32; ++i) r[i] = 0u;
+        }
+        if (qi < p.Sq) {
+#pragma unroll
+          for (int i = 0; i < 32; i += 8) {
+            uint4 v;
+            v.x = pack_bf16x2(__uint_as_float(r[i]) * inv, __uint_as_float(r[i + 1]) * inv);
+            v.y = pack_bf16x2(__uint_as_float(r[i + 2]) * inv, __uint_as_float(r[i + 3]) * inv);
+            v.z = pack_bf16x2(__uint_as_float(r[i + 4]) * inv, __uint_as_float(r[i + 5]) * inv);
+            v.w = pack_bf16x2(__uint_as_float(r[i + 6]) * inv, __uint_as_float(r[i + 7]) * inv);
+            *reinterpret_cast<uint4*>(dst + c + i) = v;
+          }
+        }
+      }
+      tc_fence_before();                           // these reads of O come before the next item's first product (via p_full)
+      if (qi < p.Sq)
+        p.lse[(static_cast<long long>(it.batch) * p.Hq + head) * p.Sq + qi] = l_run > 0.f ? (m_run + log2f(l_run)) * kWfLn2 : -INFINITY;
+    }
+  }
+
+  // -------------------------------------------------------------------- teardown
+  tc_fence_before();
+  __syncthreads();
+  if (*abort_flag) {
+    __nanosleep(50000);
+    if (threadIdx.x == 0) {
+      atomicOr(&p.status[0], MB_ERR_MBAR_TIMEOUT);
+      p.status[1] = static_cast<int>(blockIdx.x);
+    }
+  }
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc(tmem_base, TMEM_COLS);
+  }
+}
+
+template <int D>
+static int launch_window_fwd(const CUtensorMap& tmQ, const CUtensorMap& tmK, const CUtensorMap& tmV, const WindowFwdArgs& args,
+                             cudaStream_t stream) {
+  constexpr size_t smem = 1024 + (2 + kWfStages) * (kWinBlock * D * 2) + 256;
+  static bool configured[64] = {false};
+  int dev = 0;
+  MB_CHECK_CUDA(cudaGetDevice(&dev));
+  if (!configured[dev & 63]) {
+    cudaFuncAttributes at;
+    MB_CHECK_CUDA(cudaFuncGetAttributes(&at, window_fwd_kernel<D>));
+    if (at.numRegs != kWfLaunchRegs) {             // the split of the register file is made for this launch size
+      set_last_error("mb_window_attn_fwd: built with another register count than the register split assumes");
+      return -6;
+    }
+    MB_CHECK_CUDA(cudaFuncSetAttribute(window_fwd_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem)));
+    configured[dev & 63] = true;
+  }
+  const int grid = args.items < sm_count() ? args.items : sm_count();
+  window_fwd_kernel<D><<<grid, kWfThreads, smem, stream>>>(tmQ, tmK, tmV, args);
+  count_launch();
+  MB_CHECK_CUDA(cudaGetLastError());
+  return 0;
+}
+
+// ---------------------------------------------------------------------------------------------- documents
+// First and one-past-last index of every token's document, one block per row: a thread owns a contiguous piece of the row,
+// the pieces are joined by a scan over the block (the last boundary to the left, the first to the right).
+constexpr int kDocThreads = 1024;
+
+template <typename T>
+__global__ void __launch_bounds__(kDocThreads) document_bounds_kernel(const T* __restrict__ ids_all, int* __restrict__ starts_all,
+                                                                      int* __restrict__ ends_all, int S) {
+  __shared__ int left[kDocThreads], right[kDocThreads];
+  const T* ids = ids_all + static_cast<long long>(blockIdx.x) * S;
+  int* starts = starts_all + static_cast<long long>(blockIdx.x) * S;
+  int* ends = ends_all + static_cast<long long>(blockIdx.x) * S;
+  const int per = (S + kDocThreads - 1) / kDocThreads;
+  const int tid = threadIdx.x;
+  const int a = min(tid * per, S), b = min(a + per, S);
+  int first = S, last = 0;                         // first and last index of the piece at which a run begins
+  for (int j = a; j < b; ++j)
+    if (j == 0 || ids[j] != ids[j - 1]) {
+      first = min(first, j);
+      last = j;
+    }
+  left[tid] = last, right[tid] = first;
+  __syncthreads();
+  for (int o = 1; o < kDocThreads; o <<= 1) {
+    const int l = tid >= o ? left[tid - o] : 0, r = tid + o < kDocThreads ? right[tid + o] : S;
+    __syncthreads();
+    left[tid] = max(left[tid], l), right[tid] = min(right[tid], r);
+    __syncthreads();
+  }
+  int s = tid ? left[tid - 1] : 0;                 // the run that the piece's first token may continue
+  const int after = tid + 1 < kDocThreads ? right[tid + 1] : S;
+  for (int j = a; j < b; ++j) {
+    if (j == 0 || ids[j] != ids[j - 1]) s = j;
+    starts[j] = ids[j] == static_cast<T>(-1) ? kWinNone : s;
+  }
+  int e = after;
+  for (int j = b - 1; j >= a; --j) {
+    ends[j] = ids[j] == static_cast<T>(-1) ? 0 : e;
+    if (j == 0 || ids[j] != ids[j - 1]) e = j;
+  }
+}
+
+// Sizes, strides and addresses that both directions ask for; nullptr or what is wrong.
+const char* window_attn_problem(int B, int Sq, int Sk, int Hq, int Hkv, int D, int window, int sinks, const long long* strides,
+                                int n_strides, const void* const* pointers, int n_pointers) {
+  if ((D != 64 && D != 128) || Hkv < 1 || Hq < 1 || Hq % Hkv != 0 || B < 1 || Sq < 1 || Sk < 1)
+    return "head_dim must be 64 or 128, query heads a multiple of key/value heads, lengths positive";
+  if (window < 1 || sinks < 0) return "window must be positive and sinks not negative";
+  if (Sq >= (1 << 30) || Sk >= (1 << 30) || B > 65535 || Hq > 65535) return "lengths of 2^30 and more, or over 65535 rows or heads";
+  for (int i = 0; i < n_strides; ++i)
+    if (strides[i] & 7) return "strides must be multiples of 8 elements";
+  for (int i = 0; i < n_pointers; ++i)
+    if (reinterpret_cast<uintptr_t>(pointers[i]) & 15) return "tensors must be 16-byte aligned";
+  return nullptr;
+}
+
+}  // namespace mb
+
+// ids [B, S] (int64 when `wide`, else int32; runs of one id are documents, -1 is padding) -> starts, ends [B, S] as in window.cuh.
+MB_API int mb_document_bounds(const void* ids, int wide, int* starts, int* ends, int B, int S, cudaStream_t stream) {
+  using namespace mb;
+  if (B < 1 || S < 1 || S >= (1 << 30)) {
+    set_last_error("mb_document_bounds: rows and lengths must be positive, lengths below 2^30");
+    return -1;
+  }
+  if (wide) document_bounds_kernel<long long><<<B, kDocThreads, 0, stream>>>(static_cast<const long long*>(ids), starts, ends, S);
+  else document_bounds_kernel<int><<<B, kDocThreads, 0, stream>>>(static_cast<const int*>(ids), starts, ends, S);
+  count_launch();
+  MB_CHECK_CUDA(cudaGetLastError());
+  return 0;
+}
+
+// q [B, Sq, Hq, D], k / v [B, Sk, Hkv, D] bf16 with element strides between tokens and batches (heads contiguous inside a
+// token), out [B, Sq, Hq, D] bf16 contiguous, lse [B, Hq, Sq] fp32 (-inf where nothing is visible). starts: mb_document_bounds
+// of the key rows, or null for one document a row.
+MB_API int mb_window_attn_fwd(const void* q, long long q_tstride, long long q_bstride, const void* k, long long k_tstride,
+                              long long k_bstride, const void* v, long long v_tstride, long long v_bstride, void* out, float* lse,
+                              const int* starts, int B, int Sq, int Sk, int Hq, int Hkv, int D, int window, int sinks, float scale,
+                              cudaStream_t stream) {
+  using namespace mb;
+  const long long strides[] = {q_tstride, q_bstride, k_tstride, k_bstride, v_tstride, v_bstride};
+  const void* pointers[] = {q, k, v, out};
+  if (const char* what = window_attn_problem(B, Sq, Sk, Hq, Hkv, D, window, sinks, strides, 6, pointers, 4)) {
+    set_last_error(what);
+    return -1;
+  }
+  int* status = status_ptr();
+  if (!status) return -4;
+  WindowFwdArgs a;
+  a.out = static_cast<__nv_bfloat16*>(out);
+  a.lse = lse;
+  a.rule = {starts, nullptr, window < Sk ? window : Sk, sinks < Sk ? sinks : Sk};
+  a.B = B, a.Sq = Sq, a.Sk = Sk, a.Hq = Hq, a.Hkv = Hkv;
+  a.scale_log2 = scale * kWfLog2e;
+  a.status = status;
+  // Two tiles to an item once there are more tiles than SMs; below that every tile gets an SM of its own.
+  const long long row_tiles = (Sq + kWinBlock - 1) / kWinBlock;
+  a.pair = row_tiles * Hq * B <= sm_count() ? 0 : (Hq / Hkv) % 2 == 0 ? 1 : 2;
+  a.row_units = static_cast<int>(a.pair == 2 ? (row_tiles + 1) / 2 : row_tiles);
+  a.head_units = a.pair == 1 ? Hq / 2 : Hq;
+  const long long items = static_cast<long long>(a.row_units) * a.head_units * B;
+  if (items >= (1ll << 31) - 65536) {
+    set_last_error("mb_window_attn_fwd: too many query tiles");
+    return -1;
+  }
+  a.items = static_cast<int>(items);
+  CUtensorMap tmQ, tmK, tmV;
+  const uint32_t box[4] = {64, 1, static_cast<uint32_t>(kWinBlock), 1};
+  auto encode = [&](CUtensorMap* m, const void* x, int heads, int S, long long tstride, long long bstride) {
+    const uint64_t dims[4] = {(uint64_t)D, (uint64_t)heads, (uint64_t)S, (uint64_t)B};
+    const uint64_t bytes[3] = {(uint64_t)D * 2, (uint64_t)tstride * 2, (uint64_t)bstride * 2};
+    return encode_tmap_4d(m, x, dims, bytes, box, 2, true);
+  };
+  if (!encode(&tmQ, q, Hq, Sq, q_tstride, q_bstride) || !encode(&tmK, k, Hkv, Sk, k_tstride, k_bstride) ||
+      !encode(&tmV, v, Hkv, Sk, v_tstride, v_bstride))
+    return -5;
+  return D == 128 ? launch_window_fwd<128>(tmQ, tmK, tmV, a, stream) : launch_window_fwd<64>(tmQ, tmK, tmV, a, stream);
+}

@@ -88,6 +88,92 @@ def causal_attention(q, k, v, *, position_ids=None, sequence_ids=None, scale: fl
                      packed_causal=True)
 
 
+# ------------------------------------------------------------------------------------------------ sliding window
+def build_window_mask(Sq: int, Sk: int, window: int, sinks: int = 0, sequence_ids=None, device=None) -> torch.Tensor:
+    """Boolean ``[B or 1, Sq, Sk]`` mask of :func:`sliding_window_attention`."""
+    device = device if sequence_ids is None else sequence_ids.device
+    key = torch.arange(Sk, device=device).view(1, 1, Sk)
+    pos = torch.arange(Sk - Sq, Sk, device=device).view(1, Sq, 1)
+    if sequence_ids is None or Sk == 0:
+        return (key <= pos) & ((pos - key < window) | (key < sinks)) & (pos >= 0)
+    begins = torch.ones_like(sequence_ids, dtype=torch.bool)
+    begins[:, 1:] = sequence_ids[:, 1:] != sequence_ids[:, :-1]
+    start = torch.where(begins, torch.arange(Sk, device=device), 0).cummax(dim=1).values
+    at = pos.view(-1).clamp_min(0)
+    start, real = start[:, at].unsqueeze(2), (sequence_ids[:, at] != PAD_SEQUENCE_ID).unsqueeze(2) & (pos >= 0)
+    return real & (key >= start) & (key <= pos) & ((pos - key < window) | (key - start < sinks))
+
+
+def sliding_window_reference(q, k, v, *, window: int, sinks: int = 0, sequence_ids=None, scale: float | None = None,
+                             return_lse: bool = False):
+    """Eager :func:`sliding_window_attention` in fp32 (fp64 for fp64 inputs); the whole ``Sq x Sk`` score matrix is formed."""
+    B, Sq, hq, D = q.shape
+    Sk, hkv = k.shape[1], k.shape[2]
+    dt = torch.float64 if q.dtype == torch.float64 else torch.float32
+    scale = scale if scale is not None else 1.0 / math.sqrt(D)
+    qf = q.to(dt).permute(0, 2, 1, 3).reshape(B, hkv, hq // hkv, Sq, D)
+    kf = k.to(dt).permute(0, 2, 1, 3).unsqueeze(2)
+    vf = v.to(dt).permute(0, 2, 1, 3).unsqueeze(2)
+    seen = build_window_mask(Sq, Sk, window, sinks, sequence_ids, q.device)[:, None, None]
+    some = seen.any(-1, keepdim=True)
+    scores = torch.matmul(qf, kf.transpose(-1, -2)) * scale
+    scores = scores.masked_fill(~seen & some, float("-inf")).masked_fill(~some, 0.0)
+    out = torch.matmul(scores.softmax(-1) * some, vf).reshape(B, hq, Sq, D).permute(0, 2, 1, 3).to(q.dtype)
+    if not return_lse:
+        return out
+    with torch.no_grad():
+        lse = torch.logsumexp(scores.masked_fill(~some, float("-inf")), dim=-1).reshape(B, hq, Sq).float()
+    return out, lse
+
+
+def _check_window_arguments(q, k, v, window, sinks, sequence_ids, scale) -> None:
+    if q.dim() != 4 or k.dim() != 4 or k.shape != v.shape:
+        raise ValueError(f"sliding_window_attention takes q [B, Sq, heads, D] and k, v [B, Sk, kv_heads, D], got {tuple(q.shape)}, "
+                         f"{tuple(k.shape)}, {tuple(v.shape)}")
+    if q.shape[0] != k.shape[0] or q.shape[3] != k.shape[3] or k.shape[2] < 1 or q.shape[2] % k.shape[2]:
+        raise ValueError(f"q {tuple(q.shape)} and k {tuple(k.shape)} need the same batch and head_dim, and query heads a multiple of "
+                         "key/value heads")
+    if not (q.dtype == k.dtype == v.dtype) or not q.is_floating_point():
+        raise ValueError(f"q, k and v need one floating-point type, got {q.dtype}, {k.dtype}, {v.dtype}")
+    if not (q.device == k.device == v.device):
+        raise ValueError(f"q, k and v are on different devices: {q.device}, {k.device}, {v.device}")
+    for name, value, least in (("window", window, 1), ("sinks", sinks, 0)):
+        if isinstance(value, bool) or not isinstance(value, int) or value < least:
+            raise ValueError(f"{name} must be an integer of at least {least}, got {value!r}")
+    if scale is not None and not 0.0 < scale < math.inf:
+        raise ValueError(f"scale must be positive and finite, got {scale!r}")
+    if sequence_ids is not None:
+        if tuple(sequence_ids.shape) != (k.shape[0], k.shape[1]) or sequence_ids.dtype not in (torch.int32, torch.int64):
+            raise ValueError(f"sequence_ids are one int32 or int64 id per key, {(k.shape[0], k.shape[1])}, got "
+                             f"{tuple(sequence_ids.shape)} {sequence_ids.dtype}")
+        if sequence_ids.device != q.device:
+            raise ValueError(f"sequence_ids are on {sequence_ids.device}, q on {q.device}")
+
+
+def sliding_window_attention(q, k, v, *, window: int, sinks: int = 0, sequence_ids=None, scale: float | None = None,
+                             return_lse: bool = False):
+    """Causal attention to the last ``window`` keys and to the first ``sinks`` tokens of the document. Differentiable.
+
+    q ``[B, Sq, heads, D]``, k / v ``[B, Sk, kv_heads, D]`` (any strides; query heads a multiple of key/value heads). Query ``i``
+    stands at key index ``p = i + Sk - Sq``: ``Sq == Sk`` in training, fewer queries for a chunk or a token behind earlier keys.
+    ``sequence_ids [B, Sk]`` packs documents into a row: a document is a RUN of equal ids (an id that comes back later begins
+    another document), -1 is padding, which sees nothing and is seen by nothing. With ``s(p)`` the first index of p's document
+
+        key j is visible  <=>  s(p) <= j <= p  and  (p - j < window  or  j - s(p) < sinks).
+
+    A query that sees nothing (padding, or ``Sq > Sk``) gets zeros and log-sum-exp -inf. ``return_lse`` adds the log-sum-exp
+    ``[B, heads, Sq]`` (fp32, not differentiable). k and v have to be finite everywhere, at padding too: a masked key has
+    weight zero, and zero times infinity is no number. On CUDA bf16 with head_dim 64 or 128 the kernels of
+    ``csrc/window_attn.cu`` and ``csrc/flash_attn_bwd.cu`` run, which visit only the key blocks that the rule reaches; other
+    types and sizes run :func:`sliding_window_reference`."""
+    _check_window_arguments(q, k, v, window, sinks, sequence_ids, scale)
+    if _kernel_eligible(q, k, v) and q.numel() and k.numel():
+        from .window_attn import window_attention
+
+        return window_attention(q, k, v, window=window, sinks=sinks, sequence_ids=sequence_ids, scale=scale, return_lse=return_lse)
+    return sliding_window_reference(q, k, v, window=window, sinks=sinks, sequence_ids=sequence_ids, scale=scale, return_lse=return_lse)
+
+
 # ------------------------------------------------------------------------------------------------ block primitives
 def attention_block_forward(q, k, v, *, q_positions, k_positions, q_sequence_ids=None, k_sequence_ids=None, scale=None):
     """One (query block, key block) attention WITHOUT autograd: returns ``(out, lse)`` with ``lse = -inf`` and

@@ -1,0 +1,115 @@
+"""Sliding-window attention with first tokens that stay visible: the kernels behind
+:func:`maltos_b200.ops.attention.sliding_window_attention` (``csrc/window_attn.cu`` forward, ``csrc/flash_attn_bwd.cu`` mode 4
+backward; the rule they share is ``csrc/window.cuh``)."""
+from __future__ import annotations
+
+import math
+
+import torch
+
+from . import _lib
+
+
+def _addressable(t: torch.Tensor) -> tuple[torch.Tensor, int, int]:
+    """``[B, S, h, D]`` as the kernels address it (heads contiguous inside a token, 16-byte aligned, token and batch strides
+    positive multiples of 8 elements), with the token and the batch stride; copied only where its strides do not fit."""
+    B, S, H, D = t.shape
+
+    def fits(stride: int, size: int) -> bool:
+        return size == 1 or (stride > 0 and stride % 8 == 0)
+
+    if t.stride(3) != 1 or (H > 1 and t.stride(2) != D) or not fits(t.stride(1), S) or not fits(t.stride(0), B) or t.data_ptr() % 16:
+        t = t.contiguous()
+    tstride = t.stride(1) if S > 1 else H * D
+    return t, tstride, t.stride(0) if B > 1 else S * tstride
+
+
+def document_bounds(sequence_ids: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
+    """First index and one past the last index of every token's document, int32 ``[B, S]`` each (padding: 2^31 - 1 and 0)."""
+    ids = sequence_ids.contiguous()
+    B, S = ids.shape
+    starts = torch.empty((2, B, S), dtype=torch.int32, device=ids.device)
+    with torch.cuda.device(ids.device):
+        _lib.check(_lib.lib().mb_document_bounds(_lib.ptr(ids), _lib.c_int(1 if ids.dtype == torch.int64 else 0), _lib.ptr(starts[0]),
+                                                 _lib.ptr(starts[1]), _lib.c_int(B), _lib.c_int(S), _lib.stream_ptr()), "mb_document_bounds")
+    return starts[0], starts[1]
+
+
+def window_forward(q, k, v, *, window: int, sinks: int, starts, scale: float):
+    """``(out [B, Sq, hq, D] bf16, lse [B, hq, Sq] fp32)``."""
+    B, Sq, Hq, D = q.shape
+    Sk, Hkv = k.shape[1], k.shape[2]
+    q, q_t, q_b = _addressable(q)
+    k, k_t, k_b = _addressable(k)
+    v, v_t, v_b = _addressable(v)
+    out = torch.empty((B, Sq, Hq, D), dtype=torch.bfloat16, device=q.device)
+    lse = torch.empty((B, Hq, Sq), dtype=torch.float32, device=q.device)
+    with torch.cuda.device(q.device):
+        _lib.check(_lib.lib().mb_window_attn_fwd(
+            _lib.ptr(q), _lib.c_ll(q_t), _lib.c_ll(q_b), _lib.ptr(k), _lib.c_ll(k_t), _lib.c_ll(k_b), _lib.ptr(v), _lib.c_ll(v_t),
+            _lib.c_ll(v_b), _lib.ptr(out), _lib.ptr(lse), _lib.ptr(starts), _lib.c_int(B), _lib.c_int(Sq), _lib.c_int(Sk),
+            _lib.c_int(Hq), _lib.c_int(Hkv), _lib.c_int(D), _lib.c_int(window), _lib.c_int(sinks), _lib.c_float(scale),
+            _lib.stream_ptr()), "mb_window_attn_fwd")
+    return out, lse
+
+
+def window_backward(q, k, v, out, lse, dout, *, window: int, sinks: int, starts, ends, scale: float):
+    """``(dq, dk, dv)`` in bf16; ``out`` and ``lse`` are the forward's."""
+    B, Sq, Hq, D = q.shape
+    Sk, Hkv = k.shape[1], k.shape[2]
+    q, q_t, q_b = _addressable(q)
+    k, k_t, k_b = _addressable(k)
+    v, v_t, v_b = _addressable(v)
+    dout, do_t, do_b = _addressable(dout.to(torch.bfloat16))
+    dq = torch.empty((B, Sq, Hq, D), dtype=torch.bfloat16, device=q.device)
+    dk = torch.empty((B, Sk, Hkv, D), dtype=torch.bfloat16, device=q.device)
+    dv = torch.empty_like(dk)
+    L = _lib.lib()
+    L.mb_window_attn_bwd_scratch_words.restype = _lib.c_ll
+    with torch.cuda.device(q.device):
+        words = int(L.mb_window_attn_bwd_scratch_words(_lib.c_int(B), _lib.c_int(Sq), _lib.c_int(Sk), _lib.c_int(Hq), _lib.c_int(Hkv),
+                                                       _lib.c_int(D)))
+        scratch = torch.empty((words,), dtype=torch.float32, device=q.device)
+        _lib.check(L.mb_window_attn_bwd(
+            _lib.ptr(q), _lib.c_ll(q_t), _lib.c_ll(q_b), _lib.ptr(k), _lib.c_ll(k_t), _lib.c_ll(k_b), _lib.ptr(v), _lib.c_ll(v_t),
+            _lib.c_ll(v_b), _lib.ptr(out), _lib.ptr(dout), _lib.c_ll(do_t), _lib.c_ll(do_b), _lib.ptr(lse), _lib.ptr(dq), _lib.ptr(dk),
+            _lib.ptr(dv), _lib.ptr(starts), _lib.ptr(ends), _lib.ptr(scratch), _lib.c_int(B), _lib.c_int(Sq), _lib.c_int(Sk),
+            _lib.c_int(Hq), _lib.c_int(Hkv), _lib.c_int(D), _lib.c_int(window), _lib.c_int(sinks), _lib.c_float(scale),
+            _lib.stream_ptr()), "mb_window_attn_bwd")
+    return dq, dk, dv
+
+
+class _WindowAttention(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, v, window, sinks, starts, ends, scale):
+        # As in dense flash attention: under activation checkpointing the recompute replays (out, lse) of the first pass.
+        from maltos_b200.utils.activation_checkpoint import current_checkpoint_stash
+
+        stash = current_checkpoint_stash()
+        kept = stash.replay() if stash is not None and stash.replaying else None
+        if kept is not None and kept[0].shape == q.shape:
+            out, lse = kept
+        else:
+            out, lse = window_forward(q, k, v, window=window, sinks=sinks, starts=starts, scale=scale)
+            if stash is not None and not stash.replaying:
+                stash.record((out, lse))
+        ctx.save_for_backward(q, k, v, out, lse, starts, ends)
+        ctx.window, ctx.sinks, ctx.scale = window, sinks, scale
+        ctx.mark_non_differentiable(lse)
+        return out, lse
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dout, _dlse):
+        q, k, v, out, lse, starts, ends = ctx.saved_tensors
+        dq, dk, dv = window_backward(q, k, v, out, lse, dout, window=ctx.window, sinks=ctx.sinks, starts=starts, ends=ends, scale=ctx.scale)
+        return dq, dk, dv, None, None, None, None, None
+
+
+def window_attention(q, k, v, *, window: int, sinks: int = 0, sequence_ids=None, scale: float | None = None, return_lse: bool = False):
+    """The kernels' differentiable entry: bf16, head_dim 64 or 128, sizes above zero, arguments as checked by the public one."""
+    Sk = k.shape[1]
+    starts, ends = document_bounds(sequence_ids) if sequence_ids is not None else (None, None)
+    scale = float(scale) if scale is not None else 1.0 / math.sqrt(q.shape[3])
+    out, lse = _WindowAttention.apply(q, k, v, min(window, Sk), min(sinks, Sk), starts, ends, scale)
+    return (out, lse) if return_lse else out
