@@ -6,6 +6,7 @@ never loaded and the ops use their PyTorch fp32 restatements, which are also the
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import os
 import threading
@@ -100,6 +101,31 @@ class _RangedLibrary:
         return wrapped
 
 
+#: Argument kinds of entry points whose callers hand over plain numbers (p pointer, l long long, i int, f float): with these known,
+#: ctypes converts in C, which for a call of twenty arguments is several microseconds less than an object per argument.
+_PROTOTYPES = {
+    "mb_document_bounds": "pippiip",
+    "mb_window_attn_fwd": "pllpllpllppp" "iiiiiiii" "fp",
+    "mb_window_attn_bwd_scratch_words": "iiiiii",
+    "mb_window_attn_bwd": "pllpllpll" "ppll" "pppp" "ppp" "iiiiiiii" "fp",
+    "mb_embedding_fwd": "pippilil" "fp",
+    "mb_embedding_bwd_scratch_words": "li",
+    "mb_embedding_bwd": "pippp" "ilill" "fp",
+    "mb_block_norm_fwd": "pppppi" "pppp" "ili" "ffp",
+    "mb_block_norm_bwd_parts": "l",
+    "mb_block_norm_bwd": "ppppppp" "i" "ppppppp" "pp" "ili" "fp",
+}
+_KINDS = {"p": c_void_p, "l": c_ll, "i": c_int, "f": c_float}
+
+
+def _declare(handle) -> None:
+    for name, kinds in _PROTOTYPES.items():
+        fn = getattr(handle, name)
+        fn.argtypes = [_KINDS[k] for k in kinds]
+        if name.endswith("_scratch_words"):
+            fn.restype = c_ll
+
+
 def library_path() -> Path:
     return _LIB_PATH
 
@@ -135,6 +161,7 @@ def lib() -> ctypes.CDLL:
             raise KernelLibraryError(f"cannot load {_LIB_PATH}: {exc}") from exc
         handle.mb_last_error.restype = ctypes.c_char_p
         handle.mb_launch_count.restype = ctypes.c_ulonglong
+        _declare(handle)
         _lib = _RangedLibrary(handle) if nvtx_enabled() else handle
     return _lib
 
@@ -146,6 +173,25 @@ def use_kernels(*tensors: torch.Tensor) -> bool:
 
 def stream_ptr() -> c_void_p:
     return c_void_p(torch.cuda.current_stream().cuda_stream)
+
+
+_NO_GUARD = contextlib.nullcontext()
+
+
+def on_device_of(t: torch.Tensor):
+    """Context in which ``t``'s device is the current one: launches, streams and the status word are per current device."""
+    index = t.get_device()
+    return _NO_GUARD if index == torch.cuda.current_device() else torch.cuda.device(index)
+
+
+def stream_of(t: torch.Tensor) -> int:
+    """The current stream of ``t``'s device, as a number for an entry point of ``_PROTOTYPES``."""
+    return torch._C._cuda_getCurrentRawStream(t.get_device())
+
+
+def address(t: torch.Tensor | None) -> int | None:
+    """Data pointer for an entry point of ``_PROTOTYPES`` (None: null)."""
+    return None if t is None else t.data_ptr()
 
 
 def ptr(t: torch.Tensor | None) -> c_void_p:

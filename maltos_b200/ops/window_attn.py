@@ -14,25 +14,27 @@ def _addressable(t: torch.Tensor) -> tuple[torch.Tensor, int, int]:
     """``[B, S, h, D]`` as the kernels address it (heads contiguous inside a token, 16-byte aligned, token and batch strides
     positive multiples of 8 elements), with the token and the batch stride; copied only where its strides do not fit."""
     B, S, H, D = t.shape
-
-    def fits(stride: int, size: int) -> bool:
-        return size == 1 or (stride > 0 and stride % 8 == 0)
-
-    if t.stride(3) != 1 or (H > 1 and t.stride(2) != D) or not fits(t.stride(1), S) or not fits(t.stride(0), B) or t.data_ptr() % 16:
+    sb, st, sh, sd = t.stride()
+    if not (sd == 1 and (sh == D or H == 1) and (S == 1 or (st > 0 and st % 8 == 0)) and (B == 1 or (sb > 0 and sb % 8 == 0))
+            and t.data_ptr() % 16 == 0):
         t = t.contiguous()
-    tstride = t.stride(1) if S > 1 else H * D
-    return t, tstride, t.stride(0) if B > 1 else S * tstride
+        if t.data_ptr() % 16:
+            t = t.clone()
+        sb, st = S * H * D, H * D
+    if S == 1:
+        st = H * D
+    return t, st, S * st if B == 1 else sb
 
 
 def document_bounds(sequence_ids: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
     """First index and one past the last index of every token's document, int32 ``[B, S]`` each (padding: 2^31 - 1 and 0)."""
     ids = sequence_ids.contiguous()
     B, S = ids.shape
-    starts = torch.empty((2, B, S), dtype=torch.int32, device=ids.device)
-    with torch.cuda.device(ids.device):
-        _lib.check(_lib.lib().mb_document_bounds(_lib.ptr(ids), _lib.c_int(1 if ids.dtype == torch.int64 else 0), _lib.ptr(starts[0]),
-                                                 _lib.ptr(starts[1]), _lib.c_int(B), _lib.c_int(S), _lib.stream_ptr()), "mb_document_bounds")
-    return starts[0], starts[1]
+    starts, ends = torch.empty((2, B, S), dtype=torch.int32, device=ids.device)
+    with _lib.on_device_of(ids):
+        _lib.check(_lib.lib().mb_document_bounds(ids.data_ptr(), 1 if ids.dtype == torch.int64 else 0, starts.data_ptr(), ends.data_ptr(),
+                                                 B, S, _lib.stream_of(ids)), "mb_document_bounds")
+    return starts, ends
 
 
 def window_forward(q, k, v, *, window: int, sinks: int, starts, scale: float):
@@ -44,12 +46,10 @@ def window_forward(q, k, v, *, window: int, sinks: int, starts, scale: float):
     v, v_t, v_b = _addressable(v)
     out = torch.empty((B, Sq, Hq, D), dtype=torch.bfloat16, device=q.device)
     lse = torch.empty((B, Hq, Sq), dtype=torch.float32, device=q.device)
-    with torch.cuda.device(q.device):
-        _lib.check(_lib.lib().mb_window_attn_fwd(
-            _lib.ptr(q), _lib.c_ll(q_t), _lib.c_ll(q_b), _lib.ptr(k), _lib.c_ll(k_t), _lib.c_ll(k_b), _lib.ptr(v), _lib.c_ll(v_t),
-            _lib.c_ll(v_b), _lib.ptr(out), _lib.ptr(lse), _lib.ptr(starts), _lib.c_int(B), _lib.c_int(Sq), _lib.c_int(Sk),
-            _lib.c_int(Hq), _lib.c_int(Hkv), _lib.c_int(D), _lib.c_int(window), _lib.c_int(sinks), _lib.c_float(scale),
-            _lib.stream_ptr()), "mb_window_attn_fwd")
+    with _lib.on_device_of(q):
+        _lib.check(_lib.lib().mb_window_attn_fwd(q.data_ptr(), q_t, q_b, k.data_ptr(), k_t, k_b, v.data_ptr(), v_t, v_b, out.data_ptr(),
+                                                 lse.data_ptr(), _lib.address(starts), B, Sq, Sk, Hq, Hkv, D, window, sinks, scale,
+                                                 _lib.stream_of(q)), "mb_window_attn_fwd")
     return out, lse
 
 
@@ -63,19 +63,14 @@ def window_backward(q, k, v, out, lse, dout, *, window: int, sinks: int, starts,
     dout, do_t, do_b = _addressable(dout.to(torch.bfloat16))
     dq = torch.empty((B, Sq, Hq, D), dtype=torch.bfloat16, device=q.device)
     dk = torch.empty((B, Sk, Hkv, D), dtype=torch.bfloat16, device=q.device)
-    dv = torch.empty_like(dk)
+    dv = torch.empty((B, Sk, Hkv, D), dtype=torch.bfloat16, device=q.device)
     L = _lib.lib()
-    L.mb_window_attn_bwd_scratch_words.restype = _lib.c_ll
-    with torch.cuda.device(q.device):
-        words = int(L.mb_window_attn_bwd_scratch_words(_lib.c_int(B), _lib.c_int(Sq), _lib.c_int(Sk), _lib.c_int(Hq), _lib.c_int(Hkv),
-                                                       _lib.c_int(D)))
-        scratch = torch.empty((words,), dtype=torch.float32, device=q.device)
-        _lib.check(L.mb_window_attn_bwd(
-            _lib.ptr(q), _lib.c_ll(q_t), _lib.c_ll(q_b), _lib.ptr(k), _lib.c_ll(k_t), _lib.c_ll(k_b), _lib.ptr(v), _lib.c_ll(v_t),
-            _lib.c_ll(v_b), _lib.ptr(out), _lib.ptr(dout), _lib.c_ll(do_t), _lib.c_ll(do_b), _lib.ptr(lse), _lib.ptr(dq), _lib.ptr(dk),
-            _lib.ptr(dv), _lib.ptr(starts), _lib.ptr(ends), _lib.ptr(scratch), _lib.c_int(B), _lib.c_int(Sq), _lib.c_int(Sk),
-            _lib.c_int(Hq), _lib.c_int(Hkv), _lib.c_int(D), _lib.c_int(window), _lib.c_int(sinks), _lib.c_float(scale),
-            _lib.stream_ptr()), "mb_window_attn_bwd")
+    with _lib.on_device_of(q):
+        scratch = torch.empty((L.mb_window_attn_bwd_scratch_words(B, Sq, Sk, Hq, Hkv, D),), dtype=torch.float32, device=q.device)
+        _lib.check(L.mb_window_attn_bwd(q.data_ptr(), q_t, q_b, k.data_ptr(), k_t, k_b, v.data_ptr(), v_t, v_b, out.data_ptr(),
+                                        dout.data_ptr(), do_t, do_b, lse.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(),
+                                        _lib.address(starts), _lib.address(ends), scratch.data_ptr(), B, Sq, Sk, Hq, Hkv, D, window, sinks,
+                                        scale, _lib.stream_of(q)), "mb_window_attn_bwd")
     return dq, dk, dv
 
 
@@ -111,5 +106,9 @@ def window_attention(q, k, v, *, window: int, sinks: int = 0, sequence_ids=None,
     Sk = k.shape[1]
     starts, ends = document_bounds(sequence_ids) if sequence_ids is not None else (None, None)
     scale = float(scale) if scale is not None else 1.0 / math.sqrt(q.shape[3])
-    out, lse = _WindowAttention.apply(q, k, v, min(window, Sk), min(sinks, Sk), starts, ends, scale)
+    window, sinks = min(window, Sk), min(sinks, Sk)
+    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
+        out, lse = _WindowAttention.apply(q, k, v, window, sinks, starts, ends, scale)
+    else:
+        out, lse = window_forward(q, k, v, window=window, sinks=sinks, starts=starts, scale=scale)
     return (out, lse) if return_lse else out

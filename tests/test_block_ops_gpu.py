@@ -1,0 +1,270 @@
+"""Scaled embedding and block norm kernels against their formulas in 64 bits, element by element. Bounds count roundings: u is half
+a step of the type (eps / 2); fp32 arithmetic is allowed 2^-19 of the sum of magnitudes (sums of up to 16384 terms that are
+added in trees, a handful of products around them)."""
+import pytest
+import torch
+
+from maltos_b200.ops import _lib
+from maltos_b200.ops.embedding import ScaledEmbedding, embedding
+from maltos_b200.ops.norm import add_rms_norm, block_norm
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda"
+F32 = 2.0 ** -19
+
+
+def _gen(seed):
+    return torch.Generator(device=DEV).manual_seed(seed)
+
+
+def _near(name, got, value, bound):
+    assert got.shape == value.shape and torch.isfinite(got).all(), name
+    # below the smallest normal number the steps stop shrinking: rounding is off by half of the smallest step, whatever the value
+    # (fp16: 2^-14 * 2^-11 = 2^-25)
+    info = torch.finfo(got.dtype)
+    over = (got.double() - value).abs() - bound - info.smallest_normal * info.eps / 2
+    assert over.max().item() <= 0, f"{name}: {over.max().item():.3g} over its bound"
+
+
+# ------------------------------------------------------------------------------------------------ embedding
+def _embedding_case(ids, rows, H, dtype, scale, pad, seed=0):
+    u = torch.finfo(dtype).eps / 2
+    w = torch.randn(rows, H, device=DEV, generator=_gen(seed)).to(dtype).requires_grad_()
+    out = embedding(ids, w, scale=scale, padding_idx=pad)
+    dout = torch.randn(out.shape, device=DEV, generator=_gen(seed + 1)).to(dtype)
+    (dw,) = torch.autograd.grad(out, w, dout)
+    _lib.fetch_status()
+    want = w.detach()[ids].double() * scale
+    _near("out", out.detach(), want, (u + 2.0 ** -23) * want.abs())
+    flat, d = ids.reshape(-1).long(), dout.reshape(-1, H).double() * scale
+    if pad is not None:
+        d = d * (flat != pad).unsqueeze(1)
+    value = torch.zeros(rows, H, dtype=torch.float64, device=DEV).index_add_(0, flat, d)
+    mags = torch.zeros_like(value).index_add_(0, flat, d.abs())
+    count = torch.bincount(flat, minlength=rows).double().unsqueeze(1)
+    # a run of n tokens is summed in fp32 one after the other, in pieces of 32: at most n roundings of 2^-24
+    _near("dweight", dw, value, u * value.abs() + 2.0 ** -24 * (count + 2) * (1 + u) * mags)
+    return out.detach(), dw
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("rows,H,n", [(1, 8, 1), (1, 8, 100), (5, 64, 33), (300, 40, 31), (256, 8, 64), (255, 24, 65), (40000, 72, 700), (70000, 16, 5000),
+                                      (97, 4096, 260)])
+def test_embedding_sizes(rows, H, n, dtype):
+    ids = torch.randint(0, rows, (n,), device=DEV, generator=_gen(n))
+    _embedding_case(ids, rows, H, dtype, 1.7, None)
+
+
+@pytest.mark.parametrize("H", [1, 3, 7, 12, 100])
+def test_embedding_odd_hidden_sizes(H):
+    for dtype in (torch.bfloat16, torch.float32):
+        _embedding_case(torch.randint(0, 19, (77,), device=DEV, generator=_gen(H)), 19, H, dtype, 0.3, 4)
+
+
+@pytest.mark.parametrize("pad", [None, 6])
+def test_embedding_frequent_tokens(pad):
+    """Runs that end inside a chunk, at its border, and that cross many chunks."""
+    for lengths in ([32, 32, 64], [31, 33, 1, 1, 30], [1000, 5, 2000], [33] * 20, [4000]):
+        ids = torch.cat([torch.full((n,), 3 * i, dtype=torch.int64) for i, n in enumerate(lengths)])
+        ids = ids[torch.randperm(ids.numel(), generator=torch.Generator().manual_seed(len(lengths)))].to(DEV)
+        _embedding_case(ids, 3 * len(lengths) + 7, 136, torch.bfloat16, 1.0, pad)
+
+
+def test_embedding_many_tokens_and_narrow_ids():
+    ids = (torch.rand(3, 30011, device=DEV, generator=_gen(5)) ** 4 * 5000).long()
+    a = _embedding_case(ids, 5000, 64, torch.float32, 2.0, 0)
+    b = _embedding_case(ids.to(torch.int32), 5000, 64, torch.float32, 2.0, 0)
+    assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
+
+
+def test_embedding_ids_outside_the_table():
+    w = torch.randn(10, 16, device=DEV).bfloat16().requires_grad_()
+    ids = torch.tensor([1, 10, 2, -1, 2 ** 40, 2], device=DEV)
+    _lib.fetch_status(raise_on_error=False)
+    out = embedding(ids, w, scale=2.0)
+    (dw,) = torch.autograd.grad(out, w, torch.ones_like(out))
+    with pytest.raises(_lib.DeviceStatusError, match="index out of bounds"):
+        _lib.fetch_status()
+    assert out[[1, 3, 4]].abs().max() == 0
+    want = torch.zeros(10, device=DEV).index_add_(0, torch.tensor([1, 2, 2], device=DEV), torch.tensor([2.0, 2.0, 2.0], device=DEV))
+    assert torch.equal(dw.float(), want.unsqueeze(1).expand(10, 16))
+
+
+def test_embedding_strides_streams_and_graphs():
+    w = torch.randn(50, 96, device=DEV).bfloat16()
+    leaf = w.t().contiguous().t().requires_grad_()                    # a transposed table is copied
+    ids = torch.randint(0, 50, (40, 6), device=DEV)[:, ::2]
+    out = embedding(ids, leaf, scale=3.0)
+    assert torch.equal(out, (w[ids].float() * 3).bfloat16())
+    d = torch.randn(96, device=DEV).bfloat16().expand(40, 3, 96)      # a broadcast gradient
+    (want,) = torch.autograd.grad(out, leaf, d)
+    del out                                                           # no eager graph of the leaf lives during the capture
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        (got,) = torch.autograd.grad(embedding(ids, leaf, scale=3.0), leaf, d)
+    torch.cuda.current_stream().wait_stream(side)
+    assert torch.equal(got, want)
+    static, graph = ids.clone(), torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        res = embedding(static, leaf, scale=3.0)
+        (held,) = torch.autograd.grad(res, leaf, d)
+    other = torch.randint(0, 50, ids.shape, device=DEV)
+    for t in (other, ids):
+        static.copy_(t)
+        graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(held, want)
+    _lib.fetch_status()
+
+
+def test_scaled_embedding_module_keeps_its_parameter():
+    m = ScaledEmbedding(64, 32, 5.0).to(DEV, torch.bfloat16)
+    ids = torch.randint(0, 64, (2, 9), device=DEV)
+    m(ids).float().sum().backward()
+    assert m.weight.grad.shape == m.weight.shape and torch.equal(m.weight.grad.float().sum(), torch.tensor(5.0 * 18 * 32, device=DEV))
+
+
+# ------------------------------------------------------------------------------------------------ block norm
+def _block_norm_case(shape, dtype, after, before, gate, scale, eps=1e-5, seed=0, only=None):
+    u, H = torch.finfo(dtype).eps / 2, shape[-1]
+    g = _gen(seed)
+    mk = lambda *s: torch.randn(*s, device=DEV, generator=g).to(dtype).requires_grad_()   # noqa: E731
+    x, r, w1, w2 = mk(*shape), mk(*shape), mk(H), mk(H)
+    w1, w2 = w1 if after else None, w2 if before else None
+    gt = None if gate is None else mk(*(shape if gate == "element" else (H,)))
+    res = block_norm(x, r, w1, w2, gate=gt, scale=scale, eps=eps)
+    y, h = res if before else (None, res)
+    dh, dy = (torch.randn(shape, device=DEV, generator=g).to(dtype) for _ in range(2))
+    outs, douts = [h], [dh]
+    if before:
+        outs, douts = ([y, h], [dy, dh]) if only is None else ([y], [dy]) if only == "y" else ([h], [dh])
+        if only == "y":
+            dh = torch.zeros_like(dh)
+        elif only == "h":
+            dy = torch.zeros_like(dy)
+    used = {n: t for n, t in (("x", x), ("r", r), ("w1", w1), ("w2", w2), ("g", gt)) if t is not None}
+    grads = dict(zip(used, torch.autograd.grad(outs, list(used.values()), douts, allow_unused=True)))
+    _lib.fetch_status()
+
+    d = lambda t: None if t is None else t.detach().double()                              # noqa: E731
+    X, R, W1, W2, G, DH, DY = (d(t) for t in (x, r, w1, w2, gt, dh, dy))
+    mean = lambda t: t.mean(-1, keepdim=True)                                             # noqa: E731
+    R1 = torch.rsqrt(mean(X * X) + eps) if after else 1.0
+    xn = X * R1
+    U = W1 * xn if after else X
+    ga = 1.0 if gate is None else G
+    Hd = R + scale * ga * U
+    mag = R.abs() + (scale * ga * U).abs()
+    e_h = F32 * mag                                          # h before its rounding
+    _near("h", h.detach(), Hd, e_h + u * (Hd.abs() + e_h))
+    dt, e_dt = DH, 0.0
+    if before:
+        R2 = torch.rsqrt(mean(Hd * Hd) + eps)
+        hn = Hd * R2
+        e_r2 = R2 ** 3 * mean(Hd.abs() * e_h) + F32 * R2     # relative error of the root's argument, halved, and fp32
+        e_y = (W2 * R2).abs() * e_h + (W2 * Hd).abs() * e_r2 + F32 * (W2 * hn).abs()
+        _near("y", y.detach(), W2 * hn, e_y + u * ((W2 * hn).abs() + e_y))
+        # the backward reads the rounded h
+        e_hn = R2 * (e_h + u * (Hd.abs() + e_h)) + Hd.abs() * e_r2 + F32 * hn.abs()
+        dn2 = DY * W2
+        c2, e_c2 = mean(dn2 * hn), mean(dn2.abs() * e_hn) + F32 * mean((dn2 * hn).abs())
+        dt = DH + R2 * (dn2 - hn * c2)
+        part = dn2.abs() + (hn * c2).abs()
+        e_dt = R2 * (e_hn * (c2.abs() + e_c2) + hn.abs() * e_c2) + e_r2 * part + F32 * (DH.abs() + R2 * part)
+        if grads["w2"] is not None:
+            total = lambda t: t.reshape(-1, H).sum(0)                                     # noqa: E731
+            _near("dw2", grads["w2"], total(DY * hn), total(DY.abs() * e_hn) + F32 * total((DY * hn).abs()) + u * total(DY * hn).abs() * 1.01)
+    total = lambda t: t.reshape(-1, H).sum(0)                                             # noqa: E731
+    _near("dresidual", grads["r"], dt, e_dt + u * (dt.abs() + e_dt))
+    sd, e_sd = scale * dt, abs(scale) * e_dt
+    du, e_du = sd * ga, abs(scale) * e_dt * (ga.abs() if gate else 1.0)
+    if gate is not None:
+        dg, e_dg = sd * U, e_sd * U.abs() + F32 * (sd * U).abs()
+        if gate == "channel":
+            dg, e_dg = total(dg), total(e_dg) + F32 * total(dg.abs())
+        _near("dgate", grads["g"], dg, e_dg + u * (dg.abs() + e_dg))
+    if after:
+        dw, e_dw = total(du * xn), total(e_du * xn.abs()) + 2 * F32 * total((du * xn).abs())
+        _near("dw1", grads["w1"], dw, e_dw + u * (dw.abs() + e_dw))
+        dn1, e_dn1 = du * W1, e_du * W1.abs()
+        # c1 comes from the means of its two parts
+        parts = mean((scale * ga * W1 * xn).abs() * (DH.abs() + ((R2 * (dn2.abs() + (hn * c2).abs())) if before else 0.0)))
+        c1, e_c1 = mean(dn1 * xn), mean(e_dn1 * xn.abs()) + 2 * F32 * parts
+        if before:      # the rounded h also enters the second part, times c2
+            e_c1 = e_c1 + mean((scale * ga * W1 * xn).abs() * R2 * (e_hn * c2.abs() + hn.abs() * e_c2))
+        dx = R1 * (dn1 - xn * c1)
+        e_dx = R1 * (e_dn1 + xn.abs() * e_c1) + 2 * F32 * R1 * (dn1.abs() + (xn * c1).abs())
+    else:
+        dx, e_dx = du, e_du + F32 * du.abs()
+    _near("dx", grads["x"], dx, e_dx + u * (dx.abs() + e_dx))
+    return res, grads
+
+
+@pytest.mark.parametrize("H", [8, 64, 264, 1024, 1032, 4096, 5120, 8192, 8200, 16384])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+def test_block_norm_hidden_sizes(H, dtype):
+    _block_norm_case((37, H), dtype, True, True, "channel", 0.5)
+    _block_norm_case((5, H), dtype, True, True, "element", 1.0)
+
+
+@pytest.mark.parametrize("rows", [1, 2, 3, 147, 297, 1000])
+def test_block_norm_rows(rows):
+    _block_norm_case((rows, 72), torch.bfloat16, True, True, None, 1.0)
+    _block_norm_case((rows, 2048), torch.float32, True, False, "channel", 0.1)
+
+
+@pytest.mark.parametrize("gate", [None, "channel", "element"])
+@pytest.mark.parametrize("after,before", [(True, True), (True, False), (False, True), (False, False)])
+@pytest.mark.parametrize("only", [None, "y", "h"])
+def test_block_norm_parts(gate, after, before, only):
+    _block_norm_case((3, 50, 520), torch.bfloat16, after, before, gate, -0.7, only=only)
+
+
+def test_block_norm_tiny_and_huge_rows():
+    x = torch.zeros(4, 64, device=DEV).bfloat16().requires_grad_()
+    x.data[1], x.data[2] = 1e-20, 1e18
+    w = torch.ones(64, device=DEV).bfloat16()
+    y, h = block_norm(x, torch.zeros_like(x), w, w, eps=1e-6)
+    (dx,) = torch.autograd.grad(y, x, torch.ones_like(y))
+    assert torch.isfinite(y).all() and torch.isfinite(h).all() and torch.isfinite(dx).all()
+    assert h[0].abs().max() == 0 and torch.equal(h[2], torch.ones_like(h[2]))
+
+
+def test_block_norm_agrees_with_add_rms_norm():
+    x, r, w = (torch.randn(*s, device=DEV, generator=_gen(3)).bfloat16() for s in ((40, 512), (40, 512), (512,)))
+    y, h = block_norm(x, r, None, w, eps=1e-5)
+    y0, h0 = add_rms_norm(x, r, w, 1e-5)
+    assert torch.equal(h, h0)
+    assert (y.float() - y0.float()).abs().max() <= 2 ** -7 * y0.float().abs().max()      # that one norms the rounded sum
+
+
+def test_block_norm_strides_streams_graphs_and_bits():
+    base = torch.randn(60, 2, 328, device=DEV, generator=_gen(4)).bfloat16()
+    x, r = base[:, 0, 4:324].requires_grad_(), base[:, 1, :320].requires_grad_()           # strided, not 16-byte aligned
+    w1, w2 = (torch.randn(321, device=DEV).bfloat16()[1:].requires_grad_() for _ in range(2))
+    dy = torch.randn(320, device=DEV).bfloat16().expand(60, 320)
+
+    def step():
+        y, h = block_norm(x, r, w1, w2, scale=0.5)
+        return (y, h, *torch.autograd.grad(y, (x, r, w1, w2), dy))
+
+    want = [t.detach().clone() for t in step()]
+    dense = [t.detach().clone().requires_grad_() for t in (x, r, w1, w2)]
+    y, h = block_norm(dense[0], dense[1], dense[2], dense[3], scale=0.5)
+    assert torch.equal(y, want[0]) and torch.equal(h, want[1])
+    assert all(torch.equal(a, b) for a, b in zip(torch.autograd.grad(y, dense, dy), want[2:]))
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        got = step()
+    torch.cuda.current_stream().wait_stream(side)
+    assert all(torch.equal(a, b) for a, b in zip(want, got))
+    del got, y, h
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        held = step()
+    graph.replay()
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(want, held))
+    _lib.fetch_status()
