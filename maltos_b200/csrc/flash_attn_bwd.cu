@@ -56,6 +56,7 @@ struct FlashBwdArgs {
   float* dv_tmp;
   long long plane;          // elements of a plane (mode 4)
   WindowRule rule;          // mode 4
+  const void* out_lo;       // mode 4: what the rounding of the output left
   int dbg;                  // probe builds only: bit 0 skip the S/dP UMMAs, bit 1 skip the accumulation UMMAs, bit 2 skip the arithmetic
 };
 
@@ -83,9 +84,10 @@ __device__ __forceinline__ float bw_exp2(float x) {
 }
 
 // ---------------------------------------------------------------------------------------------- preprocessing
-// One warp per (batch, head, query row): delta = sum_d out * dout; lse2 = lse * log2(e).
-template <int D>
-__global__ void flash_bwd_prep_kernel(const __nv_bfloat16* __restrict__ out, const __nv_bfloat16* __restrict__ dout,
+// One warp per (batch, head, query row): delta = sum_d out * dout; lse2 = lse * log2(e). LO (mode 4): out comes with what its
+// rounding left, and the statistics are in the exp2 domain already.
+template <int D, bool LO>
+__global__ void flash_bwd_prep_kernel(const __nv_bfloat16* __restrict__ out, const __nv_bfloat16* __restrict__ out_lo, const __nv_bfloat16* __restrict__ dout,
                                       long long o_tstride, long long o_bstride, long long do_tstride, long long do_bstride,
                                       const float* __restrict__ lse, float* __restrict__ lse2, float* __restrict__ delta,
                                       int B, int Sq, int Hq, int Sq_pad) {
@@ -99,18 +101,24 @@ __global__ void flash_bwd_prep_kernel(const __nv_bfloat16* __restrict__ out, con
   float acc = 0.f, l2 = INFINITY;
   if (qi < Sq) {
     constexpr int PER = D / 32;   // 2 or 4 bf16 per lane
-    const __nv_bfloat16* po = out + b * o_bstride + qi * o_tstride + static_cast<long long>(h) * D + lane * PER;
+    const long long o_at = b * o_bstride + qi * o_tstride + static_cast<long long>(h) * D + lane * PER;
+    const __nv_bfloat16* po = out + o_at;
     const __nv_bfloat16* pd = dout + b * do_bstride + qi * do_tstride + static_cast<long long>(h) * D + lane * PER;
 #pragma unroll
     for (int i = 0; i < PER; i += 2) {
       const __nv_bfloat162 a = *reinterpret_cast<const __nv_bfloat162*>(po + i);
       const __nv_bfloat162 g = *reinterpret_cast<const __nv_bfloat162*>(pd + i);
-      acc += __bfloat162float(a.x) * __bfloat162float(g.x) + __bfloat162float(a.y) * __bfloat162float(g.y);
+      float ax = __bfloat162float(a.x), ay = __bfloat162float(a.y);
+      if (LO) {
+        const __nv_bfloat162 l = *reinterpret_cast<const __nv_bfloat162*>(out_lo + o_at + i);
+        ax += __bfloat162float(l.x), ay += __bfloat162float(l.y);
+      }
+      acc += ax * __bfloat162float(g.x) + ay * __bfloat162float(g.y);
     }
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) acc += __shfl_xor_sync(0xffffffffu, acc, o);
     const float l = lse[(static_cast<long long>(b) * Hq + h) * Sq + qi];
-    l2 = (l == -INFINITY) ? INFINITY : l * kBwLog2e;
+    l2 = (l == -INFINITY) ? INFINITY : LO ? l : l * kBwLog2e;
   }
   if (lane == 0) {
     lse2[warp_global] = l2;
@@ -809,6 +817,11 @@ flash_bwd_dq_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_consta
       my_seq = p.qseq[at];
     }
     const float scale_log2 = p.scale_log2;
+    // Mode 4 takes the forward's own rounded weights, so that the terms of dS cancel as exactly as there: weights relative to a
+    // whole power of two (the forward's differ from it by another such factor), rounded to bf16, times what is left of 2^-lse.
+    const float my_shift = MODE == 4 ? floorf(my_lse) : my_lse;
+    const float my_factor = MODE == 4 && my_lse != INFINITY ? bw_exp2(my_shift - my_lse) : 0.f;
+    const float my_offset = my_delta * my_factor;
     bool ok = true;
     for (int j = 0; j < n_blocks; ++j) {
       const int s = j & 1;
@@ -834,7 +847,7 @@ flash_bwd_dq_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_consta
       if (causal) need_mask = need_mask || (j * kDqKeys + kDqKeys - 1 > q0 + causal_off);
       float pr[32];
 #pragma unroll
-      for (int c = 0; c < 32; ++c) pr[c] = bw_exp2(fmaf(__uint_as_float(sc[c]), scale_log2, -my_lse));
+      for (int c = 0; c < 32; ++c) pr[c] = bw_exp2(fmaf(__uint_as_float(sc[c]), scale_log2, -my_shift));
       if (MODE == 4) {
         if (need_mask) {
           const uint32_t seen = window_bits(wr, key0);
@@ -866,8 +879,17 @@ flash_bwd_dq_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_consta
       }
       uint32_t dsp[16];
 #pragma unroll
-      for (int c = 0; c < 32; c += 2)
-        dsp[c >> 1] = pack_bf16x2(pr[c] * (__uint_as_float(dp[c]) - my_delta), pr[c + 1] * (__uint_as_float(dp[c + 1]) - my_delta));
+      for (int c = 0; c < 32; c += 2) {
+        if (MODE == 4) {
+          const uint32_t w = pack_bf16x2(pr[c], pr[c + 1]);
+          const uint64_t t = fma_f32x2(f32x2(__uint_as_float(dp[c]), __uint_as_float(dp[c + 1])), f32x2(my_factor, my_factor), f32x2(-my_offset, -my_offset));
+          float a, b;
+          f32x2_split(mul_f32x2(bf16x2_as_f32x2(w), t), a, b);
+          dsp[c >> 1] = pack_bf16x2(a, b);
+        } else {
+          dsp[c >> 1] = pack_bf16x2(pr[c] * (__uint_as_float(dp[c]) - my_delta), pr[c + 1] * (__uint_as_float(dp[c + 1]) - my_delta));
+        }
+      }
       MB_PROBE(warp == 2 && lane == 0, j, 10);
       tmem_st_32x32b_x16(t_s, dsp);               // dS over the first half of this thread's own score columns
       tmem_st_wait();
@@ -941,8 +963,8 @@ static int launch_flash_bwd(const void* q, long long q_tstride, long long q_bstr
   {
     const long long threads = n_rows * 32;
     const int block = 256;
-    flash_bwd_prep_kernel<D><<<static_cast<unsigned>((threads + block - 1) / block), block, 0, stream>>>(
-        static_cast<const __nv_bfloat16*>(out), static_cast<const __nv_bfloat16*>(dout), o_tstride, o_bstride, do_tstride,
+    flash_bwd_prep_kernel<D, MODE == 4><<<static_cast<unsigned>((threads + block - 1) / block), block, 0, stream>>>(
+        static_cast<const __nv_bfloat16*>(out), static_cast<const __nv_bfloat16*>(a.out_lo), static_cast<const __nv_bfloat16*>(dout), o_tstride, o_bstride, do_tstride,
         do_bstride, lse, lse2, delta, a.B, a.Sq, a.Hq, a.Sq_pad);
     count_launch();
   }
@@ -1099,17 +1121,17 @@ MB_API long long mb_window_attn_bwd_scratch_words(int B, int Sq, int Sk, int Hq,
   return words;
 }
 
-// Backward of mb_window_attn_fwd. q, k, v, out, dout as there (dout with strides of its own), dq / dk / dv bf16 contiguous.
+// Backward of mb_window_attn_fwd. q, k, v, out, out_lo, lse2 as there, dout with strides of its own, dq / dk / dv bf16 contiguous.
 // starts, ends: mb_document_bounds of the key rows, or both null. scratch: mb_window_attn_bwd_scratch_words() words.
 MB_API int mb_window_attn_bwd(const void* q, long long q_tstride, long long q_bstride, const void* k, long long k_tstride,
                               long long k_bstride, const void* v, long long v_tstride, long long v_bstride, const void* out,
-                              const void* dout, long long do_tstride, long long do_bstride, const float* lse, void* dq, void* dk,
-                              void* dv, const int* starts, const int* ends, float* scratch, int B, int Sq, int Sk, int Hq, int Hkv,
+                              const void* out_lo, const void* dout, long long do_tstride, long long do_bstride, const float* lse2, void* dq,
+                              void* dk, void* dv, const int* starts, const int* ends, float* scratch, int B, int Sq, int Sk, int Hq, int Hkv,
                               int D, int window, int sinks, float scale, cudaStream_t stream) {
   using namespace mb;
   const long long strides[] = {q_tstride, q_bstride, k_tstride, k_bstride, v_tstride, v_bstride, do_tstride, do_bstride};
-  const void* pointers[] = {q, k, v, out, dout, dq, dk, dv, scratch};
-  if (const char* what = window_attn_problem(B, Sq, Sk, Hq, Hkv, D, window, sinks, strides, 8, pointers, 9)) {
+  const void* pointers[] = {q, k, v, out, out_lo, dout, dq, dk, dv, scratch};
+  if (const char* what = window_attn_problem(B, Sq, Sk, Hq, Hkv, D, window, sinks, strides, 8, pointers, 10)) {
     set_last_error(what);
     return -1;
   }
@@ -1120,7 +1142,7 @@ MB_API int mb_window_attn_bwd(const void* q, long long q_tstride, long long q_bs
   int* status = status_ptr();
   if (!status) return -4;
   FlashBwdArgs a{};
-  a.dq = dq, a.dk = dk, a.dv = dv;
+  a.dq = dq, a.dk = dk, a.dv = dv, a.out_lo = out_lo;
   a.dq_tstride = static_cast<long long>(Hq) * D, a.dkv_tstride = static_cast<long long>(Hkv) * D;
   a.B = B, a.Sq = Sq, a.Sk = Sk, a.Hq = Hq, a.Hkv = Hkv;
   a.Sq_pad = (Sq + 127) / 128 * 128, a.Sk_pad = (Sk + 127) / 128 * 128;
@@ -1131,7 +1153,7 @@ MB_API int mb_window_attn_bwd(const void* q, long long q_tstride, long long q_bs
   const long long o_tstride = static_cast<long long>(Hq) * D, o_bstride = o_tstride * Sq;
   if (D == 128)
     return launch_flash_bwd<128, 4>(q, q_tstride, q_bstride, k, v, k_tstride, k_bstride, v_tstride, v_bstride, out, o_tstride, o_bstride,
-                                    dout, do_tstride, do_bstride, lse, nullptr, nullptr, nullptr, nullptr, scratch, a, stream);
+                                    dout, do_tstride, do_bstride, lse2, nullptr, nullptr, nullptr, nullptr, scratch, a, stream);
   return launch_flash_bwd<64, 4>(q, q_tstride, q_bstride, k, v, k_tstride, k_bstride, v_tstride, v_bstride, out, o_tstride, o_bstride,
-                                 dout, do_tstride, do_bstride, lse, nullptr, nullptr, nullptr, nullptr, scratch, a, stream);
+                                 dout, do_tstride, do_bstride, lse2, nullptr, nullptr, nullptr, nullptr, scratch, a, stream);
 }

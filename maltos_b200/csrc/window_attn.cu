@@ -7,6 +7,11 @@
 // The two tiles are two query heads of one key/value head on the same rows where the group is even, else neighbouring rows of
 // one head. O is rescaled only when a row's maximum has grown by more than 2^8 since the last rescale: P then stays below 2^8
 // and its bf16 rounding is relative, so nothing is lost, and after the first blocks the rescale hardly ever happens.
+//
+// What P is relative to is a whole power of two, and O is divided by the sum of the ROUNDED P. The backward can then form the
+// very same rounded weights, for which the terms of dS cancel as they do in the exact softmax; with weights rounded in one
+// place only, a row whose keys have much in common (first tokens that take most of the weight) or that sees few keys loses
+// up to a few per cent of dq. For the same reason the forward of a training step keeps what the rounding of O left (out_lo).
 #include "host.h"
 #include "ptx.cuh"
 #include "window.cuh"
@@ -23,7 +28,9 @@ constexpr float kWfGrowth = 8.f;                   // log2 of how far P may exce
 
 struct WindowFwdArgs {
   __nv_bfloat16* out;       // [B, Sq, Hq, D]
-  float* lse;               // [B, Hq, Sq]
+  __nv_bfloat16* out_lo;    // the same shape: O - out, for the backward; or null
+  float* lse2;              // [B, Hq, Sq] log2 of the sum of the rounded weights, for the backward; or null
+  float* lse;               // [B, Hq, Sq] log-sum-exp of the scores; or null (then its sum is not formed)
   WindowRule rule;
   int B, Sq, Sk, Hq, Hkv;
   int pair;                 // tiles of an item: 0 one tile, 1 two heads of a group, 2 two neighbouring row tiles
@@ -77,7 +84,7 @@ __device__ __forceinline__ void window_item_blocks(const WindowFwdArgs& p, Windo
   it.n = it.na + w1 - it.w0;
 }
 
-template <int D>
+template <int D, bool LSE>
 __global__ void __launch_bounds__(kWfThreads, 1)
 window_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
                   const __grid_constant__ CUtensorMap tmV, const WindowFwdArgs p) {
@@ -270,7 +277,8 @@ window_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
       const int n = tile.count();
       const int qi = q0 + row;
       const WindowRow w = window_row(p.rule, it.batch, p.Sk, qi + p.Sk - p.Sq, qi < p.Sq);
-      float m_run = -INFINITY, l_run = 0.f;        // maximum (exp2 domain) that P is relative to, sum of P
+      // m_run: the power of two that P is relative to; l_run: sum of the rounded P; x_run: of P as it was before
+      float m_run = -INFINITY, l_run = 0.f, x_run = 0.f;
       for (int j = 0; j < n; ++j) {
         ok = mbar_wait(&s_full[t], s_count & 1, abort_flag);
         ok = __all_sync(0xffffffffu, ok);
@@ -296,10 +304,11 @@ window_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
         for (int i = 0; i < 128; ++i) mx[i & 3] = fmaxf(mx[i & 3], __uint_as_float(s[i]));
         const float m_blk = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * p.scale_log2;
         if (__any_sync(0xffffffffu, m_blk > m_run + kWfGrowth)) {
-          const float m_new = fmaxf(m_run, m_blk);
-          const float alpha = m_run == -INFINITY ? 0.f : wf_exp2(m_run - m_new);
+          const float m_new = fmaxf(m_run, ceilf(m_blk));
+          const float alpha = m_run == -INFINITY ? 0.f : wf_exp2(m_run - m_new);   // a power of two
           m_run = m_new;
           l_run *= alpha;
+          if (LSE) x_run *= alpha;
           if (j > 0) {
 #pragma unroll 1
             for (int c = 0; c < D; c += 16) {
@@ -313,20 +322,29 @@ window_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
           }
         }
         const float m_safe = m_run == -INFINITY ? 0.f : m_run;
-        float sum[4] = {0.f, 0.f, 0.f, 0.f};
+        const uint64_t scale2 = f32x2(p.scale_log2, p.scale_log2), shift2 = f32x2(-m_safe, -m_safe);
+        uint64_t sum[2] = {0, 0}, sum_x[2] = {0, 0};
 #pragma unroll
         for (int c = 0; c < 4; ++c) {              // 32 keys: 16 columns of packed P
           uint32_t pk[16];
 #pragma unroll
           for (int i = 0; i < 16; ++i) {
-            const float a = wf_exp2(fmaf(__uint_as_float(s[c * 32 + 2 * i]), p.scale_log2, -m_safe));
-            const float b = wf_exp2(fmaf(__uint_as_float(s[c * 32 + 2 * i + 1]), p.scale_log2, -m_safe));
-            sum[i & 3] += a + b;
+            float a, b;
+            f32x2_split(fma_f32x2(f32x2(__uint_as_float(s[c * 32 + 2 * i]), __uint_as_float(s[c * 32 + 2 * i + 1])), scale2, shift2), a, b);
+            a = wf_exp2(a), b = wf_exp2(b);
             pk[i] = pack_bf16x2(a, b);
+            sum[i & 1] = add_f32x2(sum[i & 1], bf16x2_as_f32x2(pk[i]));
+            if (LSE) sum_x[i & 1] = add_f32x2(sum_x[i & 1], f32x2(a, b));
           }
           tmem_st_32x32b_x16(s_tmem + c * 16, pk);
         }
-        l_run += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+        float lo, hi;
+        f32x2_split(add_f32x2(sum[0], sum[1]), lo, hi);
+        l_run += lo + hi;
+        if (LSE) {
+          f32x2_split(add_f32x2(sum_x[0], sum_x[1]), lo, hi);
+          x_run += lo + hi;
+        }
         tmem_st_wait();
         tc_fence_before();
         __syncwarp();
@@ -342,7 +360,7 @@ window_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
         tc_fence_after();
       }
       const float inv = l_run > 0.f ? 1.f / l_run : 0.f;
-      __nv_bfloat16* dst = p.out + ((static_cast<long long>(it.batch) * p.Sq + qi) * p.Hq + head) * D;
+      const long long at = ((static_cast<long long>(it.batch) * p.Sq + qi) * p.Hq + head) * D;
 #pragma unroll 1
       for (int c = 0; c < D; c += 32) {
         uint32_t r[32];
@@ -356,18 +374,24 @@ window_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
         if (qi < p.Sq) {
 #pragma unroll
           for (int i = 0; i < 32; i += 8) {
-            uint4 v;
-            v.x = pack_bf16x2(__uint_as_float(r[i]) * inv, __uint_as_float(r[i + 1]) * inv);
-            v.y = pack_bf16x2(__uint_as_float(r[i + 2]) * inv, __uint_as_float(r[i + 3]) * inv);
-            v.z = pack_bf16x2(__uint_as_float(r[i + 4]) * inv, __uint_as_float(r[i + 5]) * inv);
-            v.w = pack_bf16x2(__uint_as_float(r[i + 6]) * inv, __uint_as_float(r[i + 7]) * inv);
-            *reinterpret_cast<uint4*>(dst + c + i) = v;
+            uint32_t v[4], w[4];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+              const float a = __uint_as_float(r[i + 2 * k]) * inv, b = __uint_as_float(r[i + 2 * k + 1]) * inv;
+              v[k] = pack_bf16x2(a, b);
+              w[k] = pack_bf16x2(a - __uint_as_float(v[k] << 16), b - __uint_as_float(v[k] & 0xffff0000u));
+            }
+            *reinterpret_cast<uint4*>(p.out + at + c + i) = make_uint4(v[0], v[1], v[2], v[3]);
+            if (p.out_lo) *reinterpret_cast<uint4*>(p.out_lo + at + c + i) = make_uint4(w[0], w[1], w[2], w[3]);
           }
         }
       }
       tc_fence_before();                           // these reads of O come before the next item's first product (via p_full)
-      if (qi < p.Sq)
-        p.lse[(static_cast<long long>(it.batch) * p.Hq + head) * p.Sq + qi] = l_run > 0.f ? (m_run + log2f(l_run)) * kWfLn2 : -INFINITY;
+      if (qi < p.Sq) {
+        const long long stat = (static_cast<long long>(it.batch) * p.Hq + head) * p.Sq + qi;
+        if (p.lse2) p.lse2[stat] = l_run > 0.f ? m_run + log2f(l_run) : -INFINITY;
+        if (LSE) p.lse[stat] = x_run > 0.f ? (m_run + log2f(x_run)) * kWfLn2 : -INFINITY;
+      }
     }
   }
 
@@ -387,7 +411,7 @@ window_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
   }
 }
 
-template <int D>
+template <int D, bool LSE>
 static int launch_window_fwd(const CUtensorMap& tmQ, const CUtensorMap& tmK, const CUtensorMap& tmV, const WindowFwdArgs& args,
                              cudaStream_t stream) {
   constexpr size_t smem = 1024 + (2 + kWfStages) * (kWinBlock * D * 2) + 256;
@@ -396,16 +420,16 @@ static int launch_window_fwd(const CUtensorMap& tmQ, const CUtensorMap& tmK, con
   MB_CHECK_CUDA(cudaGetDevice(&dev));
   if (!configured[dev & 63]) {
     cudaFuncAttributes at;
-    MB_CHECK_CUDA(cudaFuncGetAttributes(&at, window_fwd_kernel<D>));
+    MB_CHECK_CUDA(cudaFuncGetAttributes(&at, window_fwd_kernel<D, LSE>));
     if (at.numRegs != kWfLaunchRegs) {             // the split of the register file is made for this launch size
       set_last_error("mb_window_attn_fwd: built with another register count than the register split assumes");
       return -6;
     }
-    MB_CHECK_CUDA(cudaFuncSetAttribute(window_fwd_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem)));
+    MB_CHECK_CUDA(cudaFuncSetAttribute(window_fwd_kernel<D, LSE>, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem)));
     configured[dev & 63] = true;
   }
   const int grid = args.items < sm_count() ? args.items : sm_count();
-  window_fwd_kernel<D><<<grid, kWfThreads, smem, stream>>>(tmQ, tmK, tmV, args);
+  window_fwd_kernel<D, LSE><<<grid, kWfThreads, smem, stream>>>(tmQ, tmK, tmV, args);
   count_launch();
   MB_CHECK_CUDA(cudaGetLastError());
   return 0;
@@ -484,16 +508,17 @@ MB_API int mb_document_bounds(const void* ids, int wide, int* starts, int* ends,
 }
 
 // q [B, Sq, Hq, D], k / v [B, Sk, Hkv, D] bf16 with element strides between tokens and batches (heads contiguous inside a
-// token), out [B, Sq, Hq, D] bf16 contiguous, lse [B, Hq, Sq] fp32 (-inf where nothing is visible). starts: mb_document_bounds
-// of the key rows, or null for one document a row.
+// token), out [B, Sq, Hq, D] bf16 contiguous. For the backward: out_lo like out and lse2 [B, Hq, Sq] fp32, or both null. lse
+// [B, Hq, Sq] fp32 or null: log-sum-exp, -inf where nothing is visible. starts: mb_document_bounds of the key rows, or null for
+// one document a row.
 MB_API int mb_window_attn_fwd(const void* q, long long q_tstride, long long q_bstride, const void* k, long long k_tstride,
-                              long long k_bstride, const void* v, long long v_tstride, long long v_bstride, void* out, float* lse,
-                              const int* starts, int B, int Sq, int Sk, int Hq, int Hkv, int D, int window, int sinks, float scale,
+                              long long k_bstride, const void* v, long long v_tstride, long long v_bstride, void* out, void* out_lo,
+                              float* lse2, float* lse, const int* starts, int B, int Sq, int Sk, int Hq, int Hkv, int D, int window, int sinks, float scale,
                               cudaStream_t stream) {
   using namespace mb;
   const long long strides[] = {q_tstride, q_bstride, k_tstride, k_bstride, v_tstride, v_bstride};
-  const void* pointers[] = {q, k, v, out};
-  if (const char* what = window_attn_problem(B, Sq, Sk, Hq, Hkv, D, window, sinks, strides, 6, pointers, 4)) {
+  const void* pointers[] = {q, k, v, out, out_lo};
+  if (const char* what = window_attn_problem(B, Sq, Sk, Hq, Hkv, D, window, sinks, strides, 6, pointers, 5)) {
     set_last_error(what);
     return -1;
   }
@@ -501,7 +526,8 @@ MB_API int mb_window_attn_fwd(const void* q, long long q_tstride, long long q_bs
   if (!status) return -4;
   WindowFwdArgs a;
   a.out = static_cast<__nv_bfloat16*>(out);
-  a.lse = lse;
+  a.out_lo = static_cast<__nv_bfloat16*>(out_lo);
+  a.lse2 = lse2, a.lse = lse;
   a.rule = {starts, nullptr, window < Sk ? window : Sk, sinks < Sk ? sinks : Sk};
   a.B = B, a.Sq = Sq, a.Sk = Sk, a.Hq = Hq, a.Hkv = Hkv;
   a.scale_log2 = scale * kWfLog2e;
@@ -527,5 +553,6 @@ MB_API int mb_window_attn_fwd(const void* q, long long q_tstride, long long q_bs
   if (!encode(&tmQ, q, Hq, Sq, q_tstride, q_bstride) || !encode(&tmK, k, Hkv, Sk, k_tstride, k_bstride) ||
       !encode(&tmV, v, Hkv, Sk, v_tstride, v_bstride))
     return -5;
-  return D == 128 ? launch_window_fwd<128>(tmQ, tmK, tmV, a, stream) : launch_window_fwd<64>(tmQ, tmK, tmV, a, stream);
+  if (D == 128) return lse ? launch_window_fwd<128, true>(tmQ, tmK, tmV, a, stream) : launch_window_fwd<128, false>(tmQ, tmK, tmV, a, stream);
+  return lse ? launch_window_fwd<64, true>(tmQ, tmK, tmV, a, stream) : launch_window_fwd<64, false>(tmQ, tmK, tmV, a, stream);
 }

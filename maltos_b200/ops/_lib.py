@@ -105,9 +105,9 @@ class _RangedLibrary:
 #: ctypes converts in C, which for a call of twenty arguments is several microseconds less than an object per argument.
 _PROTOTYPES = {
     "mb_document_bounds": "pippiip",
-    "mb_window_attn_fwd": "pllpllpllppp" "iiiiiiii" "fp",
+    "mb_window_attn_fwd": "pllpllpll" "ppppp" "iiiiiiii" "fp",
     "mb_window_attn_bwd_scratch_words": "iiiiii",
-    "mb_window_attn_bwd": "pllpllpll" "ppll" "pppp" "ppp" "iiiiiiii" "fp",
+    "mb_window_attn_bwd": "pllpllpll" "pppll" "pppp" "ppp" "iiiiiiii" "fp",
     "mb_embedding_fwd": "pippilil" "fp",
     "mb_embedding_bwd_scratch_words": "li",
     "mb_embedding_bwd": "pippp" "ilill" "fp",

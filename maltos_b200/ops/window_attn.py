@@ -37,24 +37,27 @@ def document_bounds(sequence_ids: torch.Tensor) -> tuple[torch.Tensor, torch.Ten
     return starts, ends
 
 
-def window_forward(q, k, v, *, window: int, sinks: int, starts, scale: float):
-    """``(out [B, Sq, hq, D] bf16, lse [B, hq, Sq] fp32)``."""
+def window_forward(q, k, v, *, window: int, sinks: int, starts, scale: float, keep: bool, want_lse: bool):
+    """``(out, out_lo, lse2, lse)``: the output ``[B, Sq, hq, D]`` in bf16; for the backward (``keep``) what its rounding left and the
+    log2 of the sum of the rounded weights ``[B, hq, Sq]``; the log-sum-exp of the scores where asked for."""
     B, Sq, Hq, D = q.shape
     Sk, Hkv = k.shape[1], k.shape[2]
     q, q_t, q_b = _addressable(q)
     k, k_t, k_b = _addressable(k)
     v, v_t, v_b = _addressable(v)
     out = torch.empty((B, Sq, Hq, D), dtype=torch.bfloat16, device=q.device)
-    lse = torch.empty((B, Hq, Sq), dtype=torch.float32, device=q.device)
+    out_lo = torch.empty_like(out) if keep else None
+    lse2 = torch.empty((B, Hq, Sq), dtype=torch.float32, device=q.device) if keep else None
+    lse = torch.empty((B, Hq, Sq), dtype=torch.float32, device=q.device) if want_lse else None
     with _lib.on_device_of(q):
         _lib.check(_lib.lib().mb_window_attn_fwd(q.data_ptr(), q_t, q_b, k.data_ptr(), k_t, k_b, v.data_ptr(), v_t, v_b, out.data_ptr(),
-                                                 lse.data_ptr(), _lib.address(starts), B, Sq, Sk, Hq, Hkv, D, window, sinks, scale,
-                                                 _lib.stream_of(q)), "mb_window_attn_fwd")
-    return out, lse
+                                                 _lib.address(out_lo), _lib.address(lse2), _lib.address(lse), _lib.address(starts), B, Sq, Sk,
+                                                 Hq, Hkv, D, window, sinks, scale, _lib.stream_of(q)), "mb_window_attn_fwd")
+    return out, out_lo, lse2, lse
 
 
-def window_backward(q, k, v, out, lse, dout, *, window: int, sinks: int, starts, ends, scale: float):
-    """``(dq, dk, dv)`` in bf16; ``out`` and ``lse`` are the forward's."""
+def window_backward(q, k, v, out, out_lo, lse2, dout, *, window: int, sinks: int, starts, ends, scale: float):
+    """``(dq, dk, dv)`` in bf16; ``out``, ``out_lo`` and ``lse2`` are the forward's."""
     B, Sq, Hq, D = q.shape
     Sk, Hkv = k.shape[1], k.shape[2]
     q, q_t, q_b = _addressable(q)
@@ -68,7 +71,7 @@ def window_backward(q, k, v, out, lse, dout, *, window: int, sinks: int, starts,
     with _lib.on_device_of(q):
         scratch = torch.empty((L.mb_window_attn_bwd_scratch_words(B, Sq, Sk, Hq, Hkv, D),), dtype=torch.float32, device=q.device)
         _lib.check(L.mb_window_attn_bwd(q.data_ptr(), q_t, q_b, k.data_ptr(), k_t, k_b, v.data_ptr(), v_t, v_b, out.data_ptr(),
-                                        dout.data_ptr(), do_t, do_b, lse.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(),
+                                        out_lo.data_ptr(), dout.data_ptr(), do_t, do_b, lse2.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(),
                                         _lib.address(starts), _lib.address(ends), scratch.data_ptr(), B, Sq, Sk, Hq, Hkv, D, window, sinks,
                                         scale, _lib.stream_of(q)), "mb_window_attn_bwd")
     return dq, dk, dv
@@ -76,29 +79,30 @@ def window_backward(q, k, v, out, lse, dout, *, window: int, sinks: int, starts,
 
 class _WindowAttention(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, q, k, v, window, sinks, starts, ends, scale):
-        # As in dense flash attention: under activation checkpointing the recompute replays (out, lse) of the first pass.
+    def forward(ctx, q, k, v, window, sinks, starts, ends, scale, want_lse):
+        # As in dense flash attention: under activation checkpointing the recompute replays the results of the first pass.
         from maltos_b200.utils.activation_checkpoint import current_checkpoint_stash
 
         stash = current_checkpoint_stash()
         kept = stash.replay() if stash is not None and stash.replaying else None
-        if kept is not None and kept[0].shape == q.shape:
-            out, lse = kept
+        if kept is not None and len(kept) == 4 and kept[0].shape == q.shape:
+            out, out_lo, lse2, lse = kept
         else:
-            out, lse = window_forward(q, k, v, window=window, sinks=sinks, starts=starts, scale=scale)
+            out, out_lo, lse2, lse = window_forward(q, k, v, window=window, sinks=sinks, starts=starts, scale=scale, keep=True, want_lse=want_lse)
             if stash is not None and not stash.replaying:
-                stash.record((out, lse))
-        ctx.save_for_backward(q, k, v, out, lse, starts, ends)
+                stash.record((out, out_lo, lse2, lse))
+        ctx.save_for_backward(q, k, v, out, out_lo, lse2, starts, ends)
         ctx.window, ctx.sinks, ctx.scale = window, sinks, scale
-        ctx.mark_non_differentiable(lse)
+        if lse is not None:
+            ctx.mark_non_differentiable(lse)
         return out, lse
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dout, _dlse):
-        q, k, v, out, lse, starts, ends = ctx.saved_tensors
-        dq, dk, dv = window_backward(q, k, v, out, lse, dout, window=ctx.window, sinks=ctx.sinks, starts=starts, ends=ends, scale=ctx.scale)
-        return dq, dk, dv, None, None, None, None, None
+        q, k, v, out, out_lo, lse2, starts, ends = ctx.saved_tensors
+        dq, dk, dv = window_backward(q, k, v, out, out_lo, lse2, dout, window=ctx.window, sinks=ctx.sinks, starts=starts, ends=ends, scale=ctx.scale)
+        return dq, dk, dv, None, None, None, None, None, None
 
 
 def window_attention(q, k, v, *, window: int, sinks: int = 0, sequence_ids=None, scale: float | None = None, return_lse: bool = False):
@@ -108,7 +112,7 @@ def window_attention(q, k, v, *, window: int, sinks: int = 0, sequence_ids=None,
     scale = float(scale) if scale is not None else 1.0 / math.sqrt(q.shape[3])
     window, sinks = min(window, Sk), min(sinks, Sk)
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
-        out, lse = _WindowAttention.apply(q, k, v, window, sinks, starts, ends, scale)
+        out, lse = _WindowAttention.apply(q, k, v, window, sinks, starts, ends, scale, return_lse)
     else:
-        out, lse = window_forward(q, k, v, window=window, sinks=sinks, starts=starts, scale=scale)
+        out, _, _, lse = window_forward(q, k, v, window=window, sinks=sinks, starts=starts, scale=scale, keep=False, want_lse=return_lse)
     return (out, lse) if return_lse else out

@@ -47,16 +47,17 @@ def _expect(q, k, v, dout, window, sinks, ids, scale):
     lse = torch.logsumexp(S, -1)
     P = torch.exp(S - lse.masked_fill(lse == -math.inf, 0.0).unsqueeze(-1))
     out = P @ V
-    # P is rounded to bf16 (u of each weight), the result once more
-    e_p = 1.05 * U + 2.0 ** -12
+    # The weights are rounded to bf16 (u of each) and divided by the sum of the rounded ones (u again at most); the result is
+    # rounded once more, for the backward it is kept to 2^-16.
+    e_p = 1.05 * 2 * U + 2.0 ** -12
     e_out = e_p * (P @ V.abs())
     b_out = e_out + U * (out.abs() + e_out)
     dP = dO @ V.transpose(-1, -2)
     delta = (dO * out).sum(-1, keepdim=True)
     dS = P * (dP - delta)
-    # delta is taken from the rounded output; dS is rounded to bf16
-    e_delta = (dO.abs() * b_out).sum(-1, keepdim=True) + 2.0 ** -12 * (dO.abs() * out.abs()).sum(-1, keepdim=True)
-    e_ds = P * e_delta + e_p * dS.abs() + 2.0 ** -12 * P * (dO.abs() @ V.abs().transpose(-1, -2))
+    # delta is taken from that output; dS is formed from rounded weights and rounded to bf16
+    e_delta = (dO.abs() * e_out).sum(-1, keepdim=True) + 2.0 ** -12 * (dO.abs() * out.abs()).sum(-1, keepdim=True)
+    e_ds = P * e_delta + (e_p + 1.05 * U) * dS.abs() + 2.0 ** -12 * P * (dO.abs() @ V.abs().transpose(-1, -2))
     fold = lambda t: t.reshape(B, hkv, g, Sk, D).sum(2)                      # noqa: E731
     dq, e_dq = scale * dS @ K, scale * e_ds @ K.abs()
     dk, e_dk = fold(scale * dS.transpose(-1, -2) @ Q), fold(scale * e_ds.transpose(-1, -2) @ Q.abs())
