@@ -326,8 +326,8 @@ MB_API int mb_block_norm_bwd(const void* dy, const void* dh, const void* x, cons
                              int gate_mode, const float* r1, const float* r2, void* dx, void* dresidual, void* dw1, void* dw2, void* dgate,
                              float* part1, float* part2, int dtype, long long rows, int H, float scale, cudaStream_t stream) {
   using namespace mb;
-  const void* pointers[] = {dy, dh, x, h, w1, w2, gate, dx, dresidual, dgate, part1, part2};
-  const char* what = block_norm_problem(dtype, rows, H, gate_mode, gate, pointers, 12);
+  const void* pointers[] = {dy, dh, x, h, w1, w2, gate, dx, dresidual, dgate};
+  const char* what = block_norm_problem(dtype, rows, H, gate_mode, gate, pointers, 10);
   if (!what && ((w1 && (!r1 || !x || !dw1)) || (w2 && (!r2 || !h || !dw2 || !part2)) || (gate && (!x || !dgate)) || !dx || !dresidual ||
                 ((w1 || gate_mode == 1) && !part1)))
     what = "mb_block_norm_bwd: a tensor that these arguments need is missing";

@@ -194,6 +194,13 @@ def address(t: torch.Tensor | None) -> int | None:
     return None if t is None else t.data_ptr()
 
 
+def refuse_second_order(what: str) -> None:
+    """For the top of a backward whose kernels record no graph: gradient recording is on there only under ``create_graph=True``,
+    whose result would silently lack the second order."""
+    if torch.is_grad_enabled():
+        raise RuntimeError(f"{what} is differentiable once; create_graph=True is not supported")
+
+
 def ptr(t: torch.Tensor | None) -> c_void_p:
     if t is None:
         return c_void_p(0)

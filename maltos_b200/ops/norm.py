@@ -108,35 +108,35 @@ def _dense(t: torch.Tensor | None) -> torch.Tensor | None:
 
 
 def _block_norm_forward(x, residual, w1, w2, g, scale, eps, keep: bool):
-    """``(y or None, h, r1, r2)`` of dense tensors; the two statistics only where the backward will ask for them."""
+    """``(y or None, h, stats)`` of dense tensors; the two norms' statistics ``[2, rows]`` only where the backward will ask for them."""
     H = x.shape[-1]
     rows = x.numel() // H
     h = torch.empty_like(x)
     y = torch.empty_like(x) if w2 is not None else None
-    r1 = torch.empty(rows, dtype=torch.float32, device=x.device) if keep and w1 is not None else None
-    r2 = torch.empty(rows, dtype=torch.float32, device=x.device) if keep and w2 is not None else None
+    stats = torch.empty((2, rows), dtype=torch.float32, device=x.device) if keep else None
+    r1 = stats.data_ptr() if keep else None
     mode, a = 0 if g is None else 1 if g.dim() == 1 and x.dim() > 1 else 2, _lib.address
     with _lib.on_device_of(x):
-        _lib.check(_lib.lib().mb_block_norm_fwd(x.data_ptr(), residual.data_ptr(), a(w1), a(w2), a(g), mode, h.data_ptr(), a(y), a(r1), a(r2),
-                                                _BLOCK_DTYPES[x.dtype], rows, H, scale, eps, _lib.stream_of(x)), "mb_block_norm_fwd")
-    return y, h, r1, r2
+        _lib.check(_lib.lib().mb_block_norm_fwd(x.data_ptr(), residual.data_ptr(), a(w1), a(w2), a(g), mode, h.data_ptr(), a(y), r1,
+                                                r1 + 4 * rows if keep else None, _BLOCK_DTYPES[x.dtype], rows, H, scale, eps, _lib.stream_of(x)), "mb_block_norm_fwd")
+    return y, h, stats
 
 
 class _BlockNorm(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, residual, weight, next_weight, gate, scale, eps):
         x, w1, w2, g = _dense(x), _dense(weight), _dense(next_weight), _dense(gate)
-        y, h, r1, r2 = _block_norm_forward(x, _dense(residual), w1, w2, g, scale, eps, True)
+        y, h, stats = _block_norm_forward(x, _dense(residual), w1, w2, g, scale, eps, True)
         # x is needed for its norm's and the gate's gradients, h for the next norm's
-        ctx.save_for_backward(x if w1 is not None or g is not None else None, h if w2 is not None else None, w1, w2, g, r1, r2)
+        ctx.save_for_backward(x if w1 is not None or g is not None else None, h if w2 is not None else None, w1, w2, g, stats)
         ctx.scale = scale
         ctx.set_materialize_grads(False)
         return h if y is None else (y, h)
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, *douts):
-        x, h, w1, w2, g, r1, r2 = ctx.saved_tensors
+        _lib.refuse_second_order("block_norm")
+        x, h, w1, w2, g, stats = ctx.saved_tensors
         dy, dh = douts if w2 is not None else (None, douts[0])
         if dy is None and dh is None:
             return (None,) * 7
@@ -149,11 +149,11 @@ class _BlockNorm(torch.autograd.Function):
         dw1, dw2, dg = (None if t is None else torch.empty_like(t) for t in (w1, w2, g))
         L = _lib.lib()
         with _lib.on_device_of(some):
-            first = w1 is not None or mode == 1
-            parts = torch.empty((int(first) + int(w2 is not None), L.mb_block_norm_bwd_parts(rows), H), dtype=torch.float32, device=some.device)
-            part1, part2 = parts[0] if first else None, parts[-1] if w2 is not None else None
-            _lib.check(L.mb_block_norm_bwd(a(dy), a(dh), a(x), a(h), a(w1), a(w2), a(g), mode, a(r1), a(r2), dx.data_ptr(), dres.data_ptr(),
-                                           a(dw1), a(dw2), a(dg), a(part1), a(part2), _BLOCK_DTYPES[some.dtype], rows, H, ctx.scale,
+            size = L.mb_block_norm_bwd_parts(rows) * H
+            parts = torch.empty(2 * size, dtype=torch.float32, device=some.device)
+            r1, part = stats.data_ptr(), parts.data_ptr()
+            _lib.check(L.mb_block_norm_bwd(a(dy), a(dh), a(x), a(h), a(w1), a(w2), a(g), mode, r1, r1 + 4 * rows, dx.data_ptr(), dres.data_ptr(),
+                                           a(dw1), a(dw2), a(dg), part, part + 4 * size, _BLOCK_DTYPES[some.dtype], rows, H, ctx.scale,
                                            _lib.stream_of(some)), "mb_block_norm_bwd")
         return dx, dres, dw1, dw2, dg, None, None
 
@@ -189,7 +189,7 @@ def block_norm(x: torch.Tensor, residual: torch.Tensor, weight: torch.Tensor | N
     if _lib.use_kernels(x) and x.dtype in _BLOCK_DTYPES and x.numel() and H % 8 == 0 and H <= _BLOCK_MAX_HIDDEN:
         if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, residual, weight, next_weight, gate)):
             return _BlockNorm.apply(x, residual, weight, next_weight, gate, float(scale), float(eps))
-        y, h, _, _ = _block_norm_forward(_dense(x), _dense(residual), _dense(weight), _dense(next_weight), _dense(gate), float(scale),
+        y, h, _ = _block_norm_forward(_dense(x), _dense(residual), _dense(weight), _dense(next_weight), _dense(gate), float(scale),
                                          float(eps), False)
         return h if y is None else (y, h)
     return block_norm_reference(x, residual, weight, next_weight, gate=gate, scale=scale, eps=eps)

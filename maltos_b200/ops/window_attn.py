@@ -7,6 +7,8 @@ import math
 
 import torch
 
+from maltos_b200.utils.activation_checkpoint import current_checkpoint_stash
+
 from . import _lib
 
 
@@ -63,7 +65,7 @@ def window_backward(q, k, v, out, out_lo, lse2, dout, *, window: int, sinks: int
     q, q_t, q_b = _addressable(q)
     k, k_t, k_b = _addressable(k)
     v, v_t, v_b = _addressable(v)
-    dout, do_t, do_b = _addressable(dout.to(torch.bfloat16))
+    dout, do_t, do_b = _addressable(dout)
     dq = torch.empty((B, Sq, Hq, D), dtype=torch.bfloat16, device=q.device)
     dk = torch.empty((B, Sk, Hkv, D), dtype=torch.bfloat16, device=q.device)
     dv = torch.empty((B, Sk, Hkv, D), dtype=torch.bfloat16, device=q.device)
@@ -81,8 +83,6 @@ class _WindowAttention(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, window, sinks, starts, ends, scale, want_lse):
         # As in dense flash attention: under activation checkpointing the recompute replays the results of the first pass.
-        from maltos_b200.utils.activation_checkpoint import current_checkpoint_stash
-
         stash = current_checkpoint_stash()
         kept = stash.replay() if stash is not None and stash.replaying else None
         if kept is not None and len(kept) == 4 and kept[0].shape == q.shape:
@@ -98,8 +98,8 @@ class _WindowAttention(torch.autograd.Function):
         return out, lse
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, dout, _dlse):
+        _lib.refuse_second_order("sliding_window_attention")
         q, k, v, out, out_lo, lse2, starts, ends = ctx.saved_tensors
         dq, dk, dv = window_backward(q, k, v, out, out_lo, lse2, dout, window=ctx.window, sinks=ctx.sinks, starts=starts, ends=ends, scale=ctx.scale)
         return dq, dk, dv, None, None, None, None, None, None
