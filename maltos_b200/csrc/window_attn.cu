@@ -2,8 +2,12 @@
 // tiles of 128 query rows that walk the same list of key blocks, so a K / V block fetched once serves both tiles and the
 // softmax of one tile runs under the matrix products of the other:
 //   warp 0       TMA producer: the tiles' queries and a ring of K and V blocks,
-//   warp 1       issues S = Q K^T and O += P V as UMMAs; S, P and O stay in tensor memory (P overwrites the scores it came from),
-//   warps 4-7 and 8-11  one warpgroup per tile, a thread per query row: running maximum and sum, P in bf16, output.
+//   warps 1, 2   one per tile: issue S = Q K^T and O += P V as UMMAs; S, P and O stay in tensor memory (P overwrites the scores it
+//                came from). A wait that is already satisfied still costs some 250 cycles while UMMAs saturate shared memory, so
+//                each tile has an issuer of its own and no barrier is asked twice,
+//   warps 4-7 and 8-11  one warpgroup per tile, a thread per query row: running maximum and sum, P in bf16, output. P is handed
+//                over in halves of 64 keys, so that O += P V begins under the second half's exponentials; a share of the
+//                exponentials runs on the multiply-add pipe, since the special-function unit alone would take as long as the UMMAs.
 // The two tiles are two query heads of one key/value head on the same rows where the group is even, else neighbouring rows of
 // one head. O is rescaled only when a row's maximum has grown by more than 2^8 since the last rescale: P then stays below 2^8
 // and its bf16 rounding is relative, so nothing is lost, and after the first blocks the rescale hardly ever happens.
@@ -24,6 +28,7 @@ constexpr int kWfStages = 5;                       // K and V blocks in flight
 constexpr int kWfLaunchRegs = 168, kWfOtherRegs = 56, kWfSoftmaxRegs = 224;
 static_assert(128 * kWfOtherRegs + 256 * kWfSoftmaxRegs <= kWfThreads * kWfLaunchRegs, "register split exceeds the launch");
 constexpr float kWfLog2e = 1.4426950408889634f, kWfLn2 = 0.6931471805599453f;
+constexpr int kWfPoly = 2, kWfPolyOf = 8;          // pairs of exponentials on the multiply-add pipe: 2 of every 8
 constexpr float kWfGrowth = 8.f;                   // log2 of how far P may exceed 1 before O is rescaled
 
 struct WindowFwdArgs {
@@ -43,6 +48,28 @@ __device__ __forceinline__ float wf_exp2(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
+}
+
+// 2^x for a pair, x <= 120, on the multiply-add pipe: x = n + f with n the nearest integer (adding 1.5 * 2^23 leaves n in the low
+// bits), 2^f by a polynomial on [-1/2, 1/2], n added to the exponent. The coefficients are the minimax fit of degree 4 to the
+// relative error with p(0) = 1 (solved as a linear programme on a grid): 2.8e-6, far below the bf16 rounding that follows.
+// x below -127 gives exactly 0: there n = -127, f = 0, and the exponent of 1 becomes that of zero.
+__device__ __forceinline__ void wf_exp2_poly(uint64_t x, float& a, float& b) {
+  float lo, hi;
+  f32x2_split(x, lo, hi);
+  x = f32x2(fmaxf(lo, -127.f), fmaxf(hi, -127.f));
+  const uint64_t magic = f32x2(12582912.f, 12582912.f), minus_magic = f32x2(-12582912.f, -12582912.f), minus_one = f32x2(-1.f, -1.f);
+  const uint64_t t = add_f32x2(x, magic);
+  const uint64_t f = fma_f32x2(add_f32x2(t, minus_magic), minus_one, x);
+  uint64_t r = fma_f32x2(f32x2(0.009582576341927052f, 0.009582576341927052f), f, f32x2(0.05590682849287987f, 0.05590682849287987f));
+  r = fma_f32x2(r, f, f32x2(0.24024106562137604f, 0.24024106562137604f));
+  r = fma_f32x2(r, f, f32x2(0.6931241154670715f, 0.6931241154670715f));
+  r = fma_f32x2(r, f, f32x2(1.f, 1.f));
+  float ta, tb, ra, rb;
+  f32x2_split(t, ta, tb);
+  f32x2_split(r, ra, rb);
+  a = __uint_as_float(__float_as_uint(ra) + (__float_as_uint(ta) << 23));
+  b = __uint_as_float(__float_as_uint(rb) + (__float_as_uint(tb) << 23));
 }
 
 struct WindowItem {
@@ -101,11 +128,12 @@ window_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
   uint64_t* q_full = bars;                         // 2
   uint64_t* q_empty = bars + 2;                    // 2
   uint64_t* s_full = bars + 4;                     // 2
-  uint64_t* p_full = bars + 6;                     // 2
-  uint64_t* o_full = bars + 8;                     // 2
-  uint64_t* kv_full = bars + 10;                   // kWfStages
+  uint64_t* p_full = bars + 6;                     // 2 tiles x 2 halves
+  uint64_t* o_full = bars + 10;                    // 2
+  uint64_t* kv_full = bars + 12;                   // kWfStages
   uint64_t* kv_empty = kv_full + kWfStages;        // kWfStages
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(kv_empty + kWfStages);
+  uint64_t* turn = kv_empty + kWfStages;           // 2: the exponentials of a block are tile t's turn
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(turn + 2);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -114,12 +142,14 @@ window_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
       mbar_init(&q_full[t], 1);
       mbar_init(&q_empty[t], 1);
       mbar_init(&s_full[t], 1);
-      mbar_init(&p_full[t], 4);
+      mbar_init(&p_full[2 * t], 4);
+      mbar_init(&p_full[2 * t + 1], 4);
       mbar_init(&o_full[t], 1);
+      mbar_init(&turn[t], 4);
     }
     for (int i = 0; i < kWfStages; ++i) {
       mbar_init(&kv_full[i], 1);
-      mbar_init(&kv_empty[i], 1);
+      mbar_init(&kv_empty[i], 2);
     }
     abort_flag[0] = 0;
     abort_flag[1] = p.status[3];
@@ -149,6 +179,15 @@ window_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
         window_item(p, item, it);
         window_item_blocks(p, it);
         if (lane == 0) {
+          // The next item's queries and first blocks on their way to L2, so that its start does not wait for HBM.
+          if (item + static_cast<int>(gridDim.x) < p.items) {
+            WindowItem next;
+            window_item(p, item + gridDim.x, next);
+            for (int t = 0; t < 2; ++t)
+              if (next.q0[t] < p.Sq)
+#pragma unroll
+                for (int a = 0; a < ATOMS; ++a) tma_prefetch_4d(&tmQ, a * 64, next.head[t], next.q0[t], next.batch);
+          }
 #pragma unroll
           for (int t = 0; t < 2; ++t) {
             if (!ok || it.tile[t].count() == 0) continue;
@@ -176,82 +215,85 @@ window_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
         ok = __shfl_sync(0xffffffffu, static_cast<int>(ok), 0) != 0;
         if (!ok) break;
       }
-    } else if (warp == 1) {
-      // ---------------------------------------------------------------- UMMA issuer
-      // Step u: for each tile first O += P V of its last block (u - 1), then its scores of block u over that P. The scores'
-      // commit therefore also says that the product before them is complete, which is what a rescale of O waits for.
+    } else if (warp <= 2) {
+      // ---------------------------------------------------------------- UMMA issuer of tile t
+      // Step u: O += P V of block u - 1, then the scores of block u over that P. The scores' commit therefore also says that the
+      // product before them is complete, which is what a rescale of O waits for.
+      const int t = warp - 1;
       const uint32_t idesc_qk = make_idesc_bf16(kWinBlock, kWinBlock, 0, 0);
       const uint32_t idesc_pv = make_idesc_bf16(kWinBlock, D, 0, 1);
       constexpr uint32_t hi = smem_desc_hi_sw128(1024);
-      int base = 0;                                // K / V blocks consumed before this item
-      int p_count[2] = {0, 0}, q_count[2] = {0, 0};
+      const uint32_t s_tmem = tmem_base + S_COL + static_cast<uint32_t>(t) * 128u, o_tmem = tmem_base + O_COL + static_cast<uint32_t>(t) * 128u;
+      const uint32_t q_lo = smem_desc_lo(smem_u32(sQ + t * TILE_BYTES), 16);
+      int ring = 0, ring_round = 0;                // position of the block's K in the ring
+      uint32_t p_phase = 0, q_phase = 0;
       bool ok = true;
       for (int item = blockIdx.x; item < p.items; item += gridDim.x) {
         WindowItem it;
         window_item(p, item, it);
         window_item_blocks(p, it);
         if (lane == 0) {
-          int left[2] = {it.tile[0].count(), it.tile[1].count()};   // blocks whose scores are not issued yet
-          bool pending[2] = {false, false}, begun[2] = {false, false}, has_o[2] = {false, false};
-          for (int u = 0; ok && u <= it.n; ++u) {
-            const int kc = base + 2 * u, vc = kc - 1;               // ring counts of K of block u and V of block u - 1
-            const int ks = kc % kWfStages, vs = (vc + kWfStages) % kWfStages;
-            const int blk = u < it.n ? it.block(u) : -1;
+          const WindowTile tile = t ? it.tile[1] : it.tile[0];
+          int left = tile.count();                 // blocks whose scores are not issued yet
+          bool pending = false, begun = false, has_o = false;
+          int vs = 0, v_round = 0;                 // ring position of V of the block before
+          for (int u = 0; u <= it.n; ++u) {
+            const int ks = ring;
+            const bool mine = u < it.n && tile.has(it.block(u));
+            // what was loaded long ago is waited for first, the only wait that matters (for P) comes last
+            ok = (u == 0 || mbar_wait(&kv_full[vs], v_round & 1, abort_flag)) && (u == it.n || mbar_wait(&kv_full[ks], ring_round & 1, abort_flag));
+            if (!ok) break;
+            if (mine && !begun) {
+              ok = mbar_wait(&q_full[t], q_phase & 1, abort_flag);
+              if (!ok) break;
+              ++q_phase;
+              begun = true;
+            }
+            if (pending) {
+              const uint32_t v_lo = smem_desc_lo(smem_u32(sKV + vs * TILE_BYTES), ATOM_BYTES);
+              const uint32_t acc0 = has_o ? 1u : 0u;
 #pragma unroll
-            for (int t = 0; t < 2; ++t) {
-              if (!ok) continue;
-              const uint32_t s_tmem = tmem_base + S_COL + static_cast<uint32_t>(t) * 128u;
-              if (pending[t]) {
-                ok = mbar_wait(&kv_full[vs], (vc / kWfStages) & 1, abort_flag) && mbar_wait(&p_full[t], p_count[t] & 1, abort_flag);
-                if (!ok) continue;
-                ++p_count[t];
+              for (int half = 0; half < 2; ++half) {
+                ok = ok && mbar_wait(&p_full[2 * t + half], p_phase & 1, abort_flag);
+                if (!ok) break;
                 tc_fence_after();
-                const uint32_t v_lo = smem_desc_lo(smem_u32(sKV + vs * TILE_BYTES), ATOM_BYTES);
-                const uint32_t o_tmem = tmem_base + O_COL + static_cast<uint32_t>(t) * 128u;
-                const uint32_t acc0 = has_o[t] ? 1u : 0u;
 #pragma unroll
-                for (int kk = 0; kk < kWinBlock / 16; ++kk)
+                for (int k2 = 0; k2 < kWinBlock / 32; ++k2) {
+                  const int kk = half * (kWinBlock / 32) + k2;
                   umma_bf16_ts_lh(o_tmem, s_tmem + static_cast<uint32_t>(kk * 8), v_lo + static_cast<uint32_t>(kk * 128), hi, idesc_pv,
                                   kk != 0 ? 1u : acc0);
-                has_o[t] = true;
-                pending[t] = false;
-                if (left[t] == 0) umma_commit(&o_full[t]);
-              }
-              if (blk >= 0 && it.tile[t].has(blk)) {
-                if (!begun[t]) {
-                  ok = mbar_wait(&q_full[t], q_count[t] & 1, abort_flag);
-                  if (!ok) continue;
-                  ++q_count[t];
-                  begun[t] = true;
                 }
-                ok = mbar_wait(&kv_full[ks], (kc / kWfStages) & 1, abort_flag);
-                if (!ok) continue;
-                tc_fence_after();
-                const uint32_t q_lo = smem_desc_lo(smem_u32(sQ + t * TILE_BYTES), 16), k_lo = smem_desc_lo(smem_u32(sKV + ks * TILE_BYTES), 16);
+              }
+              if (!ok) break;
+              ++p_phase;
+              has_o = true;
+            }
+            if (mine) {
+              tc_fence_after();
+              const uint32_t k_lo = smem_desc_lo(smem_u32(sKV + ks * TILE_BYTES), 16);
 #pragma unroll
-                for (int kk = 0; kk < D / 16; ++kk) {
-                  const uint32_t off = static_cast<uint32_t>(((kk >> 2) * ATOM_BYTES + (kk & 3) * 32) >> 4);
-                  umma_bf16_ss_lh(s_tmem, q_lo + off, hi, k_lo + off, hi, idesc_qk, kk != 0 ? 1u : 0u);
-                }
-                umma_commit(&s_full[t]);
-                pending[t] = true;
-                if (--left[t] == 0) umma_commit(&q_empty[t]);
+              for (int kk = 0; kk < D / 16; ++kk) {
+                const uint32_t off = static_cast<uint32_t>(((kk >> 2) * ATOM_BYTES + (kk & 3) * 32) >> 4);
+                umma_bf16_ss_lh(s_tmem, q_lo + off, hi, k_lo + off, hi, idesc_qk, kk != 0 ? 1u : 0u);
               }
-            }
-            if (!ok) break;
-            // A block that no tile needed (a gap of the union) still has to have arrived before its slot is given back.
-            if (u > 0) {
-              ok = mbar_wait(&kv_full[vs], (vc / kWfStages) & 1, abort_flag);
-              if (!ok) break;
-              umma_commit(&kv_empty[vs]);
-            }
-            if (u < it.n) {
-              ok = mbar_wait(&kv_full[ks], (kc / kWfStages) & 1, abort_flag);
-              if (!ok) break;
+              umma_commit(&s_full[t]);
               umma_commit(&kv_empty[ks]);
+              if (--left == 0) umma_commit(&q_empty[t]);
+            } else if (u < it.n) {
+              mbar_arrive(&kv_empty[ks]);          // the other tile's block
+            }
+            if (u > 0) {
+              if (pending) umma_commit(&kv_empty[vs]);
+              else mbar_arrive(&kv_empty[vs]);
+              if (pending && !mine && left == 0) umma_commit(&o_full[t]);
+            }
+            pending = mine;
+            if (u < it.n) {
+              if (++ring == kWfStages) ring = 0, ++ring_round;
+              vs = ring, v_round = ring_round;
+              if (++ring == kWfStages) ring = 0, ++ring_round;
             }
           }
-          base += 2 * it.n;
         }
         ok = __shfl_sync(0xffffffffu, static_cast<int>(ok), 0) != 0;
         if (!ok) break;
@@ -267,6 +309,7 @@ window_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
     const uint32_t s_tmem = tmem_base + S_COL + static_cast<uint32_t>(t) * 128u + t_lane;
     const uint32_t o_tmem = tmem_base + O_COL + static_cast<uint32_t>(t) * 128u + t_lane;
     int s_count = 0, o_count = 0;
+    uint32_t turn_phase = 0;
     bool ok = true;
     for (int item = blockIdx.x; item < p.items; item += gridDim.x) {
       WindowItem it;
@@ -274,7 +317,10 @@ window_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
       const int q0 = it.q0[t], head = it.head[t];
       if (q0 >= p.Sq) continue;                    // the missing second tile
       const WindowTile tile = window_tile(p.rule, it.batch, p.Sq, p.Sk, q0);
+      const WindowTile other = p.pair == 1 ? tile : window_tile(p.rule, it.batch, p.Sq, p.Sk, it.q0[t ^ 1]);
+      const bool paired = p.pair != 0;
       const int n = tile.count();
+      bool owed = false;                           // tile 0: the other tile had the block before too
       const int qi = q0 + row;
       const WindowRow w = window_row(p.rule, it.batch, p.Sk, qi + p.Sk - p.Sq, qi < p.Sq);
       // m_run: the power of two that P is relative to; l_run: sum of the rounded P; x_run: of P as it was before
@@ -290,10 +336,13 @@ window_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
 #pragma unroll
         for (int c = 0; c < 4; ++c) tmem_ld_32x32b_x32(s_tmem + c * 32, reinterpret_cast<uint32_t(&)[32]>(s[c * 32]));
         tmem_ld_wait();
+        uint32_t none = 0;                         // bit c: no row of the warp sees a key of chunk c (of 32)
         if (key0 < tile.full_lo || key0 + kWinBlock - 1 > tile.full_hi) {
 #pragma unroll
           for (int c = 0; c < 4; ++c) {
             const uint32_t seen = window_bits(w, key0 + c * 32);
+            if (__all_sync(0xffffffffu, seen == 0xffffffffu)) continue;
+            if (__all_sync(0xffffffffu, seen == 0u)) none |= 1u << c;
 #pragma unroll
             for (int i = 0; i < 32; ++i)
               if (!((seen >> i) & 1u)) s[c * 32 + i] = __float_as_uint(-INFINITY);
@@ -301,7 +350,9 @@ window_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
         }
         float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-        for (int i = 0; i < 128; ++i) mx[i & 3] = fmaxf(mx[i & 3], __uint_as_float(s[i]));
+        for (int i = 0; i < 128; i += 8)
+#pragma unroll
+          for (int k = 0; k < 4; ++k) mx[k] = fmaxf(fmaxf(mx[k], __uint_as_float(s[i + 2 * k])), __uint_as_float(s[i + 2 * k + 1]));
         const float m_blk = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * p.scale_log2;
         if (__any_sync(0xffffffffu, m_blk > m_run + kWfGrowth)) {
           const float m_new = fmaxf(m_run, ceilf(m_blk));
@@ -321,22 +372,53 @@ window_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
             }
           }
         }
+        // The two tiles take turns with their exponentials: block by block, tile 0 first. Left alone they fall into step, both on
+        // the exponentials and then both on the tensor cores, and neither is hidden.
+        const int blk = tile.block(j);
+        const bool both = paired && other.has(blk);
+        if (t == 0 ? owed : both) {
+          ok = mbar_wait(&turn[t], turn_phase & 1, abort_flag);
+          ok = __all_sync(0xffffffffu, ok);
+          if (!ok) break;
+          ++turn_phase;
+        }
         const float m_safe = m_run == -INFINITY ? 0.f : m_run;
         const uint64_t scale2 = f32x2(p.scale_log2, p.scale_log2), shift2 = f32x2(-m_safe, -m_safe);
         uint64_t sum[2] = {0, 0}, sum_x[2] = {0, 0};
 #pragma unroll
         for (int c = 0; c < 4; ++c) {              // 32 keys: 16 columns of packed P
           uint32_t pk[16];
+          if ((none >> c) & 1u) {
 #pragma unroll
-          for (int i = 0; i < 16; ++i) {
-            float a, b;
-            f32x2_split(fma_f32x2(f32x2(__uint_as_float(s[c * 32 + 2 * i]), __uint_as_float(s[c * 32 + 2 * i + 1])), scale2, shift2), a, b);
-            a = wf_exp2(a), b = wf_exp2(b);
-            pk[i] = pack_bf16x2(a, b);
-            sum[i & 1] = add_f32x2(sum[i & 1], bf16x2_as_f32x2(pk[i]));
-            if (LSE) sum_x[i & 1] = add_f32x2(sum_x[i & 1], f32x2(a, b));
+            for (int i = 0; i < 16; ++i) pk[i] = 0u;
+          } else {
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+              float a, b;
+              const uint64_t x = fma_f32x2(f32x2(__uint_as_float(s[c * 32 + 2 * i]), __uint_as_float(s[c * 32 + 2 * i + 1])), scale2, shift2);
+              if (i % kWfPolyOf < kWfPoly) {
+                wf_exp2_poly(x, a, b);
+              } else {
+                f32x2_split(x, a, b);
+                a = wf_exp2(a), b = wf_exp2(b);
+              }
+              pk[i] = pack_bf16x2(a, b);
+              sum[i & 1] = add_f32x2(sum[i & 1], bf16x2_as_f32x2(pk[i]));
+              if (LSE) sum_x[i & 1] = add_f32x2(sum_x[i & 1], f32x2(a, b));
+            }
           }
           tmem_st_32x32b_x16(s_tmem + c * 16, pk);
+          if (c == 3) {
+            const bool hand_over = t == 0 ? both : both && other.b1 - 1 > blk;
+            owed = both && j + 1 < n;
+            if (hand_over && lane == 0) mbar_arrive(&turn[t ^ 1]);
+          }
+          if (c & 1) {
+            tmem_st_wait();
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&p_full[2 * t + (c >> 1)]);
+          }
         }
         float lo, hi;
         f32x2_split(add_f32x2(sum[0], sum[1]), lo, hi);
@@ -345,10 +427,6 @@ window_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
           f32x2_split(add_f32x2(sum_x[0], sum_x[1]), lo, hi);
           x_run += lo + hi;
         }
-        tmem_st_wait();
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&p_full[t]);
       }
       if (!ok) break;
       // ---------------------------------------------------------------- output
