@@ -6,8 +6,7 @@
 //                came from). A wait that is already satisfied still costs some 250 cycles while UMMAs saturate shared memory, so
 //                each tile has an issuer of its own and no barrier is asked twice,
 //   warps 4-7 and 8-11  one warpgroup per tile, a thread per query row: running maximum and sum, P in bf16, output. P is handed
-//                over in halves of 64 keys, so that O += P V begins under the second half's exponentials; a share of the
-//                exponentials runs on the multiply-add pipe, since the special-function unit alone would take as long as the UMMAs.
+//                over in halves of 64 keys, so that O += P V begins under the second half's exponentials.
 // The two tiles are two query heads of one key/value head on the same rows where the group is even, else neighbouring rows of
 // one head. O is rescaled only when a row's maximum has grown by more than 2^8 since the last rescale: P then stays below 2^8
 // and its bf16 rounding is relative, so nothing is lost, and after the first blocks the rescale hardly ever happens.
@@ -28,7 +27,6 @@ constexpr int kWfStages = 5;                       // K and V blocks in flight
 constexpr int kWfLaunchRegs = 168, kWfOtherRegs = 56, kWfSoftmaxRegs = 224;
 static_assert(128 * kWfOtherRegs + 256 * kWfSoftmaxRegs <= kWfThreads * kWfLaunchRegs, "register split exceeds the launch");
 constexpr float kWfLog2e = 1.4426950408889634f, kWfLn2 = 0.6931471805599453f;
-constexpr int kWfPoly = 2, kWfPolyOf = 8;          // pairs of exponentials on the multiply-add pipe: 2 of every 8
 constexpr float kWfGrowth = 8.f;                   // log2 of how far P may exceed 1 before O is rescaled
 
 struct WindowFwdArgs {
@@ -48,28 +46,6 @@ __device__ __forceinline__ float wf_exp2(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
-}
-
-// 2^x for a pair, x <= 120, on the multiply-add pipe: x = n + f with n the nearest integer (adding 1.5 * 2^23 leaves n in the low
-// bits), 2^f by a polynomial on [-1/2, 1/2], n added to the exponent. The coefficients are the minimax fit of degree 4 to the
-// relative error with p(0) = 1 (solved as a linear programme on a grid): 2.8e-6, far below the bf16 rounding that follows.
-// x below -127 gives exactly 0: there n = -127, f = 0, and the exponent of 1 becomes that of zero.
-__device__ __forceinline__ void wf_exp2_poly(uint64_t x, float& a, float& b) {
-  float lo, hi;
-  f32x2_split(x, lo, hi);
-  x = f32x2(fmaxf(lo, -127.f), fmaxf(hi, -127.f));
-  const uint64_t magic = f32x2(12582912.f, 12582912.f), minus_magic = f32x2(-12582912.f, -12582912.f), minus_one = f32x2(-1.f, -1.f);
-  const uint64_t t = add_f32x2(x, magic);
-  const uint64_t f = fma_f32x2(add_f32x2(t, minus_magic), minus_one, x);
-  uint64_t r = fma_f32x2(f32x2(0.009582576341927052f, 0.009582576341927052f), f, f32x2(0.05590682849287987f, 0.05590682849287987f));
-  r = fma_f32x2(r, f, f32x2(0.24024106562137604f, 0.24024106562137604f));
-  r = fma_f32x2(r, f, f32x2(0.6931241154670715f, 0.6931241154670715f));
-  r = fma_f32x2(r, f, f32x2(1.f, 1.f));
-  float ta, tb, ra, rb;
-  f32x2_split(t, ta, tb);
-  f32x2_split(r, ra, rb);
-  a = __uint_as_float(__float_as_uint(ra) + (__float_as_uint(ta) << 23));
-  b = __uint_as_float(__float_as_uint(rb) + (__float_as_uint(tb) << 23));
 }
 
 struct WindowItem {
@@ -396,12 +372,8 @@ window_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
             for (int i = 0; i < 16; ++i) {
               float a, b;
               const uint64_t x = fma_f32x2(f32x2(__uint_as_float(s[c * 32 + 2 * i]), __uint_as_float(s[c * 32 + 2 * i + 1])), scale2, shift2);
-              if (i % kWfPolyOf < kWfPoly) {
-                wf_exp2_poly(x, a, b);
-              } else {
-                f32x2_split(x, a, b);
-                a = wf_exp2(a), b = wf_exp2(b);
-              }
+              f32x2_split(x, a, b);
+              a = wf_exp2(a), b = wf_exp2(b);
               pk[i] = pack_bf16x2(a, b);
               sum[i & 1] = add_f32x2(sum[i & 1], bf16x2_as_f32x2(pk[i]));
               if (LSE) sum_x[i & 1] = add_f32x2(sum_x[i & 1], f32x2(a, b));
