@@ -15,16 +15,13 @@
 //   flash_bwd_dq_kernel     one CTA per 128 query rows of one (batch, head): loops over 128-key blocks, S double-buffered
 //                           in TMEM, dS written over S as the A operand of dQ += dS K.
 // dK/dV and dQ are each owned by exactly one CTA: no atomics, results are deterministic. Masks and GQA as in the
-// forward (mode 0 all visible, 1 causal with offset, 2 positions + sequence ids, 3 causal by index + same sequence id);
-// mode 4 is the sliding window with first tokens of window.cuh: its CTAs visit only the blocks that the rule reaches, and heads
-// that are divided over CTAs are summed in a fixed order.
+// forward (mode 0 all visible, 1 causal with offset, 2 positions + sequence ids, 3 causal by index + same sequence id).
 // Every wait is bounded (see ptx.cuh). The reference gets this op from the flash-attn 2 package
 // (runtime/layers/flash_utils.py:218-260) or from autograd through SDPA.
 #include <cstdlib>
 
 #include "host.h"
 #include "ptx.cuh"
-#include "window.cuh"
 
 namespace mb {
 
@@ -52,11 +49,8 @@ struct FlashBwdArgs {
   float scale, scale_log2;
   int* status;
   int split;                // dK/dV kernel: the query heads of a group are divided over `split` CTAs (1 = no split)
-  float* dk_tmp;            // split > 1: fp32 [B, Sk, Hkv, D] sums the CTAs add their parts to (mode 4: one such plane a part)
+  float* dk_tmp;            // split > 1: fp32 [B, Sk, Hkv, D] sums the CTAs add their parts to
   float* dv_tmp;
-  long long plane;          // elements of a plane (mode 4)
-  WindowRule rule;          // mode 4
-  const void* out_lo;       // mode 4: what the rounding of the output left
   int dbg;                  // probe builds only: bit 0 skip the S/dP UMMAs, bit 1 skip the accumulation UMMAs, bit 2 skip the arithmetic
 };
 
@@ -84,10 +78,9 @@ __device__ __forceinline__ float bw_exp2(float x) {
 }
 
 // ---------------------------------------------------------------------------------------------- preprocessing
-// One warp per (batch, head, query row): delta = sum_d out * dout; lse2 = lse * log2(e). LO (mode 4): out comes with what its
-// rounding left, and the statistics are in the exp2 domain already.
-template <int D, bool LO>
-__global__ void flash_bwd_prep_kernel(const __nv_bfloat16* __restrict__ out, const __nv_bfloat16* __restrict__ out_lo, const __nv_bfloat16* __restrict__ dout,
+// One warp per (batch, head, query row): delta = sum_d out * dout; lse2 = lse * log2(e).
+template <int D>
+__global__ void flash_bwd_prep_kernel(const __nv_bfloat16* __restrict__ out, const __nv_bfloat16* __restrict__ dout,
                                       long long o_tstride, long long o_bstride, long long do_tstride, long long do_bstride,
                                       const float* __restrict__ lse, float* __restrict__ lse2, float* __restrict__ delta,
                                       int B, int Sq, int Hq, int Sq_pad) {
@@ -101,24 +94,18 @@ __global__ void flash_bwd_prep_kernel(const __nv_bfloat16* __restrict__ out, con
   float acc = 0.f, l2 = INFINITY;
   if (qi < Sq) {
     constexpr int PER = D / 32;   // 2 or 4 bf16 per lane
-    const long long o_at = b * o_bstride + qi * o_tstride + static_cast<long long>(h) * D + lane * PER;
-    const __nv_bfloat16* po = out + o_at;
+    const __nv_bfloat16* po = out + b * o_bstride + qi * o_tstride + static_cast<long long>(h) * D + lane * PER;
     const __nv_bfloat16* pd = dout + b * do_bstride + qi * do_tstride + static_cast<long long>(h) * D + lane * PER;
 #pragma unroll
     for (int i = 0; i < PER; i += 2) {
       const __nv_bfloat162 a = *reinterpret_cast<const __nv_bfloat162*>(po + i);
       const __nv_bfloat162 g = *reinterpret_cast<const __nv_bfloat162*>(pd + i);
-      float ax = __bfloat162float(a.x), ay = __bfloat162float(a.y);
-      if (LO) {
-        const __nv_bfloat162 l = *reinterpret_cast<const __nv_bfloat162*>(out_lo + o_at + i);
-        ax += __bfloat162float(l.x), ay += __bfloat162float(l.y);
-      }
-      acc += ax * __bfloat162float(g.x) + ay * __bfloat162float(g.y);
+      acc += __bfloat162float(a.x) * __bfloat162float(g.x) + __bfloat162float(a.y) * __bfloat162float(g.y);
     }
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) acc += __shfl_xor_sync(0xffffffffu, acc, o);
     const float l = lse[(static_cast<long long>(b) * Hq + h) * Sq + qi];
-    l2 = (l == -INFINITY) ? INFINITY : LO ? l : l * kBwLog2e;
+    l2 = (l == -INFINITY) ? INFINITY : l * kBwLog2e;
   }
   if (lane == 0) {
     lse2[warp_global] = l2;
@@ -222,19 +209,12 @@ flash_bwd_dkdv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_cons
 
   // query sub-blocks this key block has to visit
   const int n_qsub_all = (p.Sq + kQSub - 1) / kQSub;
-  int qb_start = 0, qb_end = n_qsub_all;
-  int full_hi = 0;                                   // mode 4: see WindowKeys
-  if (MODE == 4) {
-    const WindowKeys wk = window_keys(p.rule, batch, p.Sq, p.Sk, k0);
-    qb_start = wk.q_lo / kQSub;
-    qb_end = (wk.q_hi + kQSub - 1) / kQSub;
-    full_hi = wk.full_hi;
-  }
+  int qb_start = 0;
   if (causal) {
     const int first_q = k0 - causal_off;             // first query row that sees key k0
     qb_start = first_q <= 0 ? 0 : first_q / kQSub;
   }
-  const int n_sub = qb_start < qb_end ? qb_end - qb_start : 0;
+  const int n_sub = qb_start < n_qsub_all ? n_qsub_all - qb_start : 0;
   const int n_iter = n_sub * heads_here;
 
   if (threadIdx.x == 0) {
@@ -274,7 +254,7 @@ flash_bwd_dkdv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_cons
         tma_load_4d(sK + a * (kKvRows * 128), &tmK, kv_full, a * 64, kv_head, k0, batch);
         tma_load_4d(sV + a * (kKvRows * 128), &tmV, kv_full, a * 64, kv_head, k0, batch);
       }
-      constexpr bool with_ids = MODE == 2 || MODE == 3;
+      constexpr bool with_ids = MODE >= 2;
       for (int it = 0; it < n_iter; ++it) {
         const int st = it % kQStages;
         if (!mbar_wait(&q_empty[st], ((it / kQStages) & 1) ^ 1, abort_flag)) break;
@@ -375,13 +355,7 @@ flash_bwd_dkdv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_cons
     const bool key_valid = kj < p.Sk;
     const uint32_t t_lane = static_cast<uint32_t>(qw * 32) << 16;
     int my_pos = 0, my_seq = 0;
-    int my_upper = 0;                             // mode 4: queries at positions [kj, my_upper) see this key
-    if (MODE == 4 && key_valid) {
-      const long long at = static_cast<long long>(batch) * p.Sk + kj;
-      const int start = p.rule.starts ? p.rule.starts[at] : 0;
-      if (start != kWinNone) my_upper = window_upper(p.rule, start, p.rule.starts ? p.rule.ends[at] : p.Sk, kj);
-    }
-    if (MODE == 2 || MODE == 3) {
+    if (MODE >= 2) {
       const long long at = static_cast<long long>(batch) * p.Sk_pad + kj;   // padded: always in range
       my_pos = p.kpos[at];
       my_seq = p.kseq[at];
@@ -423,15 +397,14 @@ flash_bwd_dkdv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_cons
       MB_PROBE(warp == 2 && lane == 0, it, 5);
       const int qsub0 = (qb_start + it % n_sub) * kQSub;      // first query row of the sub-block
       // does this sub-block contain a masked pair? (warp-uniform)
-      bool need_mask = (k0 + kKvRows > p.Sk) || MODE == 2 || MODE == 3;
-      if (MODE == 4) need_mask = qsub0 + causal_off < k0 + kKvRows - 1 || qsub0 + kQSub + causal_off > full_hi;
+      bool need_mask = (k0 + kKvRows > p.Sk) || MODE >= 2;
       if (causal) need_mask = need_mask || (k0 + kKvRows - 1 > qsub0 + causal_off);
       float pr[16];
 #pragma unroll
       for (int c = 0; c < 16; ++c) pr[c] = MB_DBG(5) ? __uint_as_float(s[c]) : bw_exp2(fmaf(__uint_as_float(s[c]), scale_log2, -lse[c]));
       if (need_mask) {
         int qp[16], qs[16];
-        if (MODE == 2 || MODE == 3) {
+        if (MODE >= 2) {
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
             const int4 a = *reinterpret_cast<const int4*>(aux + 2 * kQSub * 4 + i * 16);
@@ -444,10 +417,9 @@ flash_bwd_dkdv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_cons
 #pragma unroll
         for (int c = 0; c < 16; ++c) {
           bool vis = key_valid;
-          if (causal || MODE == 4) vis = vis && (kj <= q_first + c);
-          if (MODE == 4) vis = vis && (q_first + c < my_upper);
+          if (causal) vis = vis && (kj <= q_first + c);
           if (MODE == 2) vis = vis && (my_pos <= qp[c]);
-          if (MODE == 2 || MODE == 3) vis = vis && (my_seq == qs[c]) && (my_seq != -1);
+          if (MODE >= 2) vis = vis && (my_seq == qs[c]) && (my_seq != -1);
           pr[c] = vis ? pr[c] : 0.f;
         }
       }
@@ -487,9 +459,7 @@ flash_bwd_dkdv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_cons
           tmem_ld_32x32b_x16(tmem_base + DV_COL + static_cast<uint32_t>(grp * QUART_D + c0) + t_lane, r);
           tmem_ld_wait();
           if (key_valid) {
-            if (MODE == 4 && p.split > 1) {
-              store_row_chunk(p.dv_tmp + part * p.plane, toff + c0, r, 1.f, true, false);
-            } else if (p.split > 1) {
+            if (p.split > 1) {
 #pragma unroll
               for (int i = 0; i < 16; ++i) atomicAdd(p.dv_tmp + toff + c0 + i, __uint_as_float(r[i]));
             } else {
@@ -499,9 +469,7 @@ flash_bwd_dkdv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_cons
           tmem_ld_32x32b_x16(tmem_base + DK_COL + static_cast<uint32_t>(grp * QUART_D + c0) + t_lane, r);
           tmem_ld_wait();
           if (key_valid) {
-            if (MODE == 4 && p.split > 1) {
-              store_row_chunk(p.dk_tmp + part * p.plane, toff + c0, r, p.scale, true, false);
-            } else if (p.split > 1) {
+            if (p.split > 1) {
 #pragma unroll
               for (int i = 0; i < 16; ++i) atomicAdd(p.dk_tmp + toff + c0 + i, __uint_as_float(r[i]) * p.scale);
             } else {
@@ -509,9 +477,6 @@ flash_bwd_dkdv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_cons
             }
           }
         }
-      } else if (MODE == 4 && key_valid && p.split > 1) {
-        store_row_zero(p.dv_tmp + part * p.plane, toff, QUART_D, true);
-        store_row_zero(p.dk_tmp + part * p.plane, toff, QUART_D, true);
       } else if (key_valid && !p.accumulate && p.split == 1) {
         store_row_zero(p.dv, off, QUART_D, p.out_fp32 != 0);
         store_row_zero(p.dk, off, QUART_D, p.out_fp32 != 0);
@@ -535,20 +500,15 @@ flash_bwd_dkdv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_cons
   }
 }
 
-// fp32 sums [planes, tokens, hd] of a split dK/dV launch -> the caller's outputs (bf16 or fp32, token stride `tstride`).
+// fp32 sums [tokens, hd] of a split dK/dV launch -> the caller's outputs (bf16 or fp32, token stride `tstride`).
 __global__ void flash_bwd_finish_split_kernel(const float* __restrict__ dk_tmp, const float* __restrict__ dv_tmp, void* dk, void* dv,
-                                              long long tokens, int hd, long long tstride, int out_fp32, int accumulate, int planes) {
+                                              long long tokens, int hd, long long tstride, int out_fp32, int accumulate) {
   const long long i4 = (static_cast<long long>(blockIdx.x) * blockDim.x + threadIdx.x) * 4;
   if (i4 >= tokens * hd) return;
   const long long t = i4 / hd;
   const int c = static_cast<int>(i4 - t * hd);
   const long long o = t * tstride + c;
-  float4 a = *reinterpret_cast<const float4*>(dk_tmp + i4), b = *reinterpret_cast<const float4*>(dv_tmp + i4);
-  for (int q = 1; q < planes; ++q) {               // in the parts' order: the same bits every time
-    const float4 x = *reinterpret_cast<const float4*>(dk_tmp + q * tokens * hd + i4), y = *reinterpret_cast<const float4*>(dv_tmp + q * tokens * hd + i4);
-    a.x += x.x, a.y += x.y, a.z += x.z, a.w += x.w;
-    b.x += y.x, b.y += y.y, b.z += y.z, b.w += y.w;
-  }
+  const float4 a = *reinterpret_cast<const float4*>(dk_tmp + i4), b = *reinterpret_cast<const float4*>(dv_tmp + i4);
   if (out_fp32) {
     float4* pk = reinterpret_cast<float4*>(static_cast<float*>(dk) + o);
     float4* pv = reinterpret_cast<float4*>(static_cast<float*>(dv) + o);
@@ -597,9 +557,8 @@ flash_bwd_dq_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_consta
   // the tensor-map loads are slow enough (64 KB take ~1400 cycles) that K needs three stages to stay ahead. With Q and
   // dO resident that fills the shared memory of the SM, so the dynamic window must start 1024-byte aligned (checked).
   // (The masks that need per-key ids keep two K stages at head_dim 128: their id arrays take the remaining space.)
-  constexpr bool with_ids = MODE == 2 || MODE == 3;
-  constexpr int K_STAGES = (D == 128) ? (with_ids ? 2 : 3) : 4;
-  constexpr int AUX_STAGES = with_ids ? K_STAGES : 0;
+  constexpr int K_STAGES = (D == 128) ? (MODE >= 2 ? 2 : 3) : 4;
+  constexpr int AUX_STAGES = MODE >= 2 ? K_STAGES : 0;
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   uint8_t* smem = smem_raw;
   uint8_t* sQ = smem;
@@ -634,12 +593,6 @@ flash_bwd_dq_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_consta
     const int last_key = min(q0 + kDqRows - 1, p.Sq - 1) + causal_off;
     n_blocks = last_key < 0 ? 0 : min(n_blocks, last_key / kDqKeys + 1);
   }
-  WindowTile wt{};                                  // mode 4: the key blocks this tile visits
-  if (MODE == 4) {
-    wt = window_tile(p.rule, batch, p.Sq, p.Sk, q0);
-    n_blocks = wt.count();
-  }
-  auto key_block = [&](int j) { return MODE == 4 ? wt.block(j) : j; };
 
   if (smem_u32(smem_raw) & 1023u) {   // uniform over the CTA: nothing has been set up yet
     if (threadIdx.x == 0) {
@@ -689,13 +642,14 @@ flash_bwd_dq_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_consta
         tma_load_4d(sQ + a * (kDqRows * 128), &tmQ, q_full, a * 64, head, q0, batch);
         tma_load_4d(sDO + a * (kDqRows * 128), &tmDO, q_full, a * 64, head, q0, batch);
       }
+      constexpr bool with_ids = MODE >= 2;
       for (int j = 0; j < n_blocks; ++j) {
         const int ks = j % K_STAGES, vs = j & 1;
         if (!mbar_wait(&k_empty[ks], ((j / K_STAGES) & 1) ^ 1, abort_flag)) break;
         mbar_arrive_expect_tx(&k_full[ks], TILE_BYTES + (with_ids ? AUX_BYTES : 0));
 #pragma unroll
         for (int a = 0; a < ATOMS; ++a)
-          tma_load_4d(sK + ks * TILE_BYTES + a * (kDqKeys * 128), &tmK, &k_full[ks], a * 64, kv_head, key_block(j) * kDqKeys, batch);
+          tma_load_4d(sK + ks * TILE_BYTES + a * (kDqKeys * 128), &tmK, &k_full[ks], a * 64, kv_head, j * kDqKeys, batch);
         if (with_ids) {
           const long long prow = static_cast<long long>(batch) * p.Sk_pad + j * kDqKeys;
           bulk_load(sAux + ks * AUX_BYTES, p.kpos + prow, kDqKeys * 4, &k_full[ks]);
@@ -705,7 +659,7 @@ flash_bwd_dq_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_consta
         mbar_arrive_expect_tx(&v_full[vs], TILE_BYTES);
 #pragma unroll
         for (int a = 0; a < ATOMS; ++a)
-          tma_load_4d(sV + vs * TILE_BYTES + a * (kDqKeys * 128), &tmV, &v_full[vs], a * 64, kv_head, key_block(j) * kDqKeys, batch);
+          tma_load_4d(sV + vs * TILE_BYTES + a * (kDqKeys * 128), &tmV, &v_full[vs], a * 64, kv_head, j * kDqKeys, batch);
       }
     }
     __syncwarp();
@@ -809,19 +763,12 @@ flash_bwd_dq_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_consta
     const float my_lse = p.lse2[arow];
     const float my_delta = p.delta[arow];
     int my_pos = 0, my_seq = 0;
-    WindowRow wr{};
-    if (MODE == 4) wr = window_row(p.rule, batch, p.Sk, qi + causal_off, row_valid);
-    if (with_ids) {
+    if (MODE >= 2) {
       const long long at = static_cast<long long>(batch) * p.Sq_pad + qi;
       my_pos = p.qpos[at];
       my_seq = p.qseq[at];
     }
     const float scale_log2 = p.scale_log2;
-    // Mode 4 takes the forward's own rounded weights, so that the terms of dS cancel as exactly as there: weights relative to a
-    // whole power of two (the forward's differ from it by another such factor), rounded to bf16, times what is left of 2^-lse.
-    const float my_shift = MODE == 4 ? floorf(my_lse) : my_lse;
-    const float my_factor = MODE == 4 && my_lse != INFINITY ? bw_exp2(my_shift - my_lse) : 0.f;
-    const float my_offset = my_delta * my_factor;
     bool ok = true;
     for (int j = 0; j < n_blocks; ++j) {
       const int s = j & 1;
@@ -841,27 +788,19 @@ flash_bwd_dq_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_consta
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive(dp_free);        // this warp's dP columns are in registers: the next block's dP may be issued
-      const int key0 = key_block(j) * kDqKeys + grp * 32;
-      bool need_mask = (j * kDqKeys + kDqKeys > p.Sk) || with_ids;
-      if (MODE == 4) need_mask = key0 < wt.full_lo || key0 + 31 > wt.full_hi;
+      const int key0 = j * kDqKeys + grp * 32;
+      bool need_mask = (j * kDqKeys + kDqKeys > p.Sk) || MODE >= 2;
       if (causal) need_mask = need_mask || (j * kDqKeys + kDqKeys - 1 > q0 + causal_off);
       float pr[32];
 #pragma unroll
-      for (int c = 0; c < 32; ++c) pr[c] = bw_exp2(fmaf(__uint_as_float(sc[c]), scale_log2, -my_shift));
-      if (MODE == 4) {
-        if (need_mask) {
-          const uint32_t seen = window_bits(wr, key0);
-#pragma unroll
-          for (int c = 0; c < 32; ++c)
-            if (!((seen >> c) & 1u)) pr[c] = 0.f;
-        }
-      } else if (need_mask) {
+      for (int c = 0; c < 32; ++c) pr[c] = bw_exp2(fmaf(__uint_as_float(sc[c]), scale_log2, -my_lse));
+      if (need_mask) {
         const uint8_t* aux = sAux + (j % K_STAGES) * AUX_BYTES + grp * 128;
         const int q_lim = qi + causal_off - key0;   // column c visible (causal modes) iff c <= q_lim
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
           int4 kp = make_int4(0, 0, 0, 0), ks = make_int4(0, 0, 0, 0);
-          if (with_ids) {
+          if (MODE >= 2) {
             kp = *reinterpret_cast<const int4*>(aux + i * 16);
             ks = *reinterpret_cast<const int4*>(aux + kDqKeys * 4 + i * 16);
           }
@@ -872,24 +811,15 @@ flash_bwd_dq_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_consta
             bool vis = key0 + c < p.Sk;
             if (causal) vis = vis && (c <= q_lim);
             if (MODE == 2) vis = vis && (kpv[u] <= my_pos);
-            if (with_ids) vis = vis && (ksv[u] == my_seq) && (ksv[u] != -1);
+            if (MODE >= 2) vis = vis && (ksv[u] == my_seq) && (ksv[u] != -1);
             pr[c] = vis ? pr[c] : 0.f;
           }
         }
       }
       uint32_t dsp[16];
 #pragma unroll
-      for (int c = 0; c < 32; c += 2) {
-        if (MODE == 4) {
-          const uint32_t w = pack_bf16x2(pr[c], pr[c + 1]);
-          const uint64_t t = fma_f32x2(f32x2(__uint_as_float(dp[c]), __uint_as_float(dp[c + 1])), f32x2(my_factor, my_factor), f32x2(-my_offset, -my_offset));
-          float a, b;
-          f32x2_split(mul_f32x2(bf16x2_as_f32x2(w), t), a, b);
-          dsp[c >> 1] = pack_bf16x2(a, b);
-        } else {
-          dsp[c >> 1] = pack_bf16x2(pr[c] * (__uint_as_float(dp[c]) - my_delta), pr[c + 1] * (__uint_as_float(dp[c + 1]) - my_delta));
-        }
-      }
+      for (int c = 0; c < 32; c += 2)
+        dsp[c >> 1] = pack_bf16x2(pr[c] * (__uint_as_float(dp[c]) - my_delta), pr[c + 1] * (__uint_as_float(dp[c + 1]) - my_delta));
       MB_PROBE(warp == 2 && lane == 0, j, 10);
       tmem_st_32x32b_x16(t_s, dsp);               // dS over the first half of this thread's own score columns
       tmem_st_wait();
@@ -939,7 +869,7 @@ flash_bwd_dq_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_consta
 
 template <int D, int MODE>
 static int launch_flash_bwd(const void* q, long long q_tstride, long long q_bstride, const void* k, const void* v,
-                            long long kv_tstride, long long kv_bstride, long long v_tstride, long long v_bstride, const void* out, long long o_tstride, long long o_bstride,
+                            long long kv_tstride, long long kv_bstride, const void* out, long long o_tstride, long long o_bstride,
                             const void* dout, long long do_tstride, long long do_bstride, const float* lse, const int* q_pos,
                             const int* k_pos, const int* q_seq, const int* k_seq, float* scratch, FlashBwdArgs a,
                             cudaStream_t stream) {
@@ -956,19 +886,18 @@ static int launch_flash_bwd(const void* q, long long q_tstride, long long q_bstr
   const long long kv_elems = static_cast<long long>(a.B) * a.Sk * a.Hkv * D;
   if (a.split > 1) {
     a.dk_tmp = reinterpret_cast<float*>(kseq + static_cast<long long>(a.B) * a.Sk_pad);
-    a.dv_tmp = a.dk_tmp + kv_elems * (MODE == 4 ? a.split : 1);
-    a.plane = kv_elems;
-    if (MODE != 4) MB_CHECK_CUDA(cudaMemsetAsync(a.dk_tmp, 0, sizeof(float) * 2 * kv_elems, stream));
+    a.dv_tmp = a.dk_tmp + kv_elems;
+    MB_CHECK_CUDA(cudaMemsetAsync(a.dk_tmp, 0, sizeof(float) * 2 * kv_elems, stream));
   }
   {
     const long long threads = n_rows * 32;
     const int block = 256;
-    flash_bwd_prep_kernel<D, MODE == 4><<<static_cast<unsigned>((threads + block - 1) / block), block, 0, stream>>>(
-        static_cast<const __nv_bfloat16*>(out), static_cast<const __nv_bfloat16*>(a.out_lo), static_cast<const __nv_bfloat16*>(dout), o_tstride, o_bstride, do_tstride,
+    flash_bwd_prep_kernel<D><<<static_cast<unsigned>((threads + block - 1) / block), block, 0, stream>>>(
+        static_cast<const __nv_bfloat16*>(out), static_cast<const __nv_bfloat16*>(dout), o_tstride, o_bstride, do_tstride,
         do_bstride, lse, lse2, delta, a.B, a.Sq, a.Hq, a.Sq_pad);
     count_launch();
   }
-  if (MODE == 2 || MODE == 3) {
+  if (MODE >= 2) {
     const int block = 256;
     const long long nq = static_cast<long long>(a.B) * a.Sq_pad, nk = static_cast<long long>(a.B) * a.Sk_pad;
     const unsigned gq = static_cast<unsigned>((nq + block - 1) / block), gk = static_cast<unsigned>((nk + block - 1) / block);
@@ -993,15 +922,13 @@ static int launch_flash_bwd(const void* q, long long q_tstride, long long q_bstr
   {
     const uint64_t dims[4] = {(uint64_t)D, (uint64_t)a.Hkv, (uint64_t)a.Sk, (uint64_t)a.B};
     const uint64_t strides[3] = {(uint64_t)D * 2, (uint64_t)kv_tstride * 2, (uint64_t)kv_bstride * 2};
-    const uint64_t v_strides[3] = {(uint64_t)D * 2, (uint64_t)v_tstride * 2, (uint64_t)v_bstride * 2};
     const uint32_t box128[4] = {64, 1, 128, 1};
-    if (!encode_tmap_4d(&tmK, k, dims, strides, box128, 2, true) || !encode_tmap_4d(&tmV, v, dims, v_strides, box128, 2, true))
+    if (!encode_tmap_4d(&tmK, k, dims, strides, box128, 2, true) || !encode_tmap_4d(&tmV, v, dims, strides, box128, 2, true))
       return -5;
   }
   constexpr size_t smem_dkdv = 1024 + 2 * (kKvRows * D * 2) + 2 * kQStages * (kQSub * D * 2) + kQStages * (4 * kQSub * 4) + 256;
-  constexpr bool with_ids = MODE == 2 || MODE == 3;
-  constexpr int k_stages = (D == 128) ? (with_ids ? 2 : 3) : 4;
-  constexpr size_t smem_dq = (4 + k_stages) * (128 * D * 2) + (with_ids ? k_stages : 0) * (2 * kDqKeys * 4) + 256;
+  constexpr int k_stages = (D == 128) ? (MODE >= 2 ? 2 : 3) : 4;
+  constexpr size_t smem_dq = (4 + k_stages) * (128 * D * 2) + (MODE >= 2 ? k_stages : 0) * (2 * kDqKeys * 4) + 256;
   static bool configured[64] = {false};   // one flag set per (D, MODE) instantiation
   int dev = 0;
   cudaGetDevice(&dev);
@@ -1017,7 +944,7 @@ static int launch_flash_bwd(const void* q, long long q_tstride, long long q_bstr
     if (a.split > 1) {
       const long long quads = kv_elems / 4;
       flash_bwd_finish_split_kernel<<<static_cast<unsigned>((quads + 255) / 256), 256, 0, stream>>>(
-          a.dk_tmp, a.dv_tmp, a.dk, a.dv, static_cast<long long>(a.B) * a.Sk, a.Hkv * D, a.dkv_tstride, a.out_fp32, a.accumulate, MODE == 4 ? a.split : 1);
+          a.dk_tmp, a.dv_tmp, a.dk, a.dv, static_cast<long long>(a.B) * a.Sk, a.Hkv * D, a.dkv_tstride, a.out_fp32, a.accumulate);
       count_launch();
     }
   }
@@ -1091,7 +1018,7 @@ MB_API int mb_flash_attn_bwd(const void* q, long long q_tstride, long long q_bst
 #ifdef MB_FLASH_PROBE
   a.dbg = getenv("MB_FLASH_DBG") ? atoi(getenv("MB_FLASH_DBG")) : 0;
 #endif
-#define MB_BWD_ARGS q, q_tstride, q_bstride, k, v, kv_tstride, kv_bstride, kv_tstride, kv_bstride, out, o_tstride, o_bstride, dout, do_tstride, do_bstride, \
+#define MB_BWD_ARGS q, q_tstride, q_bstride, k, v, kv_tstride, kv_bstride, out, o_tstride, o_bstride, dout, do_tstride, do_bstride, \
                     lse, q_pos, k_pos, q_seq, k_seq, scratch, a, stream
   if (D == 128) {
     switch (mode) {
@@ -1108,52 +1035,4 @@ MB_API int mb_flash_attn_bwd(const void* q, long long q_tstride, long long q_bst
     default: return launch_flash_bwd<64, 3>(MB_BWD_ARGS);
   }
 #undef MB_BWD_ARGS
-}
-
-// Words of scratch memory mb_window_attn_bwd needs for these sizes.
-MB_API long long mb_window_attn_bwd_scratch_words(int B, int Sq, int Sk, int Hq, int Hkv, int D) {
-  const long long sq_pad = (static_cast<long long>(Sq) + 127) / 128 * 128, sk_pad = (static_cast<long long>(Sk) + 127) / 128 * 128;
-  long long words = 2 * B * Hq * sq_pad + 2 * B * sq_pad + 2 * B * sk_pad;
-  if (Hkv >= 1 && Hq % Hkv == 0) {
-    const int split = mb::dkdv_split(B, Sk, Hq, Hkv);
-    if (split > 1) words += 2ll * split * B * Sk * Hkv * D;   // a plane of dK and of dV for every part
-  }
-  return words;
-}
-
-// Backward of mb_window_attn_fwd. q, k, v, out, out_lo, lse2 as there, dout with strides of its own, dq / dk / dv bf16 contiguous.
-// starts, ends: mb_document_bounds of the key rows, or both null. scratch: mb_window_attn_bwd_scratch_words() words.
-MB_API int mb_window_attn_bwd(const void* q, long long q_tstride, long long q_bstride, const void* k, long long k_tstride,
-                              long long k_bstride, const void* v, long long v_tstride, long long v_bstride, const void* out,
-                              const void* out_lo, const void* dout, long long do_tstride, long long do_bstride, const float* lse2, void* dq,
-                              void* dk, void* dv, const int* starts, const int* ends, float* scratch, int B, int Sq, int Sk, int Hq, int Hkv,
-                              int D, int window, int sinks, float scale, cudaStream_t stream) {
-  using namespace mb;
-  const long long strides[] = {q_tstride, q_bstride, k_tstride, k_bstride, v_tstride, v_bstride, do_tstride, do_bstride};
-  const void* pointers[] = {q, k, v, out, out_lo, dout, dq, dk, dv, scratch};
-  if (const char* what = window_attn_problem(B, Sq, Sk, Hq, Hkv, D, window, sinks, strides, 8, pointers, 10)) {
-    set_last_error(what);
-    return -1;
-  }
-  if ((starts == nullptr) != (ends == nullptr)) {
-    set_last_error("mb_window_attn_bwd: starts and ends come together");
-    return -2;
-  }
-  int* status = status_ptr();
-  if (!status) return -4;
-  FlashBwdArgs a{};
-  a.dq = dq, a.dk = dk, a.dv = dv, a.out_lo = out_lo;
-  a.dq_tstride = static_cast<long long>(Hq) * D, a.dkv_tstride = static_cast<long long>(Hkv) * D;
-  a.B = B, a.Sq = Sq, a.Sk = Sk, a.Hq = Hq, a.Hkv = Hkv;
-  a.Sq_pad = (Sq + 127) / 128 * 128, a.Sk_pad = (Sk + 127) / 128 * 128;
-  a.mode = 4;
-  a.scale = scale, a.scale_log2 = scale * kBwLog2e;
-  a.rule = {starts, ends, window < Sk ? window : Sk, sinks < Sk ? sinks : Sk};
-  a.status = status;
-  const long long o_tstride = static_cast<long long>(Hq) * D, o_bstride = o_tstride * Sq;
-  if (D == 128)
-    return launch_flash_bwd<128, 4>(q, q_tstride, q_bstride, k, v, k_tstride, k_bstride, v_tstride, v_bstride, out, o_tstride, o_bstride,
-                                    dout, do_tstride, do_bstride, lse2, nullptr, nullptr, nullptr, nullptr, scratch, a, stream);
-  return launch_flash_bwd<64, 4>(q, q_tstride, q_bstride, k, v, k_tstride, k_bstride, v_tstride, v_bstride, out, o_tstride, o_bstride,
-                                 dout, do_tstride, do_bstride, lse2, nullptr, nullptr, nullptr, nullptr, scratch, a, stream);
 }

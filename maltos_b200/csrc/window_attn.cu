@@ -286,6 +286,7 @@ window_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
     const uint32_t o_tmem = tmem_base + O_COL + static_cast<uint32_t>(t) * 128u + t_lane;
     int s_count = 0, o_count = 0;
     uint32_t turn_phase = 0;
+    bool owed = false;                             // tile 0: the other tile had its last block too, and hands the turn back
     bool ok = true;
     for (int item = blockIdx.x; item < p.items; item += gridDim.x) {
       WindowItem it;
@@ -296,7 +297,6 @@ window_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
       const WindowTile other = p.pair == 1 ? tile : window_tile(p.rule, it.batch, p.Sq, p.Sk, it.q0[t ^ 1]);
       const bool paired = p.pair != 0;
       const int n = tile.count();
-      bool owed = false;                           // tile 0: the other tile had the block before too
       const int qi = q0 + row;
       const WindowRow w = window_row(p.rule, it.batch, p.Sk, qi + p.Sk - p.Sq, qi < p.Sq);
       // m_run: the power of two that P is relative to; l_run: sum of the rounded P; x_run: of P as it was before
@@ -381,9 +381,9 @@ window_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
           }
           tmem_st_32x32b_x16(s_tmem + c * 16, pk);
           if (c == 3) {
-            const bool hand_over = t == 0 ? both : both && other.b1 - 1 > blk;
-            owed = both && j + 1 < n;
-            if (hand_over && lane == 0) mbar_arrive(&turn[t ^ 1]);
+            // one arrival and one wait each way for every block that both have, so neither barrier gets two phases ahead
+            owed = both;
+            if (both && lane == 0) mbar_arrive(&turn[t ^ 1]);
           }
           if (c & 1) {
             tmem_st_wait();

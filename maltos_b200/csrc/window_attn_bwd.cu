@@ -1,0 +1,1021 @@
+// Backward of sliding-window attention for sm_100a (rule: window.cuh, forward: window_attn.cu):
+//   P = 2^(c S - lse2),  dP = dO V^T,  dS = P * (dP - delta),  delta = rowsum(dO * (out + out_lo)),
+//   dV = P^T dO,  dK = scale * dS^T Q,  dQ = scale * dS K.
+// Launches:
+//   window_bwd_prep_kernel    delta and lse2, padded to whole tiles (padding rows get lse2 = +inf, so their P is zero); its first CTA
+//                             writes the list of work for dK / dV;
+//   window_bwd_dkdv_kernel    persistent; an item is 128 keys of one key/value head and a piece of the (query head, 128 query rows)
+//                             that see them. Transposed products S^T = K Q^T and dP^T = V dO^T (TMEM lane = key) leave P^T and dS^T
+//                             in tensor memory as the A operands of dV += P^T dO and dK += dS^T Q;
+//   window_bwd_join_kernel    adds up key blocks whose work was cut into pieces, in the pieces' order;
+//   window_bwd_dq_kernel      persistent; an item is 128 query rows of one head, S double-buffered, dS written over S.
+// The keys of first tokens are seen by every later query, so a block that holds some has many times the work of the others; and
+// with few heads there are fewer blocks than SMs. Both are met by cutting a block's work into pieces. No atomics: the same bits
+// every time.
+// What bounds it: the UMMAs (7 products of 128 x 128 x D a tile pair, against 5 that the mathematics needs) and the waits
+// between them; see the notes at the two loops.
+#include "host.h"
+#include "ptx.cuh"
+#include "window.cuh"
+
+namespace mb {
+
+constexpr int kWbArithWarps = 16;
+constexpr int kWbThreads = 32 * (2 + kWbArithWarps);   // warp 0 TMA producer, warp 1 UMMA issuer, warps 2..17 arithmetic
+constexpr float kWbLog2e = 1.4426950408889634f;
+
+struct WindowBwdArgs {
+  __nv_bfloat16 *dq, *dk, *dv;   // contiguous [B, S, H, D]
+  const float *lse2, *delta;     // [B * Hq, Sq_pad]
+  const int* list;               // [0]: entries; from 4 on: int4 {block, first, one past the last iteration, slot or -1}
+  const int2* pieces;            // [B * key blocks] {first slot, pieces}; pieces 1: no slot
+  float* parts;                  // [slots, Hkv, 2 (dK, dV), 128, D]
+  WindowRule rule;
+  int B, Sq, Sk, Hq, Hkv, Sq_pad;
+  int key_blocks;                // of one row
+  int row_tiles;                 // of 128 query rows
+  float scale, scale_log2;
+  int* status;
+};
+
+struct WindowBwdPrepArgs {
+  const __nv_bfloat16 *out, *out_lo, *dout;
+  long long do_tstride, do_bstride;
+  const float* lse2_in;          // [B, Hq, Sq]
+  float *lse2, *delta;
+  int* list;
+  int2* pieces;
+  WindowRule rule;
+  int B, Sq, Sk, Hq, Hkv, Sq_pad, key_blocks;
+  int piece;                     // iterations of a piece
+  int max_slots;
+};
+
+__device__ __forceinline__ float wb_exp2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// ---------------------------------------------------------------------------------------------- preparation
+constexpr int kWbPrepThreads = 1024;
+
+// The list of work: every key block's iterations, (query heads of the group) x (query tiles that see it), cut into pieces.
+__device__ void window_bwd_list(const WindowBwdPrepArgs& p) {
+  __shared__ int warp_entries[32], warp_slots[32];
+  __shared__ int total_entries, total_slots;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int blocks = p.B * p.key_blocks, group = p.Hq / p.Hkv;
+  int4* entry = reinterpret_cast<int4*>(p.list + 4);
+  if (tid == 0) total_entries = total_slots = 0;
+  __syncthreads();
+  for (int base = 0; base < blocks; base += kWbPrepThreads) {
+    // a block per thread; with documents its range is a warp's work, one block after the other
+    int n_iter = 0;
+    const int mine = base + tid;
+    if (p.rule.starts == nullptr) {
+      if (mine < blocks) {
+        const WindowKeys k = window_keys(p.rule, 0, p.Sq, p.Sk, (mine % p.key_blocks) * kWinBlock);
+        const int n = k.q_hi > k.q_lo ? (k.q_hi + kWinBlock - 1) / kWinBlock - k.q_lo / kWinBlock : 0;
+        n_iter = n * group;
+      }
+    } else {
+      for (int i = 0; i < 32; ++i) {
+        const int b = base + warp * 32 + i;
+        if (b >= blocks) break;
+        const WindowKeys k = window_keys(p.rule, b / p.key_blocks, p.Sq, p.Sk, (b % p.key_blocks) * kWinBlock);
+        const int n = k.q_hi > k.q_lo ? (k.q_hi + kWinBlock - 1) / kWinBlock - k.q_lo / kWinBlock : 0;
+        if (i == lane) n_iter = n * group;
+      }
+    }
+    int n = mine < blocks ? max(1, (n_iter + p.piece - 1) / p.piece) : 0;   // a block that nobody sees still has zeros to write
+    // positions by a scan over the block
+    auto scan = [&](int v, int* warps, int& total, int& before) {
+      int inc = v;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int x = __shfl_up_sync(0xffffffffu, inc, o);
+        if (lane >= o) inc += x;
+      }
+      if (lane == 31) warps[warp] = inc;
+      __syncthreads();
+      int w = lane < warp ? warps[lane] : 0, all = warps[lane];
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) w += __shfl_xor_sync(0xffffffffu, w, o), all += __shfl_xor_sync(0xffffffffu, all, o);
+      before = total + w + inc - v;
+      __syncthreads();
+      if (tid == 0) total += all;
+      __syncthreads();
+    };
+    int slot = 0, at = 0;
+    scan(n > 1 ? n : 0, warp_slots, total_slots, slot);
+    if (n > 1 && slot + n > p.max_slots) n = 1;    // the caller's bound says that this does not happen
+    scan(n, warp_entries, total_entries, at);
+    if (mine < blocks) {
+      p.pieces[mine] = make_int2(slot, n);
+      const int per = n > 1 ? p.piece : n_iter;
+      for (int i = 0; i < n; ++i) entry[at + i] = make_int4(mine, i * per, min(n_iter, (i + 1) * per), n > 1 ? slot + i : -1);
+    }
+  }
+  if (tid == 0) p.list[0] = total_entries;
+}
+
+// CTA 0: the list. Others: delta and lse2, D / 8 lanes a row, rows in memory order.
+template <int D>
+__global__ void __launch_bounds__(kWbPrepThreads) window_bwd_prep_kernel(const WindowBwdPrepArgs p) {
+  if (blockIdx.x == 0) {
+    window_bwd_list(p);
+    return;
+  }
+  constexpr int LANES = D / 8;
+  const long long row = (static_cast<long long>(blockIdx.x - 1) * kWbPrepThreads + threadIdx.x) / LANES;   // (b, q, h), q to Sq_pad
+  const int lane = threadIdx.x % LANES;
+  if (row >= static_cast<long long>(p.B) * p.Sq_pad * p.Hq) return;   // whole warps: the product is a multiple of 128
+  const int h = static_cast<int>(row % p.Hq);
+  const long long bq = row / p.Hq;
+  const int q = static_cast<int>(bq % p.Sq_pad), b = static_cast<int>(bq / p.Sq_pad);
+  float acc = 0.f, l2 = INFINITY;
+  if (q < p.Sq) {
+    const long long o_at = ((static_cast<long long>(b) * p.Sq + q) * p.Hq + h) * D + lane * 8;
+    const uint4 o = *reinterpret_cast<const uint4*>(p.out + o_at), r = *reinterpret_cast<const uint4*>(p.out_lo + o_at);
+    const uint4 d = *reinterpret_cast<const uint4*>(p.dout + b * p.do_bstride + q * p.do_tstride + static_cast<long long>(h) * D + lane * 8);
+    const uint32_t ov[4] = {o.x, o.y, o.z, o.w}, rv[4] = {r.x, r.y, r.z, r.w}, dv[4] = {d.x, d.y, d.z, d.w};
+    uint64_t sum = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) sum = fma_f32x2(add_f32x2(bf16x2_as_f32x2(ov[i]), bf16x2_as_f32x2(rv[i])), bf16x2_as_f32x2(dv[i]), sum);
+    float lo, hi;
+    f32x2_split(sum, lo, hi);
+    acc = lo + hi;
+    if (lane == 0) {
+      l2 = p.lse2_in[(static_cast<long long>(b) * p.Hq + h) * p.Sq + q];
+      if (l2 == -INFINITY) l2 = INFINITY;
+    }
+  }
+#pragma unroll
+  for (int o = LANES / 2; o > 0; o >>= 1) acc += __shfl_xor_sync(0xffffffffu, acc, o);
+  if (lane == 0) {
+    const long long at = (static_cast<long long>(b) * p.Hq + h) * p.Sq_pad + q;
+    p.lse2[at] = l2;
+    p.delta[at] = acc;
+  }
+}
+
+// ---------------------------------------------------------------------------------------------- dK / dV
+// One iteration is 128 keys x 128 queries of one head; S^T and dP^T have one TMEM buffer each. The issuer goes
+//     dV(i) | S(i+1) | dK(i) | dP(i+1)
+// and the arithmetic warps alternate between the exponentials of S(i+1) (under dK(i), dP(i+1)) and dS(i) (under dV(i), S(i+1)).
+// Blocks of 64 queries, which would leave room for two buffers, are bound by shared memory: a UMMA with 64 columns reads its
+// operands at 192 bytes a cycle, of 128 that there are, and everything else that needs shared memory (barriers too) waits.
+template <int D>
+__global__ void __launch_bounds__(kWbThreads, 1)
+window_bwd_dkdv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmDO,
+                       const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV, const WindowBwdArgs p) {
+  constexpr int ATOMS = D / 64;
+  constexpr int TILE_BYTES = kWinBlock * D * 2, ATOM_BYTES = kWinBlock * 128;
+  constexpr int STAGES = 2;
+  constexpr int AUX_BYTES = 2 * kWinBlock * 4;      // lse2, delta of one query tile
+  constexpr uint32_t TMEM_COLS = 512, S_COL = 0, DP_COL = 128, DV_COL = 256, DK_COL = 256 + D;
+
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint8_t* sK = smem;
+  uint8_t* sV = sK + TILE_BYTES;
+  uint8_t* sQ = sV + TILE_BYTES;                    // STAGES tiles
+  uint8_t* sDO = sQ + STAGES * TILE_BYTES;          // STAGES tiles
+  uint8_t* sAux = sDO + STAGES * TILE_BYTES;        // STAGES x AUX_BYTES, with Q
+  uint64_t* bars = reinterpret_cast<uint64_t*>(sAux + STAGES * AUX_BYTES);
+  uint64_t* kv_full = bars;                 // 1
+  uint64_t* kv_empty = bars + 1;            // 1
+  uint64_t* q_full = bars + 2;              // STAGES
+  uint64_t* q_empty = bars + 4;
+  uint64_t* do_full = bars + 6;
+  uint64_t* do_empty = bars + 8;
+  uint64_t* s_full = bars + 10;             // 1
+  uint64_t* p_full = bars + 11;             // 1
+  uint64_t* dp_full = bars + 12;            // 1
+  uint64_t* ds_full = bars + 13;            // 1
+  uint64_t* acc_full = bars + 14;           // 1
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 15);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (threadIdx.x == 0) {
+    mbar_init(kv_full, 1);
+    mbar_init(kv_empty, 1);
+    for (int i = 0; i < STAGES; ++i) {
+      mbar_init(&q_full[i], 1);
+      mbar_init(&q_empty[i], 1);
+      mbar_init(&do_full[i], 1);
+      mbar_init(&do_empty[i], 1);
+    }
+    mbar_init(s_full, 1);
+    mbar_init(p_full, kWbArithWarps);
+    mbar_init(dp_full, 1);
+    mbar_init(ds_full, kWbArithWarps);
+    mbar_init(acc_full, 1);
+    abort_flag[0] = 0;
+    abort_flag[1] = p.status[3];
+    fence_barrier_init();
+    prefetch_tmap(&tmQ);
+    prefetch_tmap(&tmDO);
+    prefetch_tmap(&tmK);
+    prefetch_tmap(&tmV);
+  }
+  if (warp == 1) {
+    tmem_alloc(tmem_slot, TMEM_COLS);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem_base = *tmem_slot;
+
+  const int group = p.Hq / p.Hkv, off = p.Sk - p.Sq;
+  const int items = p.list[0] * p.Hkv;
+  const int4* entry = reinterpret_cast<const int4*>(p.list + 4);
+
+  if (warp == 0) {
+    // ------------------------------------------------------------------ TMA producer
+    uint32_t kv_phase = 0;
+    int n = 0;                                      // query tiles loaded so far
+    bool ok = true;
+    for (int item = blockIdx.x; item < items; item += gridDim.x) {
+      const int4 e = entry[item / p.Hkv];
+      const int kv_head = item % p.Hkv, batch = e.x / p.key_blocks, k0 = (e.x % p.key_blocks) * kWinBlock;
+      const WindowKeys wk = window_keys(p.rule, batch, p.Sq, p.Sk, k0);
+      const int qb = wk.q_lo / kWinBlock, n_q = (wk.q_hi + kWinBlock - 1) / kWinBlock - qb;
+      if (lane == 0 && e.z > e.y) {
+        ok = mbar_wait(kv_empty, (kv_phase & 1) ^ 1, abort_flag);
+        ++kv_phase;
+        if (ok) {
+          mbar_arrive_expect_tx(kv_full, 2 * TILE_BYTES);
+#pragma unroll
+          for (int a = 0; a < ATOMS; ++a) {
+            tma_load_4d(sK + a * ATOM_BYTES, &tmK, kv_full, a * 64, kv_head, k0, batch);
+            tma_load_4d(sV + a * ATOM_BYTES, &tmV, kv_full, a * 64, kv_head, k0, batch);
+          }
+        }
+        for (int it = e.y; ok && it < e.z; ++it, ++n) {
+          const int st = n % STAGES, head = kv_head * group + it / n_q, q0 = (qb + it % n_q) * kWinBlock;
+          const uint32_t parity = ((n / STAGES) & 1) ^ 1;
+          ok = mbar_wait(&q_empty[st], parity, abort_flag);
+          if (!ok) break;
+          mbar_arrive_expect_tx(&q_full[st], TILE_BYTES + AUX_BYTES);
+#pragma unroll
+          for (int a = 0; a < ATOMS; ++a) tma_load_4d(sQ + st * TILE_BYTES + a * ATOM_BYTES, &tmQ, &q_full[st], a * 64, head, q0, batch);
+          const long long row = (static_cast<long long>(batch) * p.Hq + head) * p.Sq_pad + q0;
+          bulk_load(sAux + st * AUX_BYTES, p.lse2 + row, kWinBlock * 4, &q_full[st]);
+          bulk_load(sAux + st * AUX_BYTES + kWinBlock * 4, p.delta + row, kWinBlock * 4, &q_full[st]);
+          ok = mbar_wait(&do_empty[st], parity, abort_flag);
+          if (!ok) break;
+          mbar_arrive_expect_tx(&do_full[st], TILE_BYTES);
+#pragma unroll
+          for (int a = 0; a < ATOMS; ++a) tma_load_4d(sDO + st * TILE_BYTES + a * ATOM_BYTES, &tmDO, &do_full[st], a * 64, head, q0, batch);
+        }
+      }
+      ok = __shfl_sync(0xffffffffu, static_cast<int>(ok), 0) != 0;
+      if (!ok) break;
+    }
+  } else if (warp == 1) {
+    // ------------------------------------------------------------------ UMMA issuer
+    if (lane == 0) {
+      const uint32_t idesc_s = make_idesc_bf16(kWinBlock, kWinBlock, 0, 0);   // [128 keys, 128 queries]
+      const uint32_t idesc_acc = make_idesc_bf16(kWinBlock, D, 0, 1);         // [128 keys, D] = A(TMEM) x B(MN-major)
+      constexpr uint32_t hi = smem_desc_hi_sw128(1024);
+      const uint32_t k_lo = smem_desc_lo(smem_u32(sK), 16), v_lo = smem_desc_lo(smem_u32(sV), 16);
+      auto scores = [&](uint32_t d_tmem, uint32_t a_lo, const uint8_t* b_tile) {
+        const uint32_t b_lo = smem_desc_lo(smem_u32(b_tile), 16);
+#pragma unroll
+        for (int kk = 0; kk < D / 16; ++kk) {
+          const uint32_t o = static_cast<uint32_t>(((kk >> 2) * ATOM_BYTES + (kk & 3) * 32) >> 4);
+          umma_bf16_ss_lh(d_tmem, a_lo + o, hi, b_lo + o, hi, idesc_s, kk != 0 ? 1u : 0u);
+        }
+      };
+      auto accumulate = [&](uint32_t d_tmem, uint32_t a_tmem, const uint8_t* b_tile, bool first) {
+        const uint32_t b_lo = smem_desc_lo(smem_u32(b_tile), ATOM_BYTES);
+        const uint32_t acc0 = first ? 0u : 1u;
+#pragma unroll
+        for (int kk = 0; kk < kWinBlock / 16; ++kk)   // the 32 queries of a warp group sit packed in the first 16 of their 32 columns
+          umma_bf16_ts_lh(d_tmem, a_tmem + static_cast<uint32_t>((kk >> 1) * 32 + (kk & 1) * 8), b_lo + static_cast<uint32_t>(kk * 128), hi,
+                          idesc_acc, kk != 0 ? 1u : acc0);
+      };
+      uint32_t kv_phase = 0;
+      int n = 0;
+      bool ok = true;
+      for (int item = blockIdx.x; ok && item < items; item += gridDim.x) {
+        const int4 e = entry[item / p.Hkv];
+        const int len = e.z - e.y;
+        if (len <= 0) continue;
+        int st = n % STAGES;
+        uint32_t par = (n / STAGES) & 1;
+        ok = mbar_wait(kv_full, kv_phase & 1, abort_flag) && mbar_wait(&q_full[st], par, abort_flag) && mbar_wait(&do_full[st], par, abort_flag);
+        ++kv_phase;
+        if (!ok) break;
+        tc_fence_after();
+        scores(tmem_base + S_COL, k_lo, sQ + st * TILE_BYTES);
+        umma_commit(s_full);
+        scores(tmem_base + DP_COL, v_lo, sDO + st * TILE_BYTES);
+        umma_commit(dp_full);
+        if (len == 1) umma_commit(kv_empty);
+        for (int i = 0; i < len; ++i, ++n) {
+          st = n % STAGES;
+          const int st1 = (n + 1) % STAGES;
+          const uint32_t par1 = ((n + 1) / STAGES) & 1;
+          const bool more = i + 1 < len;
+          ok = (!more || (mbar_wait(&q_full[st1], par1, abort_flag) && mbar_wait(&do_full[st1], par1, abort_flag))) &&
+               mbar_wait(p_full, n & 1, abort_flag);
+          if (!ok) break;
+          tc_fence_after();
+          accumulate(tmem_base + DV_COL, tmem_base + S_COL, sDO + st * TILE_BYTES, i == 0);
+          if (more) {
+            scores(tmem_base + S_COL, k_lo, sQ + st1 * TILE_BYTES);
+            umma_commit(s_full);
+          }
+          umma_commit(&do_empty[st]);
+          ok = mbar_wait(ds_full, n & 1, abort_flag);
+          if (!ok) break;
+          tc_fence_after();
+          accumulate(tmem_base + DK_COL, tmem_base + DP_COL, sQ + st * TILE_BYTES, i == 0);
+          if (more) {
+            scores(tmem_base + DP_COL, v_lo, sDO + st1 * TILE_BYTES);
+            umma_commit(dp_full);
+            if (i + 2 == len) umma_commit(kv_empty);   // K and V are not read again: the next item's may come
+          }
+          umma_commit(&q_empty[st]);
+        }
+        if (ok) umma_commit(acc_full);
+      }
+    }
+    __syncwarp();
+  } else {
+    // ------------------------------------------------------------------ arithmetic: lane = key, 32 query columns per thread
+    const int qw = warp & 3;                        // TMEM lane quarter this warp may touch
+    const int grp = (warp - 2) >> 2;                // which 32 of the 128 queries
+    const int row = qw * 32 + lane;
+    const uint32_t t_lane = static_cast<uint32_t>(qw * 32) << 16;
+    const uint32_t t_s = tmem_base + S_COL + static_cast<uint32_t>(grp * 32) + t_lane;
+    const uint32_t t_dp = tmem_base + DP_COL + static_cast<uint32_t>(grp * 32) + t_lane;
+    const uint64_t scale2 = f32x2(p.scale_log2, p.scale_log2), minus = f32x2(-1.f, -1.f);
+    uint32_t acc_phase = 0;
+    int n = 0;
+    bool ok = true;
+    for (int item = blockIdx.x; item < items; item += gridDim.x) {
+      const int4 e = entry[item / p.Hkv];
+      const int kv_head = item % p.Hkv, batch = e.x / p.key_blocks, k0 = (e.x % p.key_blocks) * kWinBlock;
+      const WindowKeys wk = window_keys(p.rule, batch, p.Sq, p.Sk, k0);
+      const int qb = wk.q_lo / kWinBlock, n_q = (wk.q_hi + kWinBlock - 1) / kWinBlock - qb;
+      const int kj = k0 + row;
+      int upper = 0;                                // queries at positions [kj, upper) see this key
+      if (kj < p.Sk) {
+        const long long at = static_cast<long long>(batch) * p.Sk + kj;
+        const int start = p.rule.starts ? p.rule.starts[at] : 0;
+        if (start != kWinNone) upper = window_upper(p.rule, start, p.rule.starts ? p.rule.ends[at] : p.Sk, kj);
+      }
+      for (int it = e.y; it < e.z; ++it, ++n) {
+        const int st = n % STAGES;
+        const float* aux = reinterpret_cast<const float*>(sAux + st * AUX_BYTES) + grp * 32;
+        const int pos0 = (qb + it % n_q) * kWinBlock + off;     // position of the tile's first query
+        ok = mbar_wait(&q_full[st], (n / STAGES) & 1, abort_flag);   // the statistics; the scores come later
+        uint64_t pr[16];                            // -lse2, then P, of 16 pairs
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const float4 v = reinterpret_cast<const float4*>(aux)[i];
+          pr[2 * i] = f32x2(-v.x, -v.y), pr[2 * i + 1] = f32x2(-v.z, -v.w);
+        }
+        ok = ok && mbar_wait(s_full, n & 1, abort_flag);
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) break;
+        tc_fence_after();
+        uint32_t t[32];
+        tmem_ld_32x32b_x32(t_s, t);
+        tmem_ld_wait();
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          float a, b;
+          f32x2_split(fma_f32x2(f32x2(__uint_as_float(t[2 * i]), __uint_as_float(t[2 * i + 1])), scale2, pr[i]), a, b);
+          pr[i] = f32x2(wb_exp2(a), wb_exp2(b));
+        }
+        if (pos0 < k0 + kWinBlock - 1 || pos0 + kWinBlock > wk.full_hi) {
+          const uint32_t seen = interval_bits(pos0 + grp * 32, kj, upper);
+          if (!__all_sync(0xffffffffu, seen == 0xffffffffu)) {
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+              float a, b;
+              f32x2_split(pr[i], a, b);
+              pr[i] = f32x2((seen >> (2 * i)) & 1u ? a : 0.f, (seen >> (2 * i + 1)) & 1u ? b : 0.f);
+            }
+          }
+        }
+        {
+          uint32_t pk[16];
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            float a, b;
+            f32x2_split(pr[i], a, b);
+            pk[i] = pack_bf16x2(a, b);
+          }
+          tmem_st_32x32b_x16(t_s, pk);
+        }
+        tmem_st_wait();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(p_full);
+        // ---------------------------------------------------------------- dS
+        ok = mbar_wait(dp_full, n & 1, abort_flag);
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) break;
+        tc_fence_after();
+        tmem_ld_32x32b_x32(t_dp, t);
+        tmem_ld_wait();
+        {
+          uint32_t ds[16];
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            const float4 v = reinterpret_cast<const float4*>(aux + kWinBlock)[i];
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+              const int j = 2 * i + k;
+              const uint64_t dl = k ? f32x2(v.z, v.w) : f32x2(v.x, v.y);
+              const uint64_t d = fma_f32x2(dl, minus, f32x2(__uint_as_float(t[2 * j]), __uint_as_float(t[2 * j + 1])));
+              float a, b;
+              f32x2_split(mul_f32x2(pr[j], d), a, b);
+              ds[j] = pack_bf16x2(a, b);
+            }
+          }
+          tmem_st_32x32b_x16(t_dp, ds);
+        }
+        tmem_st_wait();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(ds_full);
+      }
+      if (!ok) break;
+      // ---------------------------------------------------------------- this piece's dK, dV rows
+      const bool any = e.z > e.y;
+      if (any) {
+        ok = mbar_wait(acc_full, acc_phase & 1, abort_flag);
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) break;
+        ++acc_phase;
+        tc_fence_after();
+      }
+      constexpr int QUART_D = D / 4;                // columns of the head dimension per thread
+      const long long to = ((static_cast<long long>(batch) * p.Sk + kj) * p.Hkv + kv_head) * D + grp * QUART_D;
+      float* part = e.w < 0 ? nullptr : p.parts + ((static_cast<long long>(e.w) * p.Hkv + kv_head) * 2 * kWinBlock + row) * D + grp * QUART_D;
+#pragma unroll
+      for (int which = 0; which < 2; ++which) {
+        const uint32_t col = (which ? DV_COL : DK_COL) + static_cast<uint32_t>(grp * QUART_D);
+        const float mul = which ? 1.f : p.scale;
+        __nv_bfloat16* dst = which ? p.dv : p.dk;
+#pragma unroll
+        for (int c = 0; c < QUART_D; c += 16) {
+          uint32_t r[16];
+#pragma unroll
+          for (int i = 0; i < 16; ++i) r[i] = 0u;
+          if (any) {
+            tmem_ld_32x32b_x16(tmem_base + col + static_cast<uint32_t>(c) + t_lane, r);
+            tmem_ld_wait();
+          }
+          if (part) {                               // rows past the end hold zeros there
+#pragma unroll
+            for (int i = 0; i < 16; i += 4)
+              *reinterpret_cast<float4*>(part + which * kWinBlock * D + c + i) =
+                  make_float4(__uint_as_float(r[i]) * mul, __uint_as_float(r[i + 1]) * mul, __uint_as_float(r[i + 2]) * mul, __uint_as_float(r[i + 3]) * mul);
+          } else if (kj < p.Sk) {
+#pragma unroll
+            for (int i = 0; i < 16; i += 8) {
+              uint32_t v[4];
+#pragma unroll
+              for (int k = 0; k < 4; ++k) v[k] = pack_bf16x2(__uint_as_float(r[i + 2 * k]) * mul, __uint_as_float(r[i + 2 * k + 1]) * mul);
+              *reinterpret_cast<uint4*>(dst + to + c + i) = make_uint4(v[0], v[1], v[2], v[3]);
+            }
+          }
+        }
+      }
+      tc_fence_before();                            // before the next item's first products (via p_full)
+    }
+  }
+
+  tc_fence_before();
+  __syncthreads();
+  if (*abort_flag) {
+    __nanosleep(50000);
+    if (threadIdx.x == 0) {
+      atomicOr(&p.status[0], MB_ERR_MBAR_TIMEOUT);
+      p.status[1] = static_cast<int>(blockIdx.x);
+      p.status[2] = 1011;
+    }
+  }
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc(tmem_base, TMEM_COLS);
+  }
+}
+
+// dK, dV of key blocks that were cut: one CTA per (block, key/value head), the pieces added in order.
+template <int D>
+__global__ void __launch_bounds__(256) window_bwd_join_kernel(const WindowBwdArgs p) {
+  const int blk = blockIdx.x / p.Hkv, kv_head = blockIdx.x % p.Hkv;
+  const int2 pc = p.pieces[blk];
+  if (pc.y <= 1) return;
+  const int batch = blk / p.key_blocks, k0 = (blk % p.key_blocks) * kWinBlock;
+  for (int i = threadIdx.x + blockIdx.y * 256; i < 2 * kWinBlock * D / 4; i += 256 * gridDim.y) {
+    const int which = i / (kWinBlock * D / 4), row = i % (kWinBlock * D / 4) / (D / 4), c = i % (D / 4) * 4;
+    if (k0 + row >= p.Sk) continue;
+    float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+    for (int s = 0; s < pc.y; ++s) {
+      const float4 x = *reinterpret_cast<const float4*>(p.parts + ((static_cast<long long>(pc.x + s) * p.Hkv + kv_head) * 2 + which) * kWinBlock * D +
+                                                        row * D + c);
+      a.x += x.x, a.y += x.y, a.z += x.z, a.w += x.w;
+    }
+    uint2 v;
+    v.x = pack_bf16x2(a.x, a.y), v.y = pack_bf16x2(a.z, a.w);
+    *reinterpret_cast<uint2*>((which ? p.dv : p.dk) + ((static_cast<long long>(batch) * p.Sk + k0 + row) * p.Hkv + kv_head) * D + c) = v;
+  }
+}
+
+// ---------------------------------------------------------------------------------------------- dQ
+// The items' key blocks form one stream; element g has its scores in TMEM buffer g & 1. The issuer goes
+//     dQ(g-1) | S(g+1) | dP(g+1)
+// while the arithmetic warps work on element g. dQ(g-1) frees the buffer of S(g+1); dP has one buffer, free as soon as the
+// arithmetic has it in registers. What was loaded long ago is waited for before the wait on dS, so that nothing but a (by then
+// satisfied) wait stands between the three products.
+template <int D>
+__global__ void __launch_bounds__(kWbThreads, 1)
+window_bwd_dq_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmDO,
+                     const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV, const WindowBwdArgs p) {
+  constexpr int ATOMS = D / 64;
+  constexpr int TILE_BYTES = kWinBlock * D * 2, ATOM_BYTES = kWinBlock * 128;
+  constexpr uint32_t TMEM_COLS = 512, DP_COL = 256, DQ_COL = 384;
+  constexpr int K_STAGES = 3, V_STAGES = 2;
+  extern __shared__ __align__(1024) uint8_t smem_raw[];   // with head_dim 128 the tiles fill it: its start has to be aligned
+  uint8_t* smem = smem_raw;
+  uint8_t* sQ = smem;
+  uint8_t* sDO = sQ + TILE_BYTES;
+  uint8_t* sK = sDO + TILE_BYTES;                   // K_STAGES
+  uint8_t* sV = sK + K_STAGES * TILE_BYTES;         // V_STAGES
+  uint64_t* bars = reinterpret_cast<uint64_t*>(sV + V_STAGES * TILE_BYTES);
+  uint64_t* q_full = bars;            // 1
+  uint64_t* q_empty = bars + 1;       // 1
+  uint64_t* k_full = bars + 2;        // K_STAGES
+  uint64_t* k_empty = bars + 5;       // K_STAGES
+  uint64_t* v_full = bars + 8;        // V_STAGES
+  uint64_t* v_empty = bars + 10;      // V_STAGES
+  uint64_t* s_full = bars + 12;       // 2
+  uint64_t* dp_full = bars + 14;      // 1
+  uint64_t* dp_free = bars + 15;      // 1
+  uint64_t* ds_full = bars + 16;      // 2: the arithmetic may finish element g + 1 before the issuer asks for element g
+  uint64_t* dq_full = bars + 18;      // 1
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 19);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (smem_u32(smem_raw) & 1023u) {   // uniform over the CTA: nothing has been set up yet
+    if (threadIdx.x == 0) {
+      atomicOr(&p.status[0], MB_ERR_BAD_INDEX);
+      p.status[2] = 1013;
+    }
+    return;
+  }
+  if (threadIdx.x == 0) {
+    mbar_init(q_full, 1);
+    mbar_init(q_empty, 1);
+    for (int i = 0; i < K_STAGES; ++i) {
+      mbar_init(&k_full[i], 1);
+      mbar_init(&k_empty[i], 1);
+    }
+    for (int i = 0; i < V_STAGES; ++i) {
+      mbar_init(&v_full[i], 1);
+      mbar_init(&v_empty[i], 1);
+    }
+    mbar_init(&s_full[0], 1);
+    mbar_init(&s_full[1], 1);
+    mbar_init(dp_full, 1);
+    mbar_init(dp_free, kWbArithWarps);
+    mbar_init(&ds_full[0], kWbArithWarps);
+    mbar_init(&ds_full[1], kWbArithWarps);
+    mbar_init(dq_full, 1);
+    abort_flag[0] = 0;
+    abort_flag[1] = p.status[3];
+    fence_barrier_init();
+    prefetch_tmap(&tmQ);
+    prefetch_tmap(&tmDO);
+    prefetch_tmap(&tmK);
+    prefetch_tmap(&tmV);
+  }
+  if (warp == 1) {
+    tmem_alloc(tmem_slot, TMEM_COLS);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem_base = *tmem_slot;
+
+  const int items = p.row_tiles * p.Hq * p.B, group = p.Hq / p.Hkv;
+  // late rows (long lists) first, the heads of one row tile next to one another
+  auto where = [&](int item, int& batch, int& head, int& q0) {
+    head = item % p.Hq;
+    const int rest = item / p.Hq;
+    q0 = (p.row_tiles - 1 - rest % p.row_tiles) * kWinBlock;
+    batch = rest / p.row_tiles;
+  };
+
+  if (warp == 0) {
+    // ------------------------------------------------------------------ TMA producer
+    uint32_t q_uses = 0;
+    int g = 0;
+    bool ok = true;
+    for (int item = blockIdx.x; item < items; item += gridDim.x) {
+      int batch, head, q0;
+      where(item, batch, head, q0);
+      const WindowTile t = window_tile(p.rule, batch, p.Sq, p.Sk, q0);
+      const int n = t.count(), kv_head = head / group;
+      if (lane == 0 && n > 0) {
+        if (item + static_cast<int>(gridDim.x) < items) {   // the next item's rows on their way to L2
+          int nb, nh, nq;
+          where(item + gridDim.x, nb, nh, nq);
+#pragma unroll
+          for (int a = 0; a < ATOMS; ++a) {
+            tma_prefetch_4d(&tmQ, a * 64, nh, nq, nb);
+            tma_prefetch_4d(&tmDO, a * 64, nh, nq, nb);
+          }
+        }
+        for (int j = 0; ok && j < n; ++j, ++g) {
+          const int ks = g % K_STAGES, vs = g % V_STAGES, key0 = t.block(j) * kWinBlock;
+          ok = mbar_wait(&k_empty[ks], ((g / K_STAGES) & 1) ^ 1, abort_flag);
+          if (!ok) break;
+          mbar_arrive_expect_tx(&k_full[ks], TILE_BYTES);
+#pragma unroll
+          for (int a = 0; a < ATOMS; ++a)
+            tma_load_4d(sK + ks * TILE_BYTES + a * ATOM_BYTES, &tmK, &k_full[ks], a * 64, kv_head, key0, batch);
+          ok = mbar_wait(&v_empty[vs], ((g / V_STAGES) & 1) ^ 1, abort_flag);
+          if (!ok) break;
+          mbar_arrive_expect_tx(&v_full[vs], TILE_BYTES);
+#pragma unroll
+          for (int a = 0; a < ATOMS; ++a)
+            tma_load_4d(sV + vs * TILE_BYTES + a * ATOM_BYTES, &tmV, &v_full[vs], a * 64, kv_head, key0, batch);
+          if (j == 0) {
+            ok = mbar_wait(q_empty, (q_uses & 1) ^ 1, abort_flag);
+            if (!ok) break;
+            ++q_uses;
+            mbar_arrive_expect_tx(q_full, 2 * TILE_BYTES);
+#pragma unroll
+            for (int a = 0; a < ATOMS; ++a) {
+              tma_load_4d(sQ + a * ATOM_BYTES, &tmQ, q_full, a * 64, head, q0, batch);
+              tma_load_4d(sDO + a * ATOM_BYTES, &tmDO, q_full, a * 64, head, q0, batch);
+            }
+          }
+        }
+      }
+      ok = __shfl_sync(0xffffffffu, static_cast<int>(ok), 0) != 0;
+      if (!ok) break;
+    }
+  } else if (warp == 1) {
+    // ------------------------------------------------------------------ UMMA issuer
+    const uint32_t idesc_s = make_idesc_bf16(kWinBlock, kWinBlock, 0, 0);   // [128 q, 128 keys]
+    const uint32_t idesc_dq = make_idesc_bf16(kWinBlock, D, 0, 1);          // [128 q, D] = A(TMEM) x B(K tile, MN-major)
+    constexpr uint32_t hi = smem_desc_hi_sw128(1024);
+    const uint32_t q_lo = smem_desc_lo(smem_u32(sQ), 16), do_lo = smem_desc_lo(smem_u32(sDO), 16);
+    auto scores = [&](uint32_t d_tmem, uint32_t a_lo, const uint8_t* b_tile) {
+      const uint32_t b_lo = smem_desc_lo(smem_u32(b_tile), 16);
+#pragma unroll
+      for (int kk = 0; kk < D / 16; ++kk) {
+        const uint32_t o = static_cast<uint32_t>(((kk >> 2) * ATOM_BYTES + (kk & 3) * 32) >> 4);
+        umma_bf16_ss_lh(d_tmem, a_lo + o, hi, b_lo + o, hi, idesc_s, kk != 0 ? 1u : 0u);
+      }
+    };
+    int g = 0;                                      // element whose scores are issued next
+    uint32_t q_phase = 0;
+    bool ok = true;
+    // place in their items of the two elements whose dQ is still to come: bit 0 first, bit 1 last
+    int place1 = 0, place2 = 0;                     // of elements g - 1 and g - 2
+    auto finish = [&](int e, int place) {           // dQ of element e
+      ok = mbar_wait(&ds_full[e & 1], (e >> 1) & 1, abort_flag);
+      if (!ok) return;
+      tc_fence_after();
+      const uint32_t k_lo = smem_desc_lo(smem_u32(sK + (e % K_STAGES) * TILE_BYTES), ATOM_BYTES);
+      const uint32_t s_col = tmem_base + static_cast<uint32_t>(e & 1) * 128u, acc0 = (place & 1) ? 0u : 1u;
+#pragma unroll
+      for (int kk = 0; kk < kWinBlock / 16; ++kk)   // the 32 keys of a warp group sit packed in the first 16 of their 32 columns
+        umma_bf16_ts_lh(tmem_base + DQ_COL, s_col + static_cast<uint32_t>((kk >> 1) * 32 + (kk & 1) * 8), k_lo + static_cast<uint32_t>(kk * 128), hi,
+                        idesc_dq, kk != 0 ? 1u : acc0);
+      umma_commit(&k_empty[e % K_STAGES]);
+      if (place & 2) umma_commit(dq_full);
+    };
+    for (int item = blockIdx.x; item < items; item += gridDim.x) {
+      int batch, head, q0;
+      where(item, batch, head, q0);
+      const int n = window_tile(p.rule, batch, p.Sq, p.Sk, q0).count();
+      if (lane == 0) {
+        for (int j = 0; j < n; ++j, ++g) {
+          const int ks = g % K_STAGES, vs = g % V_STAGES;
+          ok = mbar_wait(&k_full[ks], (g / K_STAGES) & 1, abort_flag) && mbar_wait(&v_full[vs], (g / V_STAGES) & 1, abort_flag);
+          if (!ok) break;
+          if (g >= 2) finish(g - 2, place2);
+          if (ok && j == 0) {
+            ok = mbar_wait(q_full, q_phase & 1, abort_flag);
+            ++q_phase;
+          }
+          if (!ok) break;
+          tc_fence_after();
+          scores(tmem_base + static_cast<uint32_t>(g & 1) * 128u, q_lo, sK + ks * TILE_BYTES);
+          umma_commit(&s_full[g & 1]);
+          if (g >= 1) {
+            ok = mbar_wait(dp_free, (g - 1) & 1, abort_flag);
+            if (!ok) break;
+            tc_fence_after();
+          }
+          scores(tmem_base + DP_COL, do_lo, sV + vs * TILE_BYTES);
+          umma_commit(dp_full);
+          umma_commit(&v_empty[vs]);
+          if (j + 1 == n) umma_commit(q_empty);
+          place2 = place1;
+          place1 = (j == 0 ? 1 : 0) | (j + 1 == n ? 2 : 0);
+        }
+      }
+      ok = __shfl_sync(0xffffffffu, static_cast<int>(ok), 0) != 0;
+      if (!ok) break;
+    }
+    if (lane == 0 && ok) {
+      if (g >= 2) finish(g - 2, place2);
+      if (ok && g >= 1) finish(g - 1, place1);
+    }
+    __syncwarp();
+  } else {
+    // ------------------------------------------------------------------ arithmetic: lane = query row, 32 key columns per thread
+    const int qw = warp & 3;
+    const int grp = (warp - 2) >> 2;                // which 32 of the 128 keys
+    const int row = qw * 32 + lane;
+    const uint32_t t_lane = static_cast<uint32_t>(qw * 32) << 16;
+    const uint32_t t_dp = tmem_base + DP_COL + static_cast<uint32_t>(grp * 32) + t_lane;
+    const uint64_t scale2 = f32x2(p.scale_log2, p.scale_log2);
+    uint32_t dq_phase = 0;
+    int g = 0;
+    bool ok = true;
+    for (int item = blockIdx.x; item < items; item += gridDim.x) {
+      int batch, head, q0;
+      where(item, batch, head, q0);
+      const WindowTile t = window_tile(p.rule, batch, p.Sq, p.Sk, q0);
+      const int n = t.count(), qi = q0 + row;
+      const long long stat = (static_cast<long long>(batch) * p.Hq + head) * p.Sq_pad + qi;   // padded: always in range
+      const float my_lse = p.lse2[stat], my_delta = p.delta[stat];
+      const WindowRow w = window_row(p.rule, batch, p.Sk, qi + p.Sk - p.Sq, qi < p.Sq);
+      // The forward's own rounded weights, so that the terms of dS cancel as exactly as there: weights relative to a whole power
+      // of two (the forward's differ from it by another such factor), rounded to bf16, times what is left of 2^-lse2.
+      const float shift = floorf(my_lse);
+      const float factor = my_lse != INFINITY ? wb_exp2(shift - my_lse) : 0.f;
+      const uint64_t shift2 = f32x2(-shift, -shift), factor2 = f32x2(factor, factor), offset2 = f32x2(-my_delta * factor, -my_delta * factor);
+      for (int j = 0; j < n; ++j, ++g) {
+        ok = mbar_wait(&s_full[g & 1], (g >> 1) & 1, abort_flag);
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) break;
+        tc_fence_after();
+        const uint32_t t_s = tmem_base + static_cast<uint32_t>((g & 1) * 128 + grp * 32) + t_lane;
+        uint32_t sc[32];
+        tmem_ld_32x32b_x32(t_s, sc);
+        tmem_ld_wait();
+        const int key0 = t.block(j) * kWinBlock;
+        uint32_t wt[16];                            // rounded weights, two a register
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          float a, b;
+          f32x2_split(fma_f32x2(f32x2(__uint_as_float(sc[2 * i]), __uint_as_float(sc[2 * i + 1])), scale2, shift2), a, b);
+          wt[i] = pack_bf16x2(wb_exp2(a), wb_exp2(b));
+        }
+        if (key0 < t.full_lo || key0 + kWinBlock - 1 > t.full_hi) {
+          const uint32_t seen = window_bits(w, key0 + grp * 32);
+          if (!__all_sync(0xffffffffu, seen == 0xffffffffu)) {
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+              if (!((seen >> (2 * i)) & 1u)) wt[i] &= 0xffff0000u;
+              if (!((seen >> (2 * i + 1)) & 1u)) wt[i] &= 0x0000ffffu;
+            }
+          }
+        }
+        ok = mbar_wait(dp_full, g & 1, abort_flag);
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) break;
+        tc_fence_after();
+        uint32_t dp[32];
+        tmem_ld_32x32b_x32(t_dp, dp);
+        tmem_ld_wait();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(dp_free);        // the next element's dP may be issued
+        uint32_t ds[16];
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          float a, b;
+          const uint64_t d = fma_f32x2(f32x2(__uint_as_float(dp[2 * i]), __uint_as_float(dp[2 * i + 1])), factor2, offset2);
+          f32x2_split(mul_f32x2(bf16x2_as_f32x2(wt[i]), d), a, b);
+          ds[i] = pack_bf16x2(a, b);
+        }
+        tmem_st_32x32b_x16(t_s, ds);
+        tmem_st_wait();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&ds_full[g & 1]);
+      }
+      if (!ok) break;
+      if (n > 0) {
+        ok = mbar_wait(dq_full, dq_phase & 1, abort_flag);
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) break;
+        ++dq_phase;
+        tc_fence_after();
+      }
+      constexpr int QUART_D = D / 4;
+      __nv_bfloat16* dst = p.dq + ((static_cast<long long>(batch) * p.Sq + qi) * p.Hq + head) * D + grp * QUART_D;
+#pragma unroll
+      for (int c = 0; c < QUART_D; c += 16) {
+        uint32_t r[16];
+#pragma unroll
+        for (int i = 0; i < 16; ++i) r[i] = 0u;
+        if (n > 0) {
+          tmem_ld_32x32b_x16(tmem_base + DQ_COL + static_cast<uint32_t>(grp * QUART_D + c) + t_lane, r);
+          tmem_ld_wait();
+        }
+        if (qi < p.Sq) {
+#pragma unroll
+          for (int i = 0; i < 16; i += 8) {
+            uint32_t v[4];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) v[k] = pack_bf16x2(__uint_as_float(r[i + 2 * k]) * p.scale, __uint_as_float(r[i + 2 * k + 1]) * p.scale);
+            *reinterpret_cast<uint4*>(dst + c + i) = make_uint4(v[0], v[1], v[2], v[3]);
+          }
+        }
+      }
+      tc_fence_before();                            // before the next item's first dQ (via ds_full)
+    }
+  }
+
+  tc_fence_before();
+  __syncthreads();
+  if (*abort_flag) {
+    __nanosleep(50000);
+    if (threadIdx.x == 0) {
+      atomicOr(&p.status[0], MB_ERR_MBAR_TIMEOUT);
+      p.status[1] = static_cast<int>(blockIdx.x);
+      p.status[2] = 1012;
+    }
+  }
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc(tmem_base, TMEM_COLS);
+  }
+}
+
+// ---------------------------------------------------------------------------------------------- host
+// How a key block's work is cut, and what that needs of scratch memory.
+struct WindowBwdPlan {
+  int sq_pad, key_blocks, row_tiles, piece;
+  long long blocks, max_slots, rows;
+  long long at_delta, at_list, at_pieces, at_parts, words;   // in 4-byte words
+};
+
+static WindowBwdPlan window_bwd_plan(int B, int Sq, int Sk, int Hq, int Hkv, int D, int window, int sinks, bool packed) {
+  WindowBwdPlan w{};
+  const long long group = Hq / Hkv;
+  w.row_tiles = (Sq + kWinBlock - 1) / kWinBlock;
+  w.key_blocks = (Sk + kWinBlock - 1) / kWinBlock;
+  w.sq_pad = w.row_tiles * kWinBlock;
+  w.blocks = static_cast<long long>(B) * w.key_blocks;
+  // iterations of a block whose keys are seen through the window only, and of one that every query of its row sees
+  const long long tiles = (static_cast<long long>(window < Sk ? window : Sk) + kWinBlock - 1) / kWinBlock + 2;
+  const long long near = (tiles < w.row_tiles ? tiles : w.row_tiles) * group, all = w.row_tiles * group;
+  const long long items = w.blocks * Hkv;
+  // Pieces a quarter longer than an ordinary block's work: only blocks with first tokens are cut. With fewer blocks than SMs
+  // ordinary blocks are cut too, into as many pieces as there are SMs for.
+  long long piece = sinks > 0 ? near + near / 4 + 1 : near;
+  if (items < sm_count()) {
+    const long long share = sm_count() / items;
+    piece = (near + share - 1) / share;
+    if (piece < 2) piece = 2;
+  }
+  const long long ordinary = (near + piece - 1) / piece;
+  long long slots = ordinary > 1 ? w.blocks * ordinary : 0;
+  if (sinks > 0 && all > piece) {
+    const long long sink_blocks = (sinks + kWinBlock - 1) / kWinBlock;
+    if (!packed) {
+      const long long n = sink_blocks < w.key_blocks ? sink_blocks : w.key_blocks;
+      slots += B * n * ((all + piece - 1) / piece);
+    } else {
+      // a row tile sees far first tokens of one document, which lie in at most sink_blocks + 1 blocks
+      const long long far = B * all * (sink_blocks + 1);
+      const long long cut = piece > near ? far / (piece - near) : w.blocks;   // blocks that far queries make too long
+      slots += far / piece + 2 * (cut < w.blocks ? cut : w.blocks);
+    }
+  }
+  w.piece = static_cast<int>(piece < (1 << 30) ? piece : (1 << 30));
+  w.max_slots = slots;
+  w.rows = static_cast<long long>(B) * Hq * w.sq_pad;
+  w.at_delta = w.rows;
+  w.at_list = 2 * w.rows;
+  w.at_pieces = w.at_list + 4 + 4 * (w.blocks + slots);
+  w.at_parts = (w.at_pieces + 2 * w.blocks + 3) / 4 * 4;
+  w.words = w.at_parts + slots * Hkv * 2 * kWinBlock * D;
+  return w;
+}
+
+struct WindowBwdMaps {
+  CUtensorMap q, dout, k, v;
+};
+
+template <int D>
+static int launch_window_bwd(const WindowBwdMaps& m, const WindowBwdPrepArgs& prep, const WindowBwdArgs& a, const WindowBwdPlan& plan,
+                             cudaStream_t stream) {
+  constexpr size_t tile = kWinBlock * D * 2;
+  constexpr size_t smem_dkdv = 1024 + 6 * tile + 2 * (2 * kWinBlock * 4) + 256, smem_dq = 7 * tile + 256;
+  static bool configured[64] = {false};
+  int dev = 0;
+  MB_CHECK_CUDA(cudaGetDevice(&dev));
+  if (!configured[dev & 63]) {
+    MB_CHECK_CUDA(cudaFuncSetAttribute(window_bwd_dkdv_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem_dkdv)));
+    MB_CHECK_CUDA(cudaFuncSetAttribute(window_bwd_dq_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem_dq)));
+    configured[dev & 63] = true;
+  }
+  const long long prep_blocks = 1 + (plan.rows * (D / 8) + kWbPrepThreads - 1) / kWbPrepThreads;
+  window_bwd_prep_kernel<D><<<static_cast<unsigned>(prep_blocks), kWbPrepThreads, 0, stream>>>(prep);
+  const long long most = (plan.blocks + plan.max_slots) * a.Hkv;
+  const int grid_kv = static_cast<int>(most < sm_count() ? most : sm_count());
+  window_bwd_dkdv_kernel<D><<<grid_kv, kWbThreads, smem_dkdv, stream>>>(m.q, m.dout, m.k, m.v, a);
+  count_launch(2);
+  if (plan.max_slots > 0) {
+    window_bwd_join_kernel<D><<<dim3(static_cast<unsigned>(plan.blocks * a.Hkv), 4), 256, 0, stream>>>(a);
+    count_launch();
+  }
+  const long long tiles = static_cast<long long>(plan.row_tiles) * a.Hq * a.B;
+  window_bwd_dq_kernel<D><<<static_cast<int>(tiles < sm_count() ? tiles : sm_count()), kWbThreads, smem_dq, stream>>>(m.q, m.dout, m.k, m.v, a);
+  count_launch();
+  MB_CHECK_CUDA(cudaGetLastError());
+  return 0;
+}
+
+}  // namespace mb
+
+// 4-byte words of scratch memory mb_window_attn_bwd needs; `packed`: it is given documents.
+MB_API long long mb_window_attn_bwd_scratch_words(int B, int Sq, int Sk, int Hq, int Hkv, int D, int window, int sinks, int packed) {
+  if (B < 1 || Sq < 1 || Sk < 1 || Hkv < 1 || Hq % Hkv != 0) return 0;
+  return mb::window_bwd_plan(B, Sq, Sk, Hq, Hkv, D, window, sinks, packed != 0).words;
+}
+
+// Backward of mb_window_attn_fwd. q, k, v, out, out_lo, lse2 as there, dout with strides of its own, dq / dk / dv bf16 contiguous.
+// starts, ends: mb_document_bounds of the key rows, or both null. scratch: mb_window_attn_bwd_scratch_words() words.
+MB_API int mb_window_attn_bwd(const void* q, long long q_tstride, long long q_bstride, const void* k, long long k_tstride,
+                              long long k_bstride, const void* v, long long v_tstride, long long v_bstride, const void* out,
+                              const void* out_lo, const void* dout, long long do_tstride, long long do_bstride, const float* lse2, void* dq,
+                              void* dk, void* dv, const int* starts, const int* ends, int* scratch, int B, int Sq, int Sk, int Hq, int Hkv,
+                              int D, int window, int sinks, float scale, cudaStream_t stream) {
+  using namespace mb;
+  const long long strides[] = {q_tstride, q_bstride, k_tstride, k_bstride, v_tstride, v_bstride, do_tstride, do_bstride};
+  const void* pointers[] = {q, k, v, out, out_lo, dout, dq, dk, dv, scratch};
+  if (const char* what = window_attn_problem(B, Sq, Sk, Hq, Hkv, D, window, sinks, strides, 8, pointers, 10)) {
+    set_last_error(what);
+    return -1;
+  }
+  if ((starts == nullptr) != (ends == nullptr)) {
+    set_last_error("mb_window_attn_bwd: starts and ends come together");
+    return -2;
+  }
+  int* status = status_ptr();
+  if (!status) return -4;
+  const WindowBwdPlan plan = window_bwd_plan(B, Sq, Sk, Hq, Hkv, D, window, sinks, starts != nullptr);
+  if (plan.blocks * Hkv >= (1ll << 31) - 65536 || static_cast<long long>(plan.row_tiles) * Hq * B >= (1ll << 31) - 65536 ||
+      plan.rows * (D / 8) / kWbPrepThreads >= (1ll << 31) - 65536 || (plan.blocks + plan.max_slots) * Hkv >= (1ll << 31) - 65536) {
+    set_last_error("mb_window_attn_bwd: too many tiles");
+    return -1;
+  }
+  const WindowRule rule = {starts, ends, window < Sk ? window : Sk, sinks < Sk ? sinks : Sk};
+  float* lse2_pad = reinterpret_cast<float*>(scratch);
+  float* delta = lse2_pad + plan.at_delta;
+  int* list = scratch + plan.at_list;
+  int2* pieces = reinterpret_cast<int2*>(scratch + plan.at_pieces);
+  WindowBwdPrepArgs prep;
+  prep.out = static_cast<const __nv_bfloat16*>(out), prep.out_lo = static_cast<const __nv_bfloat16*>(out_lo);
+  prep.dout = static_cast<const __nv_bfloat16*>(dout);
+  prep.do_tstride = do_tstride, prep.do_bstride = do_bstride;
+  prep.lse2_in = lse2, prep.lse2 = lse2_pad, prep.delta = delta, prep.list = list, prep.pieces = pieces, prep.rule = rule;
+  prep.B = B, prep.Sq = Sq, prep.Sk = Sk, prep.Hq = Hq, prep.Hkv = Hkv, prep.Sq_pad = plan.sq_pad, prep.key_blocks = plan.key_blocks;
+  prep.piece = plan.piece, prep.max_slots = static_cast<int>(plan.max_slots);
+  WindowBwdArgs a;
+  a.dq = static_cast<__nv_bfloat16*>(dq), a.dk = static_cast<__nv_bfloat16*>(dk), a.dv = static_cast<__nv_bfloat16*>(dv);
+  a.lse2 = lse2_pad, a.delta = delta, a.list = list, a.pieces = pieces, a.parts = reinterpret_cast<float*>(scratch + plan.at_parts);
+  a.rule = rule;
+  a.B = B, a.Sq = Sq, a.Sk = Sk, a.Hq = Hq, a.Hkv = Hkv, a.Sq_pad = plan.sq_pad;
+  a.key_blocks = plan.key_blocks, a.row_tiles = plan.row_tiles;
+  a.scale = scale, a.scale_log2 = scale * kWbLog2e;
+  a.status = status;
+  WindowBwdMaps m;
+  const uint32_t box[4] = {64, 1, static_cast<uint32_t>(kWinBlock), 1};
+  auto encode = [&](CUtensorMap* t, const void* x, int heads, int S, long long tstride, long long bstride) {
+    const uint64_t dims[4] = {(uint64_t)D, (uint64_t)heads, (uint64_t)S, (uint64_t)B};
+    const uint64_t bytes[3] = {(uint64_t)D * 2, (uint64_t)tstride * 2, (uint64_t)bstride * 2};
+    return encode_tmap_4d(t, x, dims, bytes, box, 2, true);
+  };
+  if (!encode(&m.q, q, Hq, Sq, q_tstride, q_bstride) || !encode(&m.dout, dout, Hq, Sq, do_tstride, do_bstride) ||
+      !encode(&m.k, k, Hkv, Sk, k_tstride, k_bstride) || !encode(&m.v, v, Hkv, Sk, v_tstride, v_bstride))
+    return -5;
+  return D == 128 ? launch_window_bwd<128>(m, prep, a, plan, stream) : launch_window_bwd<64>(m, prep, a, plan, stream);
+}

@@ -1,5 +1,5 @@
 """Sliding-window attention with first tokens that stay visible: the kernels behind
-:func:`maltos_b200.ops.attention.sliding_window_attention` (``csrc/window_attn.cu`` forward, ``csrc/flash_attn_bwd.cu`` mode 4
+:func:`maltos_b200.ops.attention.sliding_window_attention` (``csrc/window_attn.cu`` forward, ``csrc/window_attn_bwd.cu``
 backward; the rule they share is ``csrc/window.cuh``)."""
 from __future__ import annotations
 
@@ -71,7 +71,8 @@ def window_backward(q, k, v, out, out_lo, lse2, dout, *, window: int, sinks: int
     dv = torch.empty((B, Sk, Hkv, D), dtype=torch.bfloat16, device=q.device)
     L = _lib.lib()
     with _lib.on_device_of(q):
-        scratch = torch.empty((L.mb_window_attn_bwd_scratch_words(B, Sq, Sk, Hq, Hkv, D),), dtype=torch.float32, device=q.device)
+        words = L.mb_window_attn_bwd_scratch_words(B, Sq, Sk, Hq, Hkv, D, window, sinks, 0 if starts is None else 1)
+        scratch = torch.empty((words,), dtype=torch.int32, device=q.device)
         _lib.check(L.mb_window_attn_bwd(q.data_ptr(), q_t, q_b, k.data_ptr(), k_t, k_b, v.data_ptr(), v_t, v_b, out.data_ptr(),
                                         out_lo.data_ptr(), dout.data_ptr(), do_t, do_b, lse2.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(),
                                         _lib.address(starts), _lib.address(ends), scratch.data_ptr(), B, Sq, Sk, Hq, Hkv, D, window, sinks,
