@@ -77,6 +77,7 @@ __device__ __forceinline__ bool mbar_try_wait(uint64_t* bar, uint32_t parity) {
 // Bounded wait. `abort_flag` lives in shared memory and is shared by all roles of the CTA.
 // Returns false when the wait was abandoned (deadline hit here or abort raised elsewhere).
 __device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t parity, volatile int* abort_flag) {
+  if (mbar_try_wait(bar, parity)) return true;   // already there: half the cost of entering the loop
 #pragma unroll 1
   for (int i = 0; i < 4096; ++i) {
     if (mbar_try_wait(bar, parity)) return true;
@@ -411,6 +412,12 @@ __device__ __forceinline__ uint64_t mul_f32x2(uint64_t a, uint64_t b) {
   uint64_t d;
   asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
   return d;
+}
+// 32 bytes in one store; the address has to be 32-byte aligned.
+__device__ __forceinline__ void store_32_bytes(void* p, const uint32_t (&r)[8]) {
+  asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]),
+               "r"(r[5]), "r"(r[6]), "r"(r[7])
+               : "memory");
 }
 // The two values that a packed bf16 pair stands for.
 __device__ __forceinline__ uint64_t bf16x2_as_f32x2(uint32_t v) { return f32x2(__uint_as_float(v << 16), __uint_as_float(v & 0xffff0000u)); }

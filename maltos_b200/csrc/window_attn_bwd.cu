@@ -21,7 +21,7 @@
 namespace mb {
 
 constexpr int kWbArithWarps = 16;
-constexpr int kWbThreads = 32 * (2 + kWbArithWarps);   // warp 0 TMA producer, warp 1 UMMA issuer, warps 2..17 arithmetic
+constexpr int kWbThreads = 32 * (3 + kWbArithWarps);   // warp 0 TMA producer, warps 1, 2 UMMA issuers, warps 3..18 arithmetic
 constexpr float kWbLog2e = 1.4426950408889634f;
 
 struct WindowBwdArgs {
@@ -64,30 +64,29 @@ constexpr int kWbPrepThreads = 1024;
 __device__ void window_bwd_list(const WindowBwdPrepArgs& p) {
   __shared__ int warp_entries[32], warp_slots[32];
   __shared__ int total_entries, total_slots;
+  __shared__ int found[kWbPrepThreads];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int blocks = p.B * p.key_blocks, group = p.Hq / p.Hkv;
   int4* entry = reinterpret_cast<int4*>(p.list + 4);
   if (tid == 0) total_entries = total_slots = 0;
   __syncthreads();
   for (int base = 0; base < blocks; base += kWbPrepThreads) {
-    // a block per thread; with documents its range is a warp's work, one block after the other
-    int n_iter = 0;
+    // a block per thread; with documents a block's range is a warp's work, the blocks dealt out to the warps
     const int mine = base + tid;
+    auto iterations = [&](int b) {
+      const WindowKeys k = window_keys(p.rule, b / p.key_blocks, p.Sq, p.Sk, (b % p.key_blocks) * kWinBlock);
+      return k.q_hi > k.q_lo ? ((k.q_hi + kWinBlock - 1) / kWinBlock - k.q_lo / kWinBlock) * group : 0;
+    };
     if (p.rule.starts == nullptr) {
-      if (mine < blocks) {
-        const WindowKeys k = window_keys(p.rule, 0, p.Sq, p.Sk, (mine % p.key_blocks) * kWinBlock);
-        const int n = k.q_hi > k.q_lo ? (k.q_hi + kWinBlock - 1) / kWinBlock - k.q_lo / kWinBlock : 0;
-        n_iter = n * group;
-      }
+      found[tid] = mine < blocks ? iterations(mine) : 0;
     } else {
-      for (int i = 0; i < 32; ++i) {
-        const int b = base + warp * 32 + i;
-        if (b >= blocks) break;
-        const WindowKeys k = window_keys(p.rule, b / p.key_blocks, p.Sq, p.Sk, (b % p.key_blocks) * kWinBlock);
-        const int n = k.q_hi > k.q_lo ? (k.q_hi + kWinBlock - 1) / kWinBlock - k.q_lo / kWinBlock : 0;
-        if (i == lane) n_iter = n * group;
+      for (int i = warp; i < kWbPrepThreads && base + i < blocks; i += 32) {
+        const int n = iterations(base + i);
+        if (lane == 0) found[i] = n;
       }
     }
+    __syncthreads();
+    const int n_iter = mine < blocks ? found[tid] : 0;
     int n = mine < blocks ? max(1, (n_iter + p.piece - 1) / p.piece) : 0;   // a block that nobody sees still has zeros to write
     // positions by a scan over the block
     auto scan = [&](int v, int* warps, int& total, int& before) {
@@ -161,58 +160,72 @@ __global__ void __launch_bounds__(kWbPrepThreads) window_bwd_prep_kernel(const W
 }
 
 // ---------------------------------------------------------------------------------------------- dK / dV
-// One iteration is 128 keys x 128 queries of one head; S^T and dP^T have one TMEM buffer each. The issuer goes
-//     dV(i) | S(i+1) | dK(i) | dP(i+1)
-// and the arithmetic warps alternate between the exponentials of S(i+1) (under dK(i), dP(i+1)) and dS(i) (under dV(i), S(i+1)).
-// Blocks of 64 queries, which would leave room for two buffers, are bound by shared memory: a UMMA with 64 columns reads its
-// operands at 192 bytes a cycle, of 128 that there are, and everything else that needs shared memory (barriers too) waits.
+// One iteration is 128 keys x 128 queries of one head; S^T and dP^T have one TMEM buffer each, and an issuer each:
+//     dV(i) | S(i+1)      and      dK(i) | dP(i+1),
+// while the arithmetic warps alternate between the exponentials of S(i+1) (under dK(i), dP(i+1)) and dS(i) (under dV(i), S(i+1)).
+// A wait that is satisfied already still costs 50 to 250 cycles, more the busier shared memory is, so the waits of the two chains
+// run side by side, and a third Q tile lets its load start a whole iteration ahead. Blocks of 64 queries, which would leave
+// room for two buffers, are bound by shared memory: a UMMA with 64 columns reads its operands at 192 bytes a cycle, of 128.
 template <int D>
 __global__ void __launch_bounds__(kWbThreads, 1)
 window_bwd_dkdv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmDO,
                        const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV, const WindowBwdArgs p) {
   constexpr int ATOMS = D / 64;
   constexpr int TILE_BYTES = kWinBlock * D * 2, ATOM_BYTES = kWinBlock * 128;
-  constexpr int STAGES = 2;
+  constexpr int Q_STAGES = 3, STAGES = 2;           // tiles of Q; of dO, and of the statistics
   constexpr int AUX_BYTES = 2 * kWinBlock * 4;      // lse2, delta of one query tile
   constexpr uint32_t TMEM_COLS = 512, S_COL = 0, DP_COL = 128, DV_COL = 256, DK_COL = 256 + D;
 
-  extern __shared__ uint8_t smem_raw[];
-  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  extern __shared__ __align__(1024) uint8_t smem_raw[];   // with head_dim 128 the tiles fill it: its start has to be aligned
+  uint8_t* smem = smem_raw;
   uint8_t* sK = smem;
   uint8_t* sV = sK + TILE_BYTES;
-  uint8_t* sQ = sV + TILE_BYTES;                    // STAGES tiles
-  uint8_t* sDO = sQ + STAGES * TILE_BYTES;          // STAGES tiles
-  uint8_t* sAux = sDO + STAGES * TILE_BYTES;        // STAGES x AUX_BYTES, with Q
+  uint8_t* sQ = sV + TILE_BYTES;                    // Q_STAGES
+  uint8_t* sDO = sQ + Q_STAGES * TILE_BYTES;        // STAGES
+  uint8_t* sAux = sDO + STAGES * TILE_BYTES;        // STAGES x AUX_BYTES
   uint64_t* bars = reinterpret_cast<uint64_t*>(sAux + STAGES * AUX_BYTES);
   uint64_t* kv_full = bars;                 // 1
-  uint64_t* kv_empty = bars + 1;            // 1
-  uint64_t* q_full = bars + 2;              // STAGES
-  uint64_t* q_empty = bars + 4;
-  uint64_t* do_full = bars + 6;
-  uint64_t* do_empty = bars + 8;
-  uint64_t* s_full = bars + 10;             // 1
-  uint64_t* p_full = bars + 11;             // 1
-  uint64_t* dp_full = bars + 12;            // 1
-  uint64_t* ds_full = bars + 13;            // 1
-  uint64_t* acc_full = bars + 14;           // 1
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 15);
+  uint64_t* kv_empty = bars + 1;            // 1 (both issuers)
+  uint64_t* q_full = bars + 2;              // Q_STAGES
+  uint64_t* q_empty = bars + 5;             // Q_STAGES (both issuers: S, dK)
+  uint64_t* do_full = bars + 8;             // STAGES
+  uint64_t* do_empty = bars + 10;           // STAGES (both issuers: dP, dV)
+  uint64_t* aux_full = bars + 12;           // STAGES
+  uint64_t* aux_empty = bars + 14;          // STAGES
+  uint64_t* s_full = bars + 16;             // 1
+  uint64_t* p_full = bars + 17;             // 1
+  uint64_t* dp_full = bars + 18;            // 1
+  uint64_t* ds_full = bars + 19;            // 1
+  uint64_t* acc_full = bars + 20;           // 1 (both issuers)
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 21);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (smem_u32(smem_raw) & 1023u) {   // uniform over the CTA: nothing has been set up yet
+    if (threadIdx.x == 0) {
+      atomicOr(&p.status[0], MB_ERR_BAD_INDEX);
+      p.status[2] = 1014;
+    }
+    return;
+  }
   if (threadIdx.x == 0) {
     mbar_init(kv_full, 1);
-    mbar_init(kv_empty, 1);
-    for (int i = 0; i < STAGES; ++i) {
+    mbar_init(kv_empty, 2);
+    for (int i = 0; i < Q_STAGES; ++i) {
       mbar_init(&q_full[i], 1);
-      mbar_init(&q_empty[i], 1);
+      mbar_init(&q_empty[i], 2);
+    }
+    for (int i = 0; i < STAGES; ++i) {
       mbar_init(&do_full[i], 1);
-      mbar_init(&do_empty[i], 1);
+      mbar_init(&do_empty[i], 2);
+      mbar_init(&aux_full[i], 1);
+      mbar_init(&aux_empty[i], kWbArithWarps);
     }
     mbar_init(s_full, 1);
     mbar_init(p_full, kWbArithWarps);
     mbar_init(dp_full, 1);
     mbar_init(ds_full, kWbArithWarps);
-    mbar_init(acc_full, 1);
+    mbar_init(acc_full, 2);
     abort_flag[0] = 0;
     abort_flag[1] = p.status[3];
     fence_barrier_init();
@@ -256,49 +269,64 @@ window_bwd_dkdv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_con
           }
         }
         for (int it = e.y; ok && it < e.z; ++it, ++n) {
-          const int st = n % STAGES, head = kv_head * group + it / n_q, q0 = (qb + it % n_q) * kWinBlock;
+          const int qs = n % Q_STAGES, st = n % STAGES, head = kv_head * group + it / n_q, q0 = (qb + it % n_q) * kWinBlock;
           const uint32_t parity = ((n / STAGES) & 1) ^ 1;
-          ok = mbar_wait(&q_empty[st], parity, abort_flag);
+          ok = mbar_wait(&q_empty[qs], ((n / Q_STAGES) & 1) ^ 1, abort_flag);
           if (!ok) break;
-          mbar_arrive_expect_tx(&q_full[st], TILE_BYTES + AUX_BYTES);
+          mbar_arrive_expect_tx(&q_full[qs], TILE_BYTES);
 #pragma unroll
-          for (int a = 0; a < ATOMS; ++a) tma_load_4d(sQ + st * TILE_BYTES + a * ATOM_BYTES, &tmQ, &q_full[st], a * 64, head, q0, batch);
-          const long long row = (static_cast<long long>(batch) * p.Hq + head) * p.Sq_pad + q0;
-          bulk_load(sAux + st * AUX_BYTES, p.lse2 + row, kWinBlock * 4, &q_full[st]);
-          bulk_load(sAux + st * AUX_BYTES + kWinBlock * 4, p.delta + row, kWinBlock * 4, &q_full[st]);
+          for (int a = 0; a < ATOMS; ++a) tma_load_4d(sQ + qs * TILE_BYTES + a * ATOM_BYTES, &tmQ, &q_full[qs], a * 64, head, q0, batch);
           ok = mbar_wait(&do_empty[st], parity, abort_flag);
           if (!ok) break;
           mbar_arrive_expect_tx(&do_full[st], TILE_BYTES);
 #pragma unroll
           for (int a = 0; a < ATOMS; ++a) tma_load_4d(sDO + st * TILE_BYTES + a * ATOM_BYTES, &tmDO, &do_full[st], a * 64, head, q0, batch);
+          ok = mbar_wait(&aux_empty[st], parity, abort_flag);
+          if (!ok) break;
+          mbar_arrive_expect_tx(&aux_full[st], AUX_BYTES);
+          const long long row = (static_cast<long long>(batch) * p.Hq + head) * p.Sq_pad + q0;
+          bulk_load(sAux + st * AUX_BYTES, p.lse2 + row, kWinBlock * 4, &aux_full[st]);
+          bulk_load(sAux + st * AUX_BYTES + kWinBlock * 4, p.delta + row, kWinBlock * 4, &aux_full[st]);
         }
       }
       ok = __shfl_sync(0xffffffffu, static_cast<int>(ok), 0) != 0;
       if (!ok) break;
     }
-  } else if (warp == 1) {
-    // ------------------------------------------------------------------ UMMA issuer
+  } else if (warp <= 2) {
+    // ------------------------------------------------------------------ UMMA issuers: warp 1 dV and S, warp 2 dK and dP
     if (lane == 0) {
+      const bool first = warp == 1;
       const uint32_t idesc_s = make_idesc_bf16(kWinBlock, kWinBlock, 0, 0);   // [128 keys, 128 queries]
       const uint32_t idesc_acc = make_idesc_bf16(kWinBlock, D, 0, 1);         // [128 keys, D] = A(TMEM) x B(MN-major)
       constexpr uint32_t hi = smem_desc_hi_sw128(1024);
-      const uint32_t k_lo = smem_desc_lo(smem_u32(sK), 16), v_lo = smem_desc_lo(smem_u32(sV), 16);
-      auto scores = [&](uint32_t d_tmem, uint32_t a_lo, const uint8_t* b_tile) {
+      const uint32_t a_lo = smem_desc_lo(smem_u32(first ? sK : sV), 16);
+      const uint32_t score = tmem_base + (first ? S_COL : DP_COL), sum = tmem_base + (first ? DV_COL : DK_COL);
+      auto scores = [&](const uint8_t* b_tile) {
         const uint32_t b_lo = smem_desc_lo(smem_u32(b_tile), 16);
 #pragma unroll
         for (int kk = 0; kk < D / 16; ++kk) {
           const uint32_t o = static_cast<uint32_t>(((kk >> 2) * ATOM_BYTES + (kk & 3) * 32) >> 4);
-          umma_bf16_ss_lh(d_tmem, a_lo + o, hi, b_lo + o, hi, idesc_s, kk != 0 ? 1u : 0u);
+          umma_bf16_ss_lh(score, a_lo + o, hi, b_lo + o, hi, idesc_s, kk != 0 ? 1u : 0u);
         }
+        umma_commit(first ? s_full : dp_full);
       };
-      auto accumulate = [&](uint32_t d_tmem, uint32_t a_tmem, const uint8_t* b_tile, bool first) {
+      auto accumulate = [&](const uint8_t* b_tile, bool begin) {
         const uint32_t b_lo = smem_desc_lo(smem_u32(b_tile), ATOM_BYTES);
-        const uint32_t acc0 = first ? 0u : 1u;
 #pragma unroll
         for (int kk = 0; kk < kWinBlock / 16; ++kk)   // the 32 queries of a warp group sit packed in the first 16 of their 32 columns
-          umma_bf16_ts_lh(d_tmem, a_tmem + static_cast<uint32_t>((kk >> 1) * 32 + (kk & 1) * 8), b_lo + static_cast<uint32_t>(kk * 128), hi,
-                          idesc_acc, kk != 0 ? 1u : acc0);
+          umma_bf16_ts_lh(sum, score + static_cast<uint32_t>((kk >> 1) * 32 + (kk & 1) * 8), b_lo + static_cast<uint32_t>(kk * 128), hi, idesc_acc,
+                          kk != 0 ? 1u : begin ? 0u : 1u);
       };
+      // the tile that the scores are formed from (Q or dO), and the one that the sums are (dO or Q)
+      auto wait_scores = [&](int n) {
+        return first ? mbar_wait(&q_full[n % Q_STAGES], (n / Q_STAGES) & 1, abort_flag) : mbar_wait(&do_full[n % STAGES], (n / STAGES) & 1, abort_flag);
+      };
+      auto wait_sums = [&](int n) {
+        return first ? mbar_wait(&do_full[n % STAGES], (n / STAGES) & 1, abort_flag) : mbar_wait(&q_full[n % Q_STAGES], (n / Q_STAGES) & 1, abort_flag);
+      };
+      auto q_tile = [&](int n) { return sQ + (n % Q_STAGES) * TILE_BYTES; };
+      auto do_tile = [&](int n) { return sDO + (n % STAGES) * TILE_BYTES; };
+      uint64_t* ready = first ? p_full : ds_full;
       uint32_t kv_phase = 0;
       int n = 0;
       bool ok = true;
@@ -306,42 +334,25 @@ window_bwd_dkdv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_con
         const int4 e = entry[item / p.Hkv];
         const int len = e.z - e.y;
         if (len <= 0) continue;
-        int st = n % STAGES;
-        uint32_t par = (n / STAGES) & 1;
-        ok = mbar_wait(kv_full, kv_phase & 1, abort_flag) && mbar_wait(&q_full[st], par, abort_flag) && mbar_wait(&do_full[st], par, abort_flag);
+        ok = mbar_wait(kv_full, kv_phase & 1, abort_flag) && wait_scores(n);
         ++kv_phase;
         if (!ok) break;
         tc_fence_after();
-        scores(tmem_base + S_COL, k_lo, sQ + st * TILE_BYTES);
-        umma_commit(s_full);
-        scores(tmem_base + DP_COL, v_lo, sDO + st * TILE_BYTES);
-        umma_commit(dp_full);
+        scores(first ? q_tile(n) : do_tile(n));
+        umma_commit(first ? &q_empty[n % Q_STAGES] : &do_empty[n % STAGES]);
         if (len == 1) umma_commit(kv_empty);
         for (int i = 0; i < len; ++i, ++n) {
-          st = n % STAGES;
-          const int st1 = (n + 1) % STAGES;
-          const uint32_t par1 = ((n + 1) / STAGES) & 1;
           const bool more = i + 1 < len;
-          ok = (!more || (mbar_wait(&q_full[st1], par1, abort_flag) && mbar_wait(&do_full[st1], par1, abort_flag))) &&
-               mbar_wait(p_full, n & 1, abort_flag);
+          ok = wait_sums(n) && (!more || wait_scores(n + 1)) && mbar_wait(ready, n & 1, abort_flag);
           if (!ok) break;
           tc_fence_after();
-          accumulate(tmem_base + DV_COL, tmem_base + S_COL, sDO + st * TILE_BYTES, i == 0);
+          accumulate(first ? do_tile(n) : q_tile(n), i == 0);
           if (more) {
-            scores(tmem_base + S_COL, k_lo, sQ + st1 * TILE_BYTES);
-            umma_commit(s_full);
-          }
-          umma_commit(&do_empty[st]);
-          ok = mbar_wait(ds_full, n & 1, abort_flag);
-          if (!ok) break;
-          tc_fence_after();
-          accumulate(tmem_base + DK_COL, tmem_base + DP_COL, sQ + st * TILE_BYTES, i == 0);
-          if (more) {
-            scores(tmem_base + DP_COL, v_lo, sDO + st1 * TILE_BYTES);
-            umma_commit(dp_full);
+            scores(first ? q_tile(n + 1) : do_tile(n + 1));
+            umma_commit(first ? &q_empty[(n + 1) % Q_STAGES] : &do_empty[(n + 1) % STAGES]);
             if (i + 2 == len) umma_commit(kv_empty);   // K and V are not read again: the next item's may come
           }
-          umma_commit(&q_empty[st]);
+          umma_commit(first ? &do_empty[n % STAGES] : &q_empty[n % Q_STAGES]);
         }
         if (ok) umma_commit(acc_full);
       }
@@ -350,7 +361,7 @@ window_bwd_dkdv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_con
   } else {
     // ------------------------------------------------------------------ arithmetic: lane = key, 32 query columns per thread
     const int qw = warp & 3;                        // TMEM lane quarter this warp may touch
-    const int grp = (warp - 2) >> 2;                // which 32 of the 128 queries
+    const int grp = (warp - 3) >> 2;                // which 32 of the 128 queries
     const int row = qw * 32 + lane;
     const uint32_t t_lane = static_cast<uint32_t>(qw * 32) << 16;
     const uint32_t t_s = tmem_base + S_COL + static_cast<uint32_t>(grp * 32) + t_lane;
@@ -375,47 +386,37 @@ window_bwd_dkdv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_con
         const int st = n % STAGES;
         const float* aux = reinterpret_cast<const float*>(sAux + st * AUX_BYTES) + grp * 32;
         const int pos0 = (qb + it % n_q) * kWinBlock + off;     // position of the tile's first query
-        ok = mbar_wait(&q_full[st], (n / STAGES) & 1, abort_flag);   // the statistics; the scores come later
-        uint64_t pr[16];                            // -lse2, then P, of 16 pairs
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const float4 v = reinterpret_cast<const float4*>(aux)[i];
-          pr[2 * i] = f32x2(-v.x, -v.y), pr[2 * i + 1] = f32x2(-v.z, -v.w);
-        }
-        ok = ok && mbar_wait(s_full, n & 1, abort_flag);
+        ok = mbar_wait(&aux_full[st], (n / STAGES) & 1, abort_flag) && mbar_wait(s_full, n & 1, abort_flag);
         ok = __all_sync(0xffffffffu, ok);
         if (!ok) break;
         tc_fence_after();
-        uint32_t t[32];
+        uint32_t t[32], wt[16];                     // scores (later dP); P in bf16, two a register
         tmem_ld_32x32b_x32(t_s, t);
+        uint32_t seen = 0xffffffffu;
+        if (pos0 < k0 + kWinBlock - 1 || pos0 + kWinBlock > wk.full_hi) seen = interval_bits(pos0 + grp * 32, kj, upper);
         tmem_ld_wait();
+        const bool some = __any_sync(0xffffffffu, seen != 0u);
+        if (some) {
 #pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          float a, b;
-          f32x2_split(fma_f32x2(f32x2(__uint_as_float(t[2 * i]), __uint_as_float(t[2 * i + 1])), scale2, pr[i]), a, b);
-          pr[i] = f32x2(wb_exp2(a), wb_exp2(b));
-        }
-        if (pos0 < k0 + kWinBlock - 1 || pos0 + kWinBlock > wk.full_hi) {
-          const uint32_t seen = interval_bits(pos0 + grp * 32, kj, upper);
+          for (int i = 0; i < 8; ++i) {
+            const float4 v = reinterpret_cast<const float4*>(aux)[i];
+            float a, b, c, d;
+            f32x2_split(fma_f32x2(f32x2(__uint_as_float(t[4 * i]), __uint_as_float(t[4 * i + 1])), scale2, f32x2(-v.x, -v.y)), a, b);
+            f32x2_split(fma_f32x2(f32x2(__uint_as_float(t[4 * i + 2]), __uint_as_float(t[4 * i + 3])), scale2, f32x2(-v.z, -v.w)), c, d);
+            wt[2 * i] = pack_bf16x2(wb_exp2(a), wb_exp2(b)), wt[2 * i + 1] = pack_bf16x2(wb_exp2(c), wb_exp2(d));
+          }
           if (!__all_sync(0xffffffffu, seen == 0xffffffffu)) {
 #pragma unroll
             for (int i = 0; i < 16; ++i) {
-              float a, b;
-              f32x2_split(pr[i], a, b);
-              pr[i] = f32x2((seen >> (2 * i)) & 1u ? a : 0.f, (seen >> (2 * i + 1)) & 1u ? b : 0.f);
+              if (!((seen >> (2 * i)) & 1u)) wt[i] &= 0xffff0000u;
+              if (!((seen >> (2 * i + 1)) & 1u)) wt[i] &= 0x0000ffffu;
             }
           }
-        }
-        {
-          uint32_t pk[16];
+        } else {                                    // far queries of a block with a few first tokens: most keys are not theirs
 #pragma unroll
-          for (int i = 0; i < 16; ++i) {
-            float a, b;
-            f32x2_split(pr[i], a, b);
-            pk[i] = pack_bf16x2(a, b);
-          }
-          tmem_st_32x32b_x16(t_s, pk);
+          for (int i = 0; i < 16; ++i) wt[i] = 0u;
         }
+        tmem_st_32x32b_x16(t_s, wt);
         tmem_st_wait();
         tc_fence_before();
         __syncwarp();
@@ -425,29 +426,26 @@ window_bwd_dkdv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_con
         ok = __all_sync(0xffffffffu, ok);
         if (!ok) break;
         tc_fence_after();
-        tmem_ld_32x32b_x32(t_dp, t);
-        tmem_ld_wait();
-        {
-          uint32_t ds[16];
+        if (some) {
+          tmem_ld_32x32b_x32(t_dp, t);
+          tmem_ld_wait();
 #pragma unroll
           for (int i = 0; i < 8; ++i) {
             const float4 v = reinterpret_cast<const float4*>(aux + kWinBlock)[i];
-#pragma unroll
-            for (int k = 0; k < 2; ++k) {
-              const int j = 2 * i + k;
-              const uint64_t dl = k ? f32x2(v.z, v.w) : f32x2(v.x, v.y);
-              const uint64_t d = fma_f32x2(dl, minus, f32x2(__uint_as_float(t[2 * j]), __uint_as_float(t[2 * j + 1])));
-              float a, b;
-              f32x2_split(mul_f32x2(pr[j], d), a, b);
-              ds[j] = pack_bf16x2(a, b);
-            }
+            float a, b, c, d;
+            f32x2_split(mul_f32x2(bf16x2_as_f32x2(wt[2 * i]), fma_f32x2(f32x2(v.x, v.y), minus, f32x2(__uint_as_float(t[4 * i]), __uint_as_float(t[4 * i + 1])))), a, b);
+            f32x2_split(mul_f32x2(bf16x2_as_f32x2(wt[2 * i + 1]), fma_f32x2(f32x2(v.z, v.w), minus, f32x2(__uint_as_float(t[4 * i + 2]), __uint_as_float(t[4 * i + 3])))), c, d);
+            wt[2 * i] = pack_bf16x2(a, b), wt[2 * i + 1] = pack_bf16x2(c, d);
           }
-          tmem_st_32x32b_x16(t_dp, ds);
         }
+        tmem_st_32x32b_x16(t_dp, wt);
         tmem_st_wait();
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive(ds_full);
+        if (lane == 0) {
+          mbar_arrive(&aux_empty[st]);
+          mbar_arrive(ds_full);
+        }
       }
       if (!ok) break;
       // ---------------------------------------------------------------- this piece's dK, dV rows
@@ -478,17 +476,17 @@ window_bwd_dkdv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_con
           }
           if (part) {                               // rows past the end hold zeros there
 #pragma unroll
-            for (int i = 0; i < 16; i += 4)
-              *reinterpret_cast<float4*>(part + which * kWinBlock * D + c + i) =
-                  make_float4(__uint_as_float(r[i]) * mul, __uint_as_float(r[i + 1]) * mul, __uint_as_float(r[i + 2]) * mul, __uint_as_float(r[i + 3]) * mul);
-          } else if (kj < p.Sk) {
-#pragma unroll
             for (int i = 0; i < 16; i += 8) {
-              uint32_t v[4];
+              uint32_t v[8];
 #pragma unroll
-              for (int k = 0; k < 4; ++k) v[k] = pack_bf16x2(__uint_as_float(r[i + 2 * k]) * mul, __uint_as_float(r[i + 2 * k + 1]) * mul);
-              *reinterpret_cast<uint4*>(dst + to + c + i) = make_uint4(v[0], v[1], v[2], v[3]);
+              for (int k = 0; k < 8; ++k) v[k] = __float_as_uint(__uint_as_float(r[i + k]) * mul);
+              store_32_bytes(part + which * kWinBlock * D + c + i, v);
             }
+          } else if (kj < p.Sk) {
+            uint32_t v[8];
+#pragma unroll
+            for (int k = 0; k < 8; ++k) v[k] = pack_bf16x2(__uint_as_float(r[2 * k]) * mul, __uint_as_float(r[2 * k + 1]) * mul);
+            store_32_bytes(dst + to + c, v);
           }
         }
       }
@@ -536,11 +534,9 @@ __global__ void __launch_bounds__(256) window_bwd_join_kernel(const WindowBwdArg
 }
 
 // ---------------------------------------------------------------------------------------------- dQ
-// The items' key blocks form one stream; element g has its scores in TMEM buffer g & 1. The issuer goes
-//     dQ(g-1) | S(g+1) | dP(g+1)
-// while the arithmetic warps work on element g. dQ(g-1) frees the buffer of S(g+1); dP has one buffer, free as soon as the
-// arithmetic has it in registers. What was loaded long ago is waited for before the wait on dS, so that nothing but a (by then
-// satisfied) wait stands between the three products.
+// The items' key blocks form one stream; element g has its scores in TMEM buffer g & 1. One issuer goes S(g) | dP(g), the other
+// dQ(g) as soon as dS(g) is there; the arithmetic warps work on element g while S and dP of g + 1 are formed. dQ(g-1) frees the
+// buffer of S(g+1); dP has one buffer, free as soon as the arithmetic has it in registers.
 template <int D>
 __global__ void __launch_bounds__(kWbThreads, 1)
 window_bwd_dq_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmDO,
@@ -567,7 +563,8 @@ window_bwd_dq_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
   uint64_t* dp_free = bars + 15;      // 1
   uint64_t* ds_full = bars + 16;      // 2: the arithmetic may finish element g + 1 before the issuer asks for element g
   uint64_t* dq_full = bars + 18;      // 1
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 19);
+  uint64_t* s_empty = bars + 19;      // 2: dQ has read the buffer
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 21);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -596,6 +593,8 @@ window_bwd_dq_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
     mbar_init(&ds_full[0], kWbArithWarps);
     mbar_init(&ds_full[1], kWbArithWarps);
     mbar_init(dq_full, 1);
+    mbar_init(&s_empty[0], 1);
+    mbar_init(&s_empty[1], 1);
     abort_flag[0] = 0;
     abort_flag[1] = p.status[3];
     fence_barrier_init();
@@ -672,8 +671,8 @@ window_bwd_dq_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
       ok = __shfl_sync(0xffffffffu, static_cast<int>(ok), 0) != 0;
       if (!ok) break;
     }
-  } else if (warp == 1) {
-    // ------------------------------------------------------------------ UMMA issuer
+  } else if (warp <= 2) {
+    // ------------------------------------------------------------------ UMMA issuers: warp 1 S and dP, warp 2 dQ
     const uint32_t idesc_s = make_idesc_bf16(kWinBlock, kWinBlock, 0, 0);   // [128 q, 128 keys]
     const uint32_t idesc_dq = make_idesc_bf16(kWinBlock, D, 0, 1);          // [128 q, D] = A(TMEM) x B(K tile, MN-major)
     constexpr uint32_t hi = smem_desc_hi_sw128(1024);
@@ -686,24 +685,9 @@ window_bwd_dq_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
         umma_bf16_ss_lh(d_tmem, a_lo + o, hi, b_lo + o, hi, idesc_s, kk != 0 ? 1u : 0u);
       }
     };
-    int g = 0;                                      // element whose scores are issued next
+    int g = 0;
     uint32_t q_phase = 0;
     bool ok = true;
-    // place in their items of the two elements whose dQ is still to come: bit 0 first, bit 1 last
-    int place1 = 0, place2 = 0;                     // of elements g - 1 and g - 2
-    auto finish = [&](int e, int place) {           // dQ of element e
-      ok = mbar_wait(&ds_full[e & 1], (e >> 1) & 1, abort_flag);
-      if (!ok) return;
-      tc_fence_after();
-      const uint32_t k_lo = smem_desc_lo(smem_u32(sK + (e % K_STAGES) * TILE_BYTES), ATOM_BYTES);
-      const uint32_t s_col = tmem_base + static_cast<uint32_t>(e & 1) * 128u, acc0 = (place & 1) ? 0u : 1u;
-#pragma unroll
-      for (int kk = 0; kk < kWinBlock / 16; ++kk)   // the 32 keys of a warp group sit packed in the first 16 of their 32 columns
-        umma_bf16_ts_lh(tmem_base + DQ_COL, s_col + static_cast<uint32_t>((kk >> 1) * 32 + (kk & 1) * 8), k_lo + static_cast<uint32_t>(kk * 128), hi,
-                        idesc_dq, kk != 0 ? 1u : acc0);
-      umma_commit(&k_empty[e % K_STAGES]);
-      if (place & 2) umma_commit(dq_full);
-    };
     for (int item = blockIdx.x; item < items; item += gridDim.x) {
       int batch, head, q0;
       where(item, batch, head, q0);
@@ -711,42 +695,46 @@ window_bwd_dq_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
       if (lane == 0) {
         for (int j = 0; j < n; ++j, ++g) {
           const int ks = g % K_STAGES, vs = g % V_STAGES;
-          ok = mbar_wait(&k_full[ks], (g / K_STAGES) & 1, abort_flag) && mbar_wait(&v_full[vs], (g / V_STAGES) & 1, abort_flag);
-          if (!ok) break;
-          if (g >= 2) finish(g - 2, place2);
-          if (ok && j == 0) {
-            ok = mbar_wait(q_full, q_phase & 1, abort_flag);
-            ++q_phase;
-          }
-          if (!ok) break;
-          tc_fence_after();
-          scores(tmem_base + static_cast<uint32_t>(g & 1) * 128u, q_lo, sK + ks * TILE_BYTES);
-          umma_commit(&s_full[g & 1]);
-          if (g >= 1) {
-            ok = mbar_wait(dp_free, (g - 1) & 1, abort_flag);
+          const uint32_t k_phase = (g / K_STAGES) & 1;
+          if (warp == 1) {
+            ok = mbar_wait(&k_full[ks], k_phase, abort_flag) && (j > 0 || mbar_wait(q_full, q_phase & 1, abort_flag)) &&
+                 mbar_wait(&s_empty[g & 1], ((g >> 1) & 1) ^ 1, abort_flag);
+            if (!ok) break;
+            if (j == 0) ++q_phase;
+            tc_fence_after();
+            scores(tmem_base + static_cast<uint32_t>(g & 1) * 128u, q_lo, sK + ks * TILE_BYTES);
+            umma_commit(&s_full[g & 1]);
+            ok = mbar_wait(&v_full[vs], (g / V_STAGES) & 1, abort_flag) && mbar_wait(dp_free, (g & 1) ^ 1, abort_flag);
             if (!ok) break;
             tc_fence_after();
+            scores(tmem_base + DP_COL, do_lo, sV + vs * TILE_BYTES);
+            umma_commit(dp_full);
+            umma_commit(&v_empty[vs]);
+            if (j + 1 == n) umma_commit(q_empty);
+          } else {
+            ok = mbar_wait(&k_full[ks], k_phase, abort_flag) && mbar_wait(&ds_full[g & 1], (g >> 1) & 1, abort_flag);
+            if (!ok) break;
+            tc_fence_after();
+            const uint32_t k_lo = smem_desc_lo(smem_u32(sK + ks * TILE_BYTES), ATOM_BYTES);
+            const uint32_t s_col = tmem_base + static_cast<uint32_t>(g & 1) * 128u;
+#pragma unroll
+            for (int kk = 0; kk < kWinBlock / 16; ++kk)   // the 32 keys of a warp group sit packed in the first 16 of their 32 columns
+              umma_bf16_ts_lh(tmem_base + DQ_COL, s_col + static_cast<uint32_t>((kk >> 1) * 32 + (kk & 1) * 8), k_lo + static_cast<uint32_t>(kk * 128),
+                              hi, idesc_dq, kk != 0 || j != 0 ? 1u : 0u);
+            umma_commit(&s_empty[g & 1]);
+            umma_commit(&k_empty[ks]);
+            if (j + 1 == n) umma_commit(dq_full);
           }
-          scores(tmem_base + DP_COL, do_lo, sV + vs * TILE_BYTES);
-          umma_commit(dp_full);
-          umma_commit(&v_empty[vs]);
-          if (j + 1 == n) umma_commit(q_empty);
-          place2 = place1;
-          place1 = (j == 0 ? 1 : 0) | (j + 1 == n ? 2 : 0);
         }
       }
       ok = __shfl_sync(0xffffffffu, static_cast<int>(ok), 0) != 0;
       if (!ok) break;
     }
-    if (lane == 0 && ok) {
-      if (g >= 2) finish(g - 2, place2);
-      if (ok && g >= 1) finish(g - 1, place1);
-    }
     __syncwarp();
   } else {
     // ------------------------------------------------------------------ arithmetic: lane = query row, 32 key columns per thread
     const int qw = warp & 3;
-    const int grp = (warp - 2) >> 2;                // which 32 of the 128 keys
+    const int grp = (warp - 3) >> 2;                // which 32 of the 128 keys
     const int row = qw * 32 + lane;
     const uint32_t t_lane = static_cast<uint32_t>(qw * 32) << 16;
     const uint32_t t_dp = tmem_base + DP_COL + static_cast<uint32_t>(grp * 32) + t_lane;
@@ -838,13 +826,10 @@ window_bwd_dq_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
           tmem_ld_wait();
         }
         if (qi < p.Sq) {
+          uint32_t v[8];
 #pragma unroll
-          for (int i = 0; i < 16; i += 8) {
-            uint32_t v[4];
-#pragma unroll
-            for (int k = 0; k < 4; ++k) v[k] = pack_bf16x2(__uint_as_float(r[i + 2 * k]) * p.scale, __uint_as_float(r[i + 2 * k + 1]) * p.scale);
-            *reinterpret_cast<uint4*>(dst + c + i) = make_uint4(v[0], v[1], v[2], v[3]);
-          }
+          for (int k = 0; k < 8; ++k) v[k] = pack_bf16x2(__uint_as_float(r[2 * k]) * p.scale, __uint_as_float(r[2 * k + 1]) * p.scale);
+          store_32_bytes(dst + c, v);
         }
       }
       tc_fence_before();                            // before the next item's first dQ (via ds_full)
@@ -913,8 +898,8 @@ static WindowBwdPlan window_bwd_plan(int B, int Sq, int Sk, int Hq, int Hkv, int
   w.rows = static_cast<long long>(B) * Hq * w.sq_pad;
   w.at_delta = w.rows;
   w.at_list = 2 * w.rows;
-  w.at_pieces = w.at_list + 4 + 4 * (w.blocks + slots);
-  w.at_parts = (w.at_pieces + 2 * w.blocks + 3) / 4 * 4;
+  w.at_pieces = w.at_list + 4 + 4 * (w.blocks + slots);       // int4 entries: at_list is a multiple of 128 words
+  w.at_parts = (w.at_pieces + 2 * w.blocks + 7) / 8 * 8;     // stored 32 bytes at a time
   w.words = w.at_parts + slots * Hkv * 2 * kWinBlock * D;
   return w;
 }
@@ -927,7 +912,7 @@ template <int D>
 static int launch_window_bwd(const WindowBwdMaps& m, const WindowBwdPrepArgs& prep, const WindowBwdArgs& a, const WindowBwdPlan& plan,
                              cudaStream_t stream) {
   constexpr size_t tile = kWinBlock * D * 2;
-  constexpr size_t smem_dkdv = 1024 + 6 * tile + 2 * (2 * kWinBlock * 4) + 256, smem_dq = 7 * tile + 256;
+  constexpr size_t smem_dkdv = 7 * tile + 2 * (2 * kWinBlock * 4) + 256, smem_dq = 7 * tile + 256;
   static bool configured[64] = {false};
   int dev = 0;
   MB_CHECK_CUDA(cudaGetDevice(&dev));
@@ -974,6 +959,11 @@ MB_API int mb_window_attn_bwd(const void* q, long long q_tstride, long long q_bs
   if (const char* what = window_attn_problem(B, Sq, Sk, Hq, Hkv, D, window, sinks, strides, 8, pointers, 10)) {
     set_last_error(what);
     return -1;
+  }
+  if ((reinterpret_cast<uintptr_t>(dq) | reinterpret_cast<uintptr_t>(dk) | reinterpret_cast<uintptr_t>(dv) |
+       reinterpret_cast<uintptr_t>(scratch)) & 31) {
+    set_last_error("mb_window_attn_bwd: gradients and scratch must be 32-byte aligned");
+    return -3;
   }
   if ((starts == nullptr) != (ends == nullptr)) {
     set_last_error("mb_window_attn_bwd: starts and ends come together");
