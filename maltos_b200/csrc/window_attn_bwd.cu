@@ -21,7 +21,7 @@
 namespace mb {
 
 constexpr int kWbArithWarps = 16;
-constexpr int kWbThreads = 32 * (3 + kWbArithWarps);   // warp 0 TMA producer, warps 1, 2 UMMA issuers, warps 3..18 arithmetic
+constexpr int kWbThreads = 32 * (4 + kWbArithWarps);   // warp 0 TMA producer, warps 1..3 UMMA issuers, warps 4..19 arithmetic
 constexpr float kWbLog2e = 1.4426950408889634f;
 
 struct WindowBwdArgs {
@@ -160,12 +160,14 @@ __global__ void __launch_bounds__(kWbPrepThreads) window_bwd_prep_kernel(const W
 }
 
 // ---------------------------------------------------------------------------------------------- dK / dV
-// One iteration is 128 keys x 128 queries of one head; S^T and dP^T have one TMEM buffer each, and an issuer each:
-//     dV(i) | S(i+1)      and      dK(i) | dP(i+1),
-// while the arithmetic warps alternate between the exponentials of S(i+1) (under dK(i), dP(i+1)) and dS(i) (under dV(i), S(i+1)).
-// A wait that is satisfied already still costs 50 to 250 cycles, more the busier shared memory is, so the waits of the two chains
-// run side by side, and a third Q tile lets its load start a whole iteration ahead. Blocks of 64 queries, which would leave
-// room for two buffers, are bound by shared memory: a UMMA with 64 columns reads its operands at 192 bytes a cycle, of 128.
+// One iteration is 128 keys x 128 queries of one head; S^T and dP^T have one TMEM buffer each. The issuer goes
+//     dV(i) | S(i+1) | dK(i) | dP(i+1)
+// and the arithmetic warps alternate between the exponentials of S(i+1) (under dK(i), dP(i+1)) and dS(i) (under dV(i), S(i+1)).
+// One thread issues all four: S(i+1) is what the arithmetic waits for, and with an issuer for each pair dK and dP share the tensor
+// cores with it (4100 cycles an iteration against 2048 of UMMAs). A wait that is satisfied already still costs 50 to 250
+// cycles, more the busier shared memory is, so tiles are waited for while the products before them run, and a third Q tile lets
+// its load start a whole iteration ahead. Blocks of 64 queries, which would leave room for two buffers, are bound by shared
+// memory: a UMMA with 64 columns reads its operands at 192 bytes a cycle, of 128 that there are.
 template <int D>
 __global__ void __launch_bounds__(kWbThreads, 1)
 window_bwd_dkdv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmDO,
@@ -185,18 +187,18 @@ window_bwd_dkdv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_con
   uint8_t* sAux = sDO + STAGES * TILE_BYTES;        // STAGES x AUX_BYTES
   uint64_t* bars = reinterpret_cast<uint64_t*>(sAux + STAGES * AUX_BYTES);
   uint64_t* kv_full = bars;                 // 1
-  uint64_t* kv_empty = bars + 1;            // 1 (both issuers)
+  uint64_t* kv_empty = bars + 1;            // 1
   uint64_t* q_full = bars + 2;              // Q_STAGES
-  uint64_t* q_empty = bars + 5;             // Q_STAGES (both issuers: S, dK)
+  uint64_t* q_empty = bars + 5;             // Q_STAGES
   uint64_t* do_full = bars + 8;             // STAGES
-  uint64_t* do_empty = bars + 10;           // STAGES (both issuers: dP, dV)
+  uint64_t* do_empty = bars + 10;           // STAGES
   uint64_t* aux_full = bars + 12;           // STAGES
   uint64_t* aux_empty = bars + 14;          // STAGES
   uint64_t* s_full = bars + 16;             // 1
   uint64_t* p_full = bars + 17;             // 1
   uint64_t* dp_full = bars + 18;            // 1
   uint64_t* ds_full = bars + 19;            // 1
-  uint64_t* acc_full = bars + 20;           // 1 (both issuers)
+  uint64_t* acc_full = bars + 20;           // 1
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 21);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
@@ -210,14 +212,14 @@ window_bwd_dkdv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_con
   }
   if (threadIdx.x == 0) {
     mbar_init(kv_full, 1);
-    mbar_init(kv_empty, 2);
+    mbar_init(kv_empty, 1);
     for (int i = 0; i < Q_STAGES; ++i) {
       mbar_init(&q_full[i], 1);
-      mbar_init(&q_empty[i], 2);
+      mbar_init(&q_empty[i], 1);
     }
     for (int i = 0; i < STAGES; ++i) {
       mbar_init(&do_full[i], 1);
-      mbar_init(&do_empty[i], 2);
+      mbar_init(&do_empty[i], 1);
       mbar_init(&aux_full[i], 1);
       mbar_init(&aux_empty[i], kWbArithWarps);
     }
@@ -225,7 +227,7 @@ window_bwd_dkdv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_con
     mbar_init(p_full, kWbArithWarps);
     mbar_init(dp_full, 1);
     mbar_init(ds_full, kWbArithWarps);
-    mbar_init(acc_full, 2);
+    mbar_init(acc_full, 1);
     abort_flag[0] = 0;
     abort_flag[1] = p.status[3];
     fence_barrier_init();
@@ -292,41 +294,32 @@ window_bwd_dkdv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_con
       ok = __shfl_sync(0xffffffffu, static_cast<int>(ok), 0) != 0;
       if (!ok) break;
     }
-  } else if (warp <= 2) {
-    // ------------------------------------------------------------------ UMMA issuers: warp 1 dV and S, warp 2 dK and dP
-    if (lane == 0) {
-      const bool first = warp == 1;
+  } else if (warp < 4) {
+    // ------------------------------------------------------------------ UMMA issuer (warp 1; 2 and 3 have nothing to do here)
+    if (warp == 1 && lane == 0) {
       const uint32_t idesc_s = make_idesc_bf16(kWinBlock, kWinBlock, 0, 0);   // [128 keys, 128 queries]
       const uint32_t idesc_acc = make_idesc_bf16(kWinBlock, D, 0, 1);         // [128 keys, D] = A(TMEM) x B(MN-major)
       constexpr uint32_t hi = smem_desc_hi_sw128(1024);
-      const uint32_t a_lo = smem_desc_lo(smem_u32(first ? sK : sV), 16);
-      const uint32_t score = tmem_base + (first ? S_COL : DP_COL), sum = tmem_base + (first ? DV_COL : DK_COL);
-      auto scores = [&](const uint8_t* b_tile) {
+      const uint32_t k_lo = smem_desc_lo(smem_u32(sK), 16), v_lo = smem_desc_lo(smem_u32(sV), 16);
+      auto scores = [&](uint32_t d_tmem, uint32_t a_lo, const uint8_t* b_tile) {
         const uint32_t b_lo = smem_desc_lo(smem_u32(b_tile), 16);
 #pragma unroll
         for (int kk = 0; kk < D / 16; ++kk) {
           const uint32_t o = static_cast<uint32_t>(((kk >> 2) * ATOM_BYTES + (kk & 3) * 32) >> 4);
-          umma_bf16_ss_lh(score, a_lo + o, hi, b_lo + o, hi, idesc_s, kk != 0 ? 1u : 0u);
+          umma_bf16_ss_lh(d_tmem, a_lo + o, hi, b_lo + o, hi, idesc_s, kk != 0 ? 1u : 0u);
         }
-        umma_commit(first ? s_full : dp_full);
       };
-      auto accumulate = [&](const uint8_t* b_tile, bool begin) {
+      auto accumulate = [&](uint32_t d_tmem, uint32_t a_tmem, const uint8_t* b_tile, bool begin) {
         const uint32_t b_lo = smem_desc_lo(smem_u32(b_tile), ATOM_BYTES);
 #pragma unroll
         for (int kk = 0; kk < kWinBlock / 16; ++kk)   // the 32 queries of a warp group sit packed in the first 16 of their 32 columns
-          umma_bf16_ts_lh(sum, score + static_cast<uint32_t>((kk >> 1) * 32 + (kk & 1) * 8), b_lo + static_cast<uint32_t>(kk * 128), hi, idesc_acc,
-                          kk != 0 ? 1u : begin ? 0u : 1u);
+          umma_bf16_ts_lh(d_tmem, a_tmem + static_cast<uint32_t>((kk >> 1) * 32 + (kk & 1) * 8), b_lo + static_cast<uint32_t>(kk * 128), hi,
+                          idesc_acc, kk != 0 ? 1u : begin ? 0u : 1u);
       };
-      // the tile that the scores are formed from (Q or dO), and the one that the sums are (dO or Q)
-      auto wait_scores = [&](int n) {
-        return first ? mbar_wait(&q_full[n % Q_STAGES], (n / Q_STAGES) & 1, abort_flag) : mbar_wait(&do_full[n % STAGES], (n / STAGES) & 1, abort_flag);
-      };
-      auto wait_sums = [&](int n) {
-        return first ? mbar_wait(&do_full[n % STAGES], (n / STAGES) & 1, abort_flag) : mbar_wait(&q_full[n % Q_STAGES], (n / Q_STAGES) & 1, abort_flag);
-      };
+      auto wait_q = [&](int n) { return mbar_wait(&q_full[n % Q_STAGES], (n / Q_STAGES) & 1, abort_flag); };
+      auto wait_do = [&](int n) { return mbar_wait(&do_full[n % STAGES], (n / STAGES) & 1, abort_flag); };
       auto q_tile = [&](int n) { return sQ + (n % Q_STAGES) * TILE_BYTES; };
       auto do_tile = [&](int n) { return sDO + (n % STAGES) * TILE_BYTES; };
-      uint64_t* ready = first ? p_full : ds_full;
       uint32_t kv_phase = 0;
       int n = 0;
       bool ok = true;
@@ -334,25 +327,36 @@ window_bwd_dkdv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_con
         const int4 e = entry[item / p.Hkv];
         const int len = e.z - e.y;
         if (len <= 0) continue;
-        ok = mbar_wait(kv_full, kv_phase & 1, abort_flag) && wait_scores(n);
+        ok = mbar_wait(kv_full, kv_phase & 1, abort_flag) && wait_q(n) && wait_do(n);
         ++kv_phase;
         if (!ok) break;
         tc_fence_after();
-        scores(first ? q_tile(n) : do_tile(n));
-        umma_commit(first ? &q_empty[n % Q_STAGES] : &do_empty[n % STAGES]);
+        scores(tmem_base + S_COL, k_lo, q_tile(n));
+        umma_commit(s_full);
+        scores(tmem_base + DP_COL, v_lo, do_tile(n));
+        umma_commit(dp_full);
         if (len == 1) umma_commit(kv_empty);
         for (int i = 0; i < len; ++i, ++n) {
           const bool more = i + 1 < len;
-          ok = wait_sums(n) && (!more || wait_scores(n + 1)) && mbar_wait(ready, n & 1, abort_flag);
+          ok = (!more || wait_q(n + 1)) && mbar_wait(p_full, n & 1, abort_flag);
           if (!ok) break;
           tc_fence_after();
-          accumulate(first ? do_tile(n) : q_tile(n), i == 0);
+          accumulate(tmem_base + DV_COL, tmem_base + S_COL, do_tile(n), i == 0);
           if (more) {
-            scores(first ? q_tile(n + 1) : do_tile(n + 1));
-            umma_commit(first ? &q_empty[(n + 1) % Q_STAGES] : &do_empty[(n + 1) % STAGES]);
+            scores(tmem_base + S_COL, k_lo, q_tile(n + 1));
+            umma_commit(s_full);
+          }
+          umma_commit(&do_empty[n % STAGES]);
+          ok = (!more || wait_do(n + 1)) && mbar_wait(ds_full, n & 1, abort_flag);
+          if (!ok) break;
+          tc_fence_after();
+          accumulate(tmem_base + DK_COL, tmem_base + DP_COL, q_tile(n), i == 0);
+          if (more) {
+            scores(tmem_base + DP_COL, v_lo, do_tile(n + 1));
+            umma_commit(dp_full);
             if (i + 2 == len) umma_commit(kv_empty);   // K and V are not read again: the next item's may come
           }
-          umma_commit(first ? &do_empty[n % STAGES] : &q_empty[n % Q_STAGES]);
+          umma_commit(&q_empty[n % Q_STAGES]);
         }
         if (ok) umma_commit(acc_full);
       }
@@ -361,7 +365,7 @@ window_bwd_dkdv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_con
   } else {
     // ------------------------------------------------------------------ arithmetic: lane = key, 32 query columns per thread
     const int qw = warp & 3;                        // TMEM lane quarter this warp may touch
-    const int grp = (warp - 3) >> 2;                // which 32 of the 128 queries
+    const int grp = (warp - 4) >> 2;                // which 32 of the 128 queries
     const int row = qw * 32 + lane;
     const uint32_t t_lane = static_cast<uint32_t>(qw * 32) << 16;
     const uint32_t t_s = tmem_base + S_COL + static_cast<uint32_t>(grp * 32) + t_lane;
@@ -534,9 +538,11 @@ __global__ void __launch_bounds__(256) window_bwd_join_kernel(const WindowBwdArg
 }
 
 // ---------------------------------------------------------------------------------------------- dQ
-// The items' key blocks form one stream; element g has its scores in TMEM buffer g & 1. One issuer goes S(g) | dP(g), the other
-// dQ(g) as soon as dS(g) is there; the arithmetic warps work on element g while S and dP of g + 1 are formed. dQ(g-1) frees the
-// buffer of S(g+1); dP has one buffer, free as soon as the arithmetic has it in registers.
+// The items' key blocks form one stream; element g has its scores in TMEM buffer g & 1. S, dP and dQ have an issuer each, which
+// issues as soon as its buffers allow it, so that nobody's wait (50 to 250 cycles even when satisfied) delays another's product;
+// the arithmetic warps work on element g while S and dP of g + 1 are formed. dQ(g-1) frees the buffer of S(g+1); dP has one
+// buffer, free as soon as the arithmetic has it in registers. With one issuer for the three an element took 3450 cycles, with two
+// 2470, of 1536 of UMMAs.
 template <int D>
 __global__ void __launch_bounds__(kWbThreads, 1)
 window_bwd_dq_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmDO,
@@ -553,7 +559,7 @@ window_bwd_dq_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
   uint8_t* sV = sK + K_STAGES * TILE_BYTES;         // V_STAGES
   uint64_t* bars = reinterpret_cast<uint64_t*>(sV + V_STAGES * TILE_BYTES);
   uint64_t* q_full = bars;            // 1
-  uint64_t* q_empty = bars + 1;       // 1
+  uint64_t* q_empty = bars + 1;       // 1 (two issuers: S, dP)
   uint64_t* k_full = bars + 2;        // K_STAGES
   uint64_t* k_empty = bars + 5;       // K_STAGES
   uint64_t* v_full = bars + 8;        // V_STAGES
@@ -577,7 +583,7 @@ window_bwd_dq_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
   }
   if (threadIdx.x == 0) {
     mbar_init(q_full, 1);
-    mbar_init(q_empty, 1);
+    mbar_init(q_empty, 2);
     for (int i = 0; i < K_STAGES; ++i) {
       mbar_init(&k_full[i], 1);
       mbar_init(&k_empty[i], 1);
@@ -671,8 +677,8 @@ window_bwd_dq_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
       ok = __shfl_sync(0xffffffffu, static_cast<int>(ok), 0) != 0;
       if (!ok) break;
     }
-  } else if (warp <= 2) {
-    // ------------------------------------------------------------------ UMMA issuers: warp 1 S and dP, warp 2 dQ
+  } else if (warp < 4) {
+    // ------------------------------------------------------------------ UMMA issuers: warp 1 S, warp 2 dP, warp 3 dQ
     const uint32_t idesc_s = make_idesc_bf16(kWinBlock, kWinBlock, 0, 0);   // [128 q, 128 keys]
     const uint32_t idesc_dq = make_idesc_bf16(kWinBlock, D, 0, 1);          // [128 q, D] = A(TMEM) x B(K tile, MN-major)
     constexpr uint32_t hi = smem_desc_hi_sw128(1024);
@@ -704,8 +710,12 @@ window_bwd_dq_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
             tc_fence_after();
             scores(tmem_base + static_cast<uint32_t>(g & 1) * 128u, q_lo, sK + ks * TILE_BYTES);
             umma_commit(&s_full[g & 1]);
-            ok = mbar_wait(&v_full[vs], (g / V_STAGES) & 1, abort_flag) && mbar_wait(dp_free, (g & 1) ^ 1, abort_flag);
+            if (j + 1 == n) umma_commit(q_empty);
+          } else if (warp == 2) {
+            ok = (j > 0 || mbar_wait(q_full, q_phase & 1, abort_flag)) && mbar_wait(&v_full[vs], (g / V_STAGES) & 1, abort_flag) &&
+                 mbar_wait(dp_free, (g & 1) ^ 1, abort_flag);
             if (!ok) break;
+            if (j == 0) ++q_phase;
             tc_fence_after();
             scores(tmem_base + DP_COL, do_lo, sV + vs * TILE_BYTES);
             umma_commit(dp_full);
@@ -734,7 +744,7 @@ window_bwd_dq_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
   } else {
     // ------------------------------------------------------------------ arithmetic: lane = query row, 32 key columns per thread
     const int qw = warp & 3;
-    const int grp = (warp - 3) >> 2;                // which 32 of the 128 keys
+    const int grp = (warp - 4) >> 2;                // which 32 of the 128 keys
     const int row = qw * 32 + lane;
     const uint32_t t_lane = static_cast<uint32_t>(qw * 32) << 16;
     const uint32_t t_dp = tmem_base + DP_COL + static_cast<uint32_t>(grp * 32) + t_lane;
