@@ -57,6 +57,42 @@ __device__ __forceinline__ float wb_exp2(float x) {
   return y;
 }
 
+// 2^x for a pair, x <= 120, on the multiply-add pipe: x = n + f with n the nearest integer (adding 1.5 * 2^23 leaves n in the low
+// bits), 2^f by a polynomial on [-1/2, 1/2], n added to the exponent. The coefficients are the minimax fit of degree 4 to the
+// relative error with p(0) = 1 (solved as a linear programme on a grid): 2.8e-6, far below the bf16 rounding that follows.
+// x below -127 gives exactly 0: there n = -127, f = 0, and the exponent of 1 becomes that of zero.
+__device__ __forceinline__ void wb_exp2_poly(uint64_t x, float& a, float& b) {
+  float lo, hi;
+  f32x2_split(x, lo, hi);
+  x = f32x2(fmaxf(lo, -127.f), fmaxf(hi, -127.f));
+  const uint64_t magic = f32x2(12582912.f, 12582912.f), minus_magic = f32x2(-12582912.f, -12582912.f), minus_one = f32x2(-1.f, -1.f);
+  const uint64_t t = add_f32x2(x, magic);
+  const uint64_t f = fma_f32x2(add_f32x2(t, minus_magic), minus_one, x);
+  uint64_t r = fma_f32x2(f32x2(0.009582576341927052f, 0.009582576341927052f), f, f32x2(0.05590682849287987f, 0.05590682849287987f));
+  r = fma_f32x2(r, f, f32x2(0.24024106562137604f, 0.24024106562137604f));
+  r = fma_f32x2(r, f, f32x2(0.6931241154670715f, 0.6931241154670715f));
+  r = fma_f32x2(r, f, f32x2(1.f, 1.f));
+  float ta, tb, ra, rb;
+  f32x2_split(t, ta, tb);
+  f32x2_split(r, ra, rb);
+  a = __uint_as_float(__float_as_uint(ra) + (__float_as_uint(ta) << 23));
+  b = __uint_as_float(__float_as_uint(rb) + (__float_as_uint(tb) << 23));
+}
+
+// Pair i of a thread's 16. Four warps share a scheduler here, and the special-function unit alone would take 1024 cycles a tile:
+// one pair in kWbPolyOf goes to the multiply-add pipe.
+constexpr int kWbPolyOf = 4;
+__device__ __forceinline__ uint32_t wb_exp2_pair(uint64_t x, int i) {
+  float a, b;
+  if (i % kWbPolyOf == 0) {
+    wb_exp2_poly(x, a, b);
+  } else {
+    f32x2_split(x, a, b);
+    a = wb_exp2(a), b = wb_exp2(b);
+  }
+  return pack_bf16x2(a, b);
+}
+
 // ---------------------------------------------------------------------------------------------- preparation
 constexpr int kWbPrepThreads = 1024;
 
@@ -160,14 +196,15 @@ __global__ void __launch_bounds__(kWbPrepThreads) window_bwd_prep_kernel(const W
 }
 
 // ---------------------------------------------------------------------------------------------- dK / dV
-// One iteration is 128 keys x 128 queries of one head; S^T and dP^T have one TMEM buffer each. The issuer goes
+// One iteration is 128 keys x 128 queries of one head; S^T and dP^T have one TMEM buffer each. The tensor cores go
 //     dV(i) | S(i+1) | dK(i) | dP(i+1)
 // and the arithmetic warps alternate between the exponentials of S(i+1) (under dK(i), dP(i+1)) and dS(i) (under dV(i), S(i+1)).
-// One thread issues all four: S(i+1) is what the arithmetic waits for, and with an issuer for each pair dK and dP share the tensor
-// cores with it (4100 cycles an iteration against 2048 of UMMAs). A wait that is satisfied already still costs 50 to 250
-// cycles, more the busier shared memory is, so tiles are waited for while the products before them run, and a third Q tile lets
-// its load start a whole iteration ahead. Blocks of 64 queries, which would leave room for two buffers, are bound by shared
-// memory: a UMMA with 64 columns reads its operands at 192 bytes a cycle, of 128 that there are.
+// S(i+1) is what the arithmetic waits for, so dK and dP are issued behind it: left to themselves they share the tensor cores
+// with it (4100 cycles an iteration, of 2048 of UMMAs). Each pair has an issuer of its own all the same, because a wait that is
+// satisfied already costs 50 to 250 cycles, more the busier shared memory is, and so one pair's waits run under the other's
+// products (3590 cycles with one issuer for all). A third Q tile lets its load start a whole iteration ahead. Blocks of 64
+// queries, which would leave room for two buffers, are bound by shared memory: a UMMA with 64 columns reads its operands at 192
+// bytes a cycle, of 128 that there are.
 template <int D>
 __global__ void __launch_bounds__(kWbThreads, 1)
 window_bwd_dkdv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmDO,
@@ -187,19 +224,20 @@ window_bwd_dkdv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_con
   uint8_t* sAux = sDO + STAGES * TILE_BYTES;        // STAGES x AUX_BYTES
   uint64_t* bars = reinterpret_cast<uint64_t*>(sAux + STAGES * AUX_BYTES);
   uint64_t* kv_full = bars;                 // 1
-  uint64_t* kv_empty = bars + 1;            // 1
+  uint64_t* kv_empty = bars + 1;            // 1 (both issuers)
   uint64_t* q_full = bars + 2;              // Q_STAGES
   uint64_t* q_empty = bars + 5;             // Q_STAGES
   uint64_t* do_full = bars + 8;             // STAGES
-  uint64_t* do_empty = bars + 10;           // STAGES
+  uint64_t* do_empty = bars + 10;           // STAGES (both issuers: dV, dP)
   uint64_t* aux_full = bars + 12;           // STAGES
   uint64_t* aux_empty = bars + 14;          // STAGES
   uint64_t* s_full = bars + 16;             // 1
   uint64_t* p_full = bars + 17;             // 1
   uint64_t* dp_full = bars + 18;            // 1
   uint64_t* ds_full = bars + 19;            // 1
-  uint64_t* acc_full = bars + 20;           // 1
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 21);
+  uint64_t* acc_full = bars + 20;           // 1 (both issuers)
+  uint64_t* s_issued = bars + 21;           // 2: S(i+1) is on its way, dK(i) may follow (two, so that none is lost)
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 23);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -212,14 +250,15 @@ window_bwd_dkdv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_con
   }
   if (threadIdx.x == 0) {
     mbar_init(kv_full, 1);
-    mbar_init(kv_empty, 1);
+    mbar_init(kv_empty, 2);
     for (int i = 0; i < Q_STAGES; ++i) {
       mbar_init(&q_full[i], 1);
       mbar_init(&q_empty[i], 1);
     }
     for (int i = 0; i < STAGES; ++i) {
       mbar_init(&do_full[i], 1);
-      mbar_init(&do_empty[i], 1);
+      mbar_init(&do_empty[i], 2);
+      mbar_init(&s_issued[i], 1);
       mbar_init(&aux_full[i], 1);
       mbar_init(&aux_empty[i], kWbArithWarps);
     }
@@ -227,7 +266,7 @@ window_bwd_dkdv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_con
     mbar_init(p_full, kWbArithWarps);
     mbar_init(dp_full, 1);
     mbar_init(ds_full, kWbArithWarps);
-    mbar_init(acc_full, 1);
+    mbar_init(acc_full, 2);
     abort_flag[0] = 0;
     abort_flag[1] = p.status[3];
     fence_barrier_init();
@@ -295,8 +334,8 @@ window_bwd_dkdv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_con
       if (!ok) break;
     }
   } else if (warp < 4) {
-    // ------------------------------------------------------------------ UMMA issuer (warp 1; 2 and 3 have nothing to do here)
-    if (warp == 1 && lane == 0) {
+    // ------------------------------------------------------------------ UMMA issuers: warp 1 dV and S, warp 2 dK and dP
+    if (warp < 3 && lane == 0) {
       const uint32_t idesc_s = make_idesc_bf16(kWinBlock, kWinBlock, 0, 0);   // [128 keys, 128 queries]
       const uint32_t idesc_acc = make_idesc_bf16(kWinBlock, D, 0, 1);         // [128 keys, D] = A(TMEM) x B(MN-major)
       constexpr uint32_t hi = smem_desc_hi_sw128(1024);
@@ -320,43 +359,55 @@ window_bwd_dkdv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_con
       auto wait_do = [&](int n) { return mbar_wait(&do_full[n % STAGES], (n / STAGES) & 1, abort_flag); };
       auto q_tile = [&](int n) { return sQ + (n % Q_STAGES) * TILE_BYTES; };
       auto do_tile = [&](int n) { return sDO + (n % STAGES) * TILE_BYTES; };
-      uint32_t kv_phase = 0;
+      uint32_t kv_phase = 0, turn[2] = {0, 0};      // turn: of s_issued, which the last iteration of an item does not use
       int n = 0;
       bool ok = true;
       for (int item = blockIdx.x; ok && item < items; item += gridDim.x) {
         const int4 e = entry[item / p.Hkv];
         const int len = e.z - e.y;
         if (len <= 0) continue;
-        ok = mbar_wait(kv_full, kv_phase & 1, abort_flag) && wait_q(n) && wait_do(n);
+        ok = mbar_wait(kv_full, kv_phase & 1, abort_flag) && (warp == 1 ? wait_q(n) : wait_do(n));
         ++kv_phase;
         if (!ok) break;
         tc_fence_after();
-        scores(tmem_base + S_COL, k_lo, q_tile(n));
-        umma_commit(s_full);
-        scores(tmem_base + DP_COL, v_lo, do_tile(n));
-        umma_commit(dp_full);
-        if (len == 1) umma_commit(kv_empty);
-        for (int i = 0; i < len; ++i, ++n) {
-          const bool more = i + 1 < len;
-          ok = (!more || wait_q(n + 1)) && mbar_wait(p_full, n & 1, abort_flag);
-          if (!ok) break;
-          tc_fence_after();
-          accumulate(tmem_base + DV_COL, tmem_base + S_COL, do_tile(n), i == 0);
-          if (more) {
-            scores(tmem_base + S_COL, k_lo, q_tile(n + 1));
-            umma_commit(s_full);
+        if (warp == 1) {
+          scores(tmem_base + S_COL, k_lo, q_tile(n));
+          umma_commit(s_full);
+          if (len == 1) umma_commit(kv_empty);
+          for (int i = 0; i < len; ++i, ++n) {
+            const bool more = i + 1 < len;
+            ok = (!more || wait_q(n + 1)) && wait_do(n) && mbar_wait(p_full, n & 1, abort_flag);
+            if (!ok) break;
+            tc_fence_after();
+            accumulate(tmem_base + DV_COL, tmem_base + S_COL, do_tile(n), i == 0);
+            if (more) {
+              scores(tmem_base + S_COL, k_lo, q_tile(n + 1));
+              mbar_arrive(&s_issued[n & 1]);
+              umma_commit(s_full);
+              if (i + 2 == len) umma_commit(kv_empty);   // K is not read again: the next item's may come
+            }
+            umma_commit(&do_empty[n % STAGES]);
           }
+        } else {
+          scores(tmem_base + DP_COL, v_lo, do_tile(n));
+          umma_commit(dp_full);
           umma_commit(&do_empty[n % STAGES]);
-          ok = (!more || wait_do(n + 1)) && mbar_wait(ds_full, n & 1, abort_flag);
-          if (!ok) break;
-          tc_fence_after();
-          accumulate(tmem_base + DK_COL, tmem_base + DP_COL, q_tile(n), i == 0);
-          if (more) {
-            scores(tmem_base + DP_COL, v_lo, do_tile(n + 1));
-            umma_commit(dp_full);
-            if (i + 2 == len) umma_commit(kv_empty);   // K and V are not read again: the next item's may come
+          if (len == 1) umma_commit(kv_empty);
+          for (int i = 0; i < len; ++i, ++n) {
+            const bool more = i + 1 < len;
+            ok = wait_q(n) && (!more || (wait_do(n + 1) && mbar_wait(&s_issued[n & 1], turn[n & 1]++ & 1, abort_flag))) &&
+                 mbar_wait(ds_full, n & 1, abort_flag);
+            if (!ok) break;
+            tc_fence_after();
+            accumulate(tmem_base + DK_COL, tmem_base + DP_COL, q_tile(n), i == 0);
+            if (more) {
+              scores(tmem_base + DP_COL, v_lo, do_tile(n + 1));
+              umma_commit(dp_full);
+              umma_commit(&do_empty[(n + 1) % STAGES]);
+              if (i + 2 == len) umma_commit(kv_empty);
+            }
+            umma_commit(&q_empty[n % Q_STAGES]);
           }
-          umma_commit(&q_empty[n % Q_STAGES]);
         }
         if (ok) umma_commit(acc_full);
       }
@@ -404,10 +455,8 @@ window_bwd_dkdv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_con
 #pragma unroll
           for (int i = 0; i < 8; ++i) {
             const float4 v = reinterpret_cast<const float4*>(aux)[i];
-            float a, b, c, d;
-            f32x2_split(fma_f32x2(f32x2(__uint_as_float(t[4 * i]), __uint_as_float(t[4 * i + 1])), scale2, f32x2(-v.x, -v.y)), a, b);
-            f32x2_split(fma_f32x2(f32x2(__uint_as_float(t[4 * i + 2]), __uint_as_float(t[4 * i + 3])), scale2, f32x2(-v.z, -v.w)), c, d);
-            wt[2 * i] = pack_bf16x2(wb_exp2(a), wb_exp2(b)), wt[2 * i + 1] = pack_bf16x2(wb_exp2(c), wb_exp2(d));
+            wt[2 * i] = wb_exp2_pair(fma_f32x2(f32x2(__uint_as_float(t[4 * i]), __uint_as_float(t[4 * i + 1])), scale2, f32x2(-v.x, -v.y)), 2 * i);
+            wt[2 * i + 1] = wb_exp2_pair(fma_f32x2(f32x2(__uint_as_float(t[4 * i + 2]), __uint_as_float(t[4 * i + 3])), scale2, f32x2(-v.z, -v.w)), 2 * i + 1);
           }
           if (!__all_sync(0xffffffffu, seen == 0xffffffffu)) {
 #pragma unroll
@@ -752,14 +801,21 @@ window_bwd_dq_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
     uint32_t dq_phase = 0;
     int g = 0;
     bool ok = true;
-    for (int item = blockIdx.x; item < items; item += gridDim.x) {
-      int batch, head, q0;
+    // what an item's rows need from memory, fetched while the item before is finished
+    int batch = 0, head = 0, q0 = 0;
+    WindowTile t{};
+    WindowRow w{};
+    float my_lse = 0.f, my_delta = 0.f;
+    auto fetch = [&](int item) {
       where(item, batch, head, q0);
-      const WindowTile t = window_tile(p.rule, batch, p.Sq, p.Sk, q0);
+      const long long stat = (static_cast<long long>(batch) * p.Hq + head) * p.Sq_pad + q0 + row;   // padded: always in range
+      my_lse = p.lse2[stat], my_delta = p.delta[stat];
+      t = window_tile(p.rule, batch, p.Sq, p.Sk, q0);
+      w = window_row(p.rule, batch, p.Sk, q0 + row + p.Sk - p.Sq, q0 + row < p.Sq);
+    };
+    if (static_cast<int>(blockIdx.x) < items) fetch(blockIdx.x);
+    for (int item = blockIdx.x; item < items; item += gridDim.x) {
       const int n = t.count(), qi = q0 + row;
-      const long long stat = (static_cast<long long>(batch) * p.Hq + head) * p.Sq_pad + qi;   // padded: always in range
-      const float my_lse = p.lse2[stat], my_delta = p.delta[stat];
-      const WindowRow w = window_row(p.rule, batch, p.Sk, qi + p.Sk - p.Sq, qi < p.Sq);
       // The forward's own rounded weights, so that the terms of dS cancel as exactly as there: weights relative to a whole power
       // of two (the forward's differ from it by another such factor), rounded to bf16, times what is left of 2^-lse2.
       const float shift = floorf(my_lse);
@@ -777,11 +833,8 @@ window_bwd_dq_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
         const int key0 = t.block(j) * kWinBlock;
         uint32_t wt[16];                            // rounded weights, two a register
 #pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          float a, b;
-          f32x2_split(fma_f32x2(f32x2(__uint_as_float(sc[2 * i]), __uint_as_float(sc[2 * i + 1])), scale2, shift2), a, b);
-          wt[i] = pack_bf16x2(wb_exp2(a), wb_exp2(b));
-        }
+        for (int i = 0; i < 16; ++i)
+          wt[i] = wb_exp2_pair(fma_f32x2(f32x2(__uint_as_float(sc[2 * i]), __uint_as_float(sc[2 * i + 1])), scale2, shift2), i);
         if (key0 < t.full_lo || key0 + kWinBlock - 1 > t.full_hi) {
           const uint32_t seen = window_bits(w, key0 + grp * 32);
           if (!__all_sync(0xffffffffu, seen == 0xffffffffu)) {
@@ -817,6 +870,9 @@ window_bwd_dq_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
         if (lane == 0) mbar_arrive(&ds_full[g & 1]);
       }
       if (!ok) break;
+      constexpr int QUART_D = D / 4;
+      __nv_bfloat16* dst = p.dq + ((static_cast<long long>(batch) * p.Sq + qi) * p.Hq + head) * D + grp * QUART_D;
+      if (item + static_cast<int>(gridDim.x) < items) fetch(item + gridDim.x);
       if (n > 0) {
         ok = mbar_wait(dq_full, dq_phase & 1, abort_flag);
         ok = __all_sync(0xffffffffu, ok);
@@ -824,8 +880,6 @@ window_bwd_dq_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
         ++dq_phase;
         tc_fence_after();
       }
-      constexpr int QUART_D = D / 4;
-      __nv_bfloat16* dst = p.dq + ((static_cast<long long>(batch) * p.Sq + qi) * p.Hq + head) * D + grp * QUART_D;
 #pragma unroll
       for (int c = 0; c < QUART_D; c += 16) {
         uint32_t r[16];
