@@ -77,8 +77,8 @@ __global__ void __launch_bounds__(kBnMaxThreads) block_norm_fwd_kernel(const Blo
     const int c = (threadIdx.x + j * blockDim.x) * kBnVec;
     a[j].zero(), b[j].zero();
     if (c < p.H) {
-      a[j].load(x + c);
-      b[j].load(res + c);
+      a[j].load_once(x + c);
+      b[j].load_once(res + c);
     }
   }
   float r1 = 1.f;
@@ -132,81 +132,111 @@ __global__ void __launch_bounds__(kBnMaxThreads) block_norm_fwd_kernel(const Blo
   }
 }
 
-// Rows blockIdx.x, + gridDim.x, ...; a thread keeps the column sums of its V vectors in registers.
-template <typename T, int V>
-__global__ void __launch_bounds__(kBnMaxThreads) block_norm_bwd_kernel(const BlockNormBwdArgs p) {
-  __shared__ float red[2][32][3];                  // two, so that one barrier a row is enough
-  const T *w1 = static_cast<const T*>(p.w1), *w2 = static_cast<const T*>(p.w2);
-  float s1[V][kBnVec], s2[V][kBnVec];
-#pragma unroll
-  for (int j = 0; j < V; ++j)
-#pragma unroll
-    for (int i = 0; i < kBnVec; ++i) s1[j][i] = s2[j][i] = 0.f;
-  int parity = 0;
-  for (long long row = blockIdx.x; row < p.rows; row += gridDim.x, parity ^= 1) {
+// What the backward reads of one row.
+template <typename T, int V, bool PRE, int GATE>
+struct BlockNormRow {
+  Vec<T, kBnVec> x[V], dh[V], h[PRE ? V : 1], dy[PRE ? V : 1], g[GATE == 2 ? V : 1];
+  float r1, r2;
+  __device__ __forceinline__ void load(const BlockNormBwdArgs& p, long long row) {
     const long long base = row * p.H;
-    const float r1 = w1 ? p.r1[row] : 1.f, r2 = w2 ? p.r2[row] : 0.f;
-    Vec<T, kBnVec> x[V], h[V], dy[V], dh[V], g[V];
+    r1 = p.w1 ? p.r1[row] : 1.f, r2 = PRE ? p.r2[row] : 0.f;
 #pragma unroll
     for (int j = 0; j < V; ++j) {
       const int c = (threadIdx.x + j * blockDim.x) * kBnVec;
-      const bool in = c < p.H;
-      x[j].zero(), h[j].zero(), dy[j].zero(), dh[j].zero(), g[j].zero();
-      if (in && p.x) x[j].load(static_cast<const T*>(p.x) + base + c);
-      if (in && w2) h[j].load(static_cast<const T*>(p.h) + base + c);
-      if (in && p.dy) dy[j].load(static_cast<const T*>(p.dy) + base + c);
-      if (in && p.dh) dh[j].load(static_cast<const T*>(p.dh) + base + c);
-      if (in && p.gate_mode) g[j].load(static_cast<const T*>(p.gate) + (p.gate_mode == 2 ? base : 0) + c);
-    }
-    float sums[3] = {0.f, 0.f, 0.f};               // dn2 * hn, e * (dh + r2 * dn2), e * r2 * hn
-#pragma unroll
-    for (int j = 0; j < V; ++j) {
-      const int c = (threadIdx.x + j * blockDim.x) * kBnVec;
+      x[j].zero(), dh[j].zero();
+      if (PRE) h[j].zero(), dy[j].zero();
+      if (GATE == 2) g[j].zero();
       if (c < p.H) {
-        Vec<T, kBnVec> v1, v2;
-        if (w1) v1.load(w1 + c);
-        if (w2) v2.load(w2 + c);
-#pragma unroll
-        for (int i = 0; i < kBnVec; ++i) {
-          const float hn = h[j].get(i) * r2, dn2 = w2 ? dy[j].get(i) * v2.get(i) : 0.f;
-          sums[0] += dn2 * hn;
-          if (w1) {
-            const float e = x[j].get(i) * r1 * v1.get(i) * p.scale * (p.gate_mode ? g[j].get(i) : 1.f);
-            sums[1] += e * (dh[j].get(i) + r2 * dn2);
-            sums[2] += e * r2 * hn;
-          }
-          s2[j][i] += dy[j].get(i) * hn;
-        }
+        if (p.x) x[j].load_once(static_cast<const T*>(p.x) + base + c);
+        if (p.dh) dh[j].load_once(static_cast<const T*>(p.dh) + base + c);
+        if (PRE) h[j].load_once(static_cast<const T*>(p.h) + base + c);
+        if (PRE && p.dy) dy[j].load_once(static_cast<const T*>(p.dy) + base + c);
+        if (GATE == 2) g[j].load_once(static_cast<const T*>(p.gate) + base + c);
       }
     }
-    if (w1 || w2) row_sums(sums, red[parity], blockDim.x);
-    const float inv = 1.f / static_cast<float>(p.H);
+  }
+};
+
+// Rows blockIdx.x, + gridDim.x, ...; a thread keeps the column sums of its V vectors and, one row ahead, its loads in registers.
+// Without the loads ahead the barrier in the middle of a row leaves memory idle: 8192 rows of 4096 in bf16 took 149 us.
+template <typename T, int V, bool PRE, int GATE>
+__global__ void __launch_bounds__(kBnMaxThreads, 1) block_norm_bwd_kernel(const BlockNormBwdArgs p) {
+  __shared__ float red[2][32][3];                  // two, so that one barrier a row is enough
+  const T *w1 = static_cast<const T*>(p.w1), *w2 = static_cast<const T*>(p.w2);
+  Vec<T, kBnVec> v1[V], v2[PRE ? V : 1], vg[GATE == 1 ? V : 1];
+  float s1[V][kBnVec], s2[PRE ? V : 1][kBnVec];
+#pragma unroll
+  for (int j = 0; j < V; ++j) {
+    const int c = (threadIdx.x + j * blockDim.x) * kBnVec;
+    if (c < p.H) {
+      if (w1) v1[j].load(w1 + c);
+      if (PRE) v2[j].load(w2 + c);
+      if (GATE == 1) vg[j].load(static_cast<const T*>(p.gate) + c);
+    }
+#pragma unroll
+    for (int i = 0; i < kBnVec; ++i) {
+      s1[j][i] = 0.f;
+      if (PRE) s2[j][i] = 0.f;
+    }
+  }
+  const float inv = 1.f / static_cast<float>(p.H);
+  int parity = 0;
+  BlockNormRow<T, V, PRE, GATE> cur, next;
+  if (static_cast<long long>(blockIdx.x) < p.rows) cur.load(p, blockIdx.x);
+  for (long long row = blockIdx.x; row < p.rows; row += gridDim.x, parity ^= 1) {
+    if (row + gridDim.x < p.rows) next.load(p, row + gridDim.x);
+    const float r1 = cur.r1, r2 = cur.r2;
+    float sums[3] = {0.f, 0.f, 0.f};               // dn2 * hn, e * (dh + r2 * dn2), e * r2 * hn
+    auto gate = [&](int j, int i) { return GATE == 1 ? vg[GATE == 1 ? j : 0].get(i) : GATE == 2 ? cur.g[GATE == 2 ? j : 0].get(i) : 1.f; };
+    if (PRE || w1) {
+#pragma unroll
+      for (int j = 0; j < V; ++j) {
+        const int c = (threadIdx.x + j * blockDim.x) * kBnVec;
+        if (c < p.H) {
+#pragma unroll
+          for (int i = 0; i < kBnVec; ++i) {
+            const float hn = PRE ? cur.h[PRE ? j : 0].get(i) * r2 : 0.f, dyi = PRE ? cur.dy[PRE ? j : 0].get(i) : 0.f;
+            const float dn2 = PRE ? dyi * v2[PRE ? j : 0].get(i) : 0.f;
+            if (PRE) {
+              sums[0] += dn2 * hn;
+              s2[PRE ? j : 0][i] += dyi * hn;
+            }
+            if (w1) {
+              const float e = cur.x[j].get(i) * r1 * v1[j].get(i) * p.scale * gate(j, i);
+              sums[1] += e * (cur.dh[j].get(i) + r2 * dn2);
+              if (PRE) sums[2] += e * r2 * hn;
+            }
+          }
+        }
+      }
+      row_sums(sums, red[parity], blockDim.x);
+    }
     const float c2 = sums[0] * inv, c1 = (sums[1] - c2 * sums[2]) * inv;
+    const long long base = row * p.H;
 #pragma unroll
     for (int j = 0; j < V; ++j) {
       const int c = (threadIdx.x + j * blockDim.x) * kBnVec;
       if (c < p.H) {
-        Vec<T, kBnVec> v1, v2, ox, or_, og;
-        if (w1) v1.load(w1 + c);
-        if (w2) v2.load(w2 + c);
+        Vec<T, kBnVec> ox, or_, og;
 #pragma unroll
         for (int i = 0; i < kBnVec; ++i) {
-          const float gi = p.gate_mode ? g[j].get(i) : 1.f;
-          float dt = dh[j].get(i);
-          if (w2) dt += r2 * (dy[j].get(i) * v2.get(i) - h[j].get(i) * r2 * c2);
-          const float sd = p.scale * dt, xn = x[j].get(i) * r1;
+          const float gi = gate(j, i);
+          float dt = cur.dh[j].get(i);
+          if (PRE) dt += r2 * (cur.dy[PRE ? j : 0].get(i) * v2[PRE ? j : 0].get(i) - cur.h[PRE ? j : 0].get(i) * r2 * c2);
+          const float sd = p.scale * dt, xn = cur.x[j].get(i) * r1;
           or_.set(i, dt);
-          og.set(i, sd * xn * (w1 ? v1.get(i) : 1.f));
-          s1[j][i] += sd * xn * (p.gate_mode == 2 ? gi : 1.f);
+          if (GATE == 2) og.set(i, sd * xn * (w1 ? v1[j].get(i) : 1.f));
+          s1[j][i] += sd * xn * (GATE == 2 ? gi : 1.f);
           float du = sd * gi;
-          if (w1) du = r1 * (du * v1.get(i) - xn * c1);
+          if (w1) du = r1 * (du * v1[j].get(i) - xn * c1);
           ox.set(i, du);
         }
         or_.store(static_cast<T*>(p.dres) + base + c);
         ox.store(static_cast<T*>(p.dx) + base + c);
-        if (p.gate_mode == 2) og.store(static_cast<T*>(p.dgate) + base + c);
+        if (GATE == 2) og.store(static_cast<T*>(p.dgate) + base + c);
       }
     }
+    cur = next;
   }
 #pragma unroll
   for (int j = 0; j < V; ++j) {
@@ -214,36 +244,43 @@ __global__ void __launch_bounds__(kBnMaxThreads) block_norm_bwd_kernel(const Blo
     if (c < p.H) {
       const long long at = static_cast<long long>(blockIdx.x) * p.H + c;
 #pragma unroll
-      for (int i = 0; i < kBnVec; ++i) {
-        if (p.part1) p.part1[at + i] = s1[j][i];
-        if (p.part2) p.part2[at + i] = s2[j][i];
+      for (int i = 0; i < kBnVec; i += 4) {
+        if (p.part1) *reinterpret_cast<float4*>(p.part1 + at + i) = make_float4(s1[j][i], s1[j][i + 1], s1[j][i + 2], s1[j][i + 3]);
+        if (PRE) *reinterpret_cast<float4*>(p.part2 + at + i) = make_float4(s2[PRE ? j : 0][i], s2[PRE ? j : 0][i + 1], s2[PRE ? j : 0][i + 2], s2[PRE ? j : 0][i + 3]);
       }
     }
   }
 }
 
 // dw1 = gate_c * S1, dgate = w1 * S1, dw2 = S2 (S: sums of the CTAs' column sums, in their order). 32 columns a block, the
-// partial rows divided over 8 warps.
+// partial rows divided over 16 warps.
+constexpr int kBnColWarps = 16;
 template <typename T>
-__global__ void __launch_bounds__(256) block_norm_columns_kernel(const float* __restrict__ part1, const float* __restrict__ part2, int parts,
-                                                                 int H, const T* __restrict__ w1, const T* __restrict__ gate, T* __restrict__ dw1,
-                                                                 T* __restrict__ dgate, T* __restrict__ dw2) {
-  __shared__ float red[2][8][33];
+__global__ void __launch_bounds__(32 * kBnColWarps) block_norm_columns_kernel(const float* __restrict__ part1, const float* __restrict__ part2,
+                                                                              int parts, int H, const T* __restrict__ w1,
+                                                                              const T* __restrict__ gate, T* __restrict__ dw1,
+                                                                              T* __restrict__ dgate, T* __restrict__ dw2) {
+  __shared__ float red[kBnColWarps][33];
   const int c = blockIdx.x * 32 + threadIdx.x;
-  float a = 0.f, b = 0.f;
-  if (c < H)
-    for (int r = threadIdx.y; r < parts; r += 8) {
-      if (part1) a += part1[static_cast<long long>(r) * H + c];
-      if (part2) b += part2[static_cast<long long>(r) * H + c];
-    }
-  red[0][threadIdx.y][threadIdx.x] = a, red[1][threadIdx.y][threadIdx.x] = b;
+  const float* part = blockIdx.y ? part2 : part1;
+  float a = 0.f;
+  if (c < H) {
+    part += c;
+#pragma unroll 10
+    for (int r = threadIdx.y; r < parts; r += kBnColWarps) a += part[static_cast<long long>(r) * H];
+  }
+  red[threadIdx.y][threadIdx.x] = a;
   __syncthreads();
   if (threadIdx.y != 0 || c >= H) return;
-  a = b = 0.f;
-  for (int r = 0; r < 8; ++r) a += red[0][r][threadIdx.x], b += red[1][r][threadIdx.x];
+  a = 0.f;
+#pragma unroll
+  for (int r = 0; r < kBnColWarps; ++r) a += red[r][threadIdx.x];
+  if (blockIdx.y) {
+    dw2[c] = from_float<T>(a);
+    return;
+  }
   if (dw1) dw1[c] = from_float<T>(gate ? a * to_float(gate[c]) : a);
   if (dgate) dgate[c] = from_float<T>(w1 ? a * to_float(w1[c]) : a);
-  if (dw2) dw2[c] = from_float<T>(b);
 }
 
 // Threads of a row for V vectors each: whole warps that cover the row.
@@ -251,7 +288,7 @@ static int bn_threads(int H, int V) { return ((H / kBnVec + V - 1) / V + 31) / 3
 
 template <typename T>
 static int launch_block_norm_fwd(const BlockNormFwdArgs& a, cudaStream_t stream) {
-  const int V = a.H <= 128 * kBnVec ? 1 : a.H <= 512 * kBnVec ? 2 : 4;
+  const int V = a.H <= 128 * kBnVec ? 1 : a.H <= 1024 * kBnVec ? 2 : 4;
   const int x = bn_threads(a.H, V), y = x == 32 ? 4 : 1;
   const long long grid = (a.rows + y - 1) / y;
   const dim3 block(x, y);
@@ -263,24 +300,41 @@ static int launch_block_norm_fwd(const BlockNormFwdArgs& a, cudaStream_t stream)
   return 0;
 }
 
-static int bn_bwd_ctas(long long rows) {
-  const long long n = 2ll * sm_count();
+static int bn_bwd_vectors(int H) { return H <= 512 * kBnVec ? 1 : H <= 1024 * kBnVec ? 2 : 4; }
+
+// CTAs of the backward, each of which leaves a row of column sums: as many as fit the SMs at once, by their threads.
+static int bn_bwd_ctas(long long rows, int H) {
+  const int x = bn_threads(H, bn_bwd_vectors(H));
+  const long long n = static_cast<long long>(sm_count()) * (x > 256 ? 1 : x > 128 ? 2 : 4);
   return static_cast<int>(rows < n ? rows : n);
+}
+
+template <typename T, int V, bool PRE>
+static void bn_bwd_gate(const BlockNormBwdArgs& a, int ctas, int x, cudaStream_t stream) {
+  if (a.gate_mode == 0) block_norm_bwd_kernel<T, V, PRE, 0><<<ctas, x, 0, stream>>>(a);
+  else if (a.gate_mode == 1) block_norm_bwd_kernel<T, V, PRE, 1><<<ctas, x, 0, stream>>>(a);
+  else block_norm_bwd_kernel<T, V, PRE, 2><<<ctas, x, 0, stream>>>(a);
 }
 
 template <typename T>
 static int launch_block_norm_bwd(const BlockNormBwdArgs& a, void* dw1, void* dgate, void* dw2, cudaStream_t stream) {
-  const int V = a.H <= 512 * kBnVec ? 1 : a.H <= 1024 * kBnVec ? 2 : 4;
-  const int ctas = bn_bwd_ctas(a.rows), x = bn_threads(a.H, V);
-  if (V == 1) block_norm_bwd_kernel<T, 1><<<ctas, x, 0, stream>>>(a);
-  else if (V == 2) block_norm_bwd_kernel<T, 2><<<ctas, x, 0, stream>>>(a);
-  else block_norm_bwd_kernel<T, 4><<<ctas, x, 0, stream>>>(a);
+  const int V = bn_bwd_vectors(a.H), ctas = bn_bwd_ctas(a.rows, a.H), x = bn_threads(a.H, V);
+  if (a.w2) {
+    if (V == 1) bn_bwd_gate<T, 1, true>(a, ctas, x, stream);
+    else if (V == 2) bn_bwd_gate<T, 2, true>(a, ctas, x, stream);
+    else bn_bwd_gate<T, 4, true>(a, ctas, x, stream);
+  } else {
+    if (V == 1) bn_bwd_gate<T, 1, false>(a, ctas, x, stream);
+    else if (V == 2) bn_bwd_gate<T, 2, false>(a, ctas, x, stream);
+    else bn_bwd_gate<T, 4, false>(a, ctas, x, stream);
+  }
   count_launch();
   MB_CHECK_CUDA(cudaGetLastError());
   if (a.part1 || a.part2) {
-    block_norm_columns_kernel<T><<<(a.H + 31) / 32, dim3(32, 8), 0, stream>>>(
-        a.part1, a.part2, ctas, a.H, static_cast<const T*>(a.w1), a.gate_mode == 1 ? static_cast<const T*>(a.gate) : nullptr,
-        static_cast<T*>(dw1), static_cast<T*>(dgate), static_cast<T*>(dw2));
+    // part1 in the grid's first row, part2 in its second; without part1 the first row has nothing to write
+    block_norm_columns_kernel<T><<<dim3((a.H + 31) / 32, a.part2 ? 2 : 1), dim3(32, kBnColWarps), 0, stream>>>(
+        a.part1 ? a.part1 : a.part2, a.part2, ctas, a.H, static_cast<const T*>(a.w1),
+        a.gate_mode == 1 ? static_cast<const T*>(a.gate) : nullptr, static_cast<T*>(dw1), static_cast<T*>(dgate), static_cast<T*>(dw2));
     count_launch();
     MB_CHECK_CUDA(cudaGetLastError());
   }
@@ -318,7 +372,9 @@ MB_API int mb_block_norm_fwd(const void* x, const void* residual, const void* w1
 }
 
 // Rows of fp32 column sums that the backward needs as scratch (H floats each, for each of the two sums that are asked for).
-MB_API int mb_block_norm_bwd_parts(long long rows) { return mb::bn_bwd_ctas(rows); }
+MB_API int mb_block_norm_bwd_parts(long long rows, int H) {
+  return H < mb::kBnVec || H > mb::kBnMaxH ? 0 : mb::bn_bwd_ctas(rows, H);
+}
 
 // Gradients of mb_block_norm_fwd. dy / dh null: that output has no gradient. dgate: [H] or [rows, H] by gate_mode. part1 goes with
 // dw1 or a [H] dgate, part2 with dw2; x null where neither w1 nor a gate needs it.
@@ -326,8 +382,8 @@ MB_API int mb_block_norm_bwd(const void* dy, const void* dh, const void* x, cons
                              int gate_mode, const float* r1, const float* r2, void* dx, void* dresidual, void* dw1, void* dw2, void* dgate,
                              float* part1, float* part2, int dtype, long long rows, int H, float scale, cudaStream_t stream) {
   using namespace mb;
-  const void* pointers[] = {dy, dh, x, h, w1, w2, gate, dx, dresidual, dgate};
-  const char* what = block_norm_problem(dtype, rows, H, gate_mode, gate, pointers, 10);
+  const void* pointers[] = {dy, dh, x, h, w1, w2, gate, dx, dresidual, dgate, part1, part2};
+  const char* what = block_norm_problem(dtype, rows, H, gate_mode, gate, pointers, 12);
   if (!what && ((w1 && (!r1 || !x || !dw1)) || (w2 && (!r2 || !h || !dw2 || !part2)) || (gate && (!x || !dgate)) || !dx || !dresidual ||
                 ((w1 || gate_mode == 1) && !part1)))
     what = "mb_block_norm_bwd: a tensor that these arguments need is missing";

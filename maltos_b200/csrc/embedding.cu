@@ -232,14 +232,23 @@ __global__ void __launch_bounds__(kEmbThreads) embedding_join_kernel(const int* 
   const int r = key[next - 1];
   if (r == rows || key[next] != r) return;                                  // nothing crosses
   if (key[first] == r && first > 0 && key[first - 1] == r) return;          // it began earlier: that chunk's CTA adds it up
+  // the chunks that the run goes on in: sorted, so the number of chunks that begin with r; looked for by the whole block at once
+  int more = 0;
+  for (int base = 0;; base += kEmbThreads) {
+    const long long at = next + static_cast<long long>(base + threadIdx.x) * kEmbChunk;
+    const int hit = __syncthreads_count(at < tokens && key[at] == r);
+    more += hit;
+    if (hit < kEmbThreads) break;
+  }
   const int c = (blockIdx.y * kEmbThreads + threadIdx.x) * N;
   if (c >= H) return;
   float acc[N];
 #pragma unroll
   for (int k = 0; k < N; ++k) acc[k] = tail[static_cast<long long>(chunk) * H + c + k];
-  for (long long at = next; at < tokens && key[at] == r; at += kEmbChunk)
+#pragma unroll 8
+  for (int i = 1; i <= more; ++i)
 #pragma unroll
-    for (int k = 0; k < N; ++k) acc[k] += head[at / kEmbChunk * H + c + k];
+    for (int k = 0; k < N; ++k) acc[k] += head[static_cast<long long>(chunk + i) * H + c + k];
   Vec<T, N> o;
 #pragma unroll
   for (int k = 0; k < N; ++k) o.set(k, acc[k] * scale);

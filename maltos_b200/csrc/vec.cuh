@@ -36,6 +36,18 @@ struct Vec {
       for (int i = 0; i < kPieces; ++i) piece[i] = __ldg(reinterpret_cast<const uint4*>(p) + i);
     }
   }
+  // for data that is read once: leaves L1 to what is read again
+  __device__ __forceinline__ void load_once(const T* p) {
+    if constexpr (N == 1) {
+      at[0] = *p;
+    } else {
+#pragma unroll
+      for (int i = 0; i < kPieces; ++i)
+        asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];"
+                     : "=r"(piece[i].x), "=r"(piece[i].y), "=r"(piece[i].z), "=r"(piece[i].w)
+                     : "l"(reinterpret_cast<const uint4*>(p) + i));
+    }
+  }
   __device__ __forceinline__ void store(T* p) const {
     if constexpr (N == 1) {
       *p = at[0];
