@@ -18,6 +18,8 @@ namespace mb {
 constexpr int kEmbThreads = 256;
 constexpr int kSortCtas = 8, kSortThreads = 1024, kSortWarps = kSortThreads / 32, kSortBins = 256;
 constexpr int kEmbChunk = 32;
+constexpr int kZeroVecs = 8 * kSortThreads;   // 32-byte pieces that a CTA writes: short pieces, since clusters leave some SMs out at first
+constexpr int kEmbJoinThreads = 64;   // narrow blocks: a frequent token's parts are added by several SMs
 
 template <typename I>
 __device__ __forceinline__ long long emb_row(const I* ids, long long t, long long rows) {
@@ -62,9 +64,9 @@ struct EmbSortArgs {
   int tokens, rows;   // rows: also the key of tokens that get no gradient (outside the table, or padding_idx)
   int pad;            // padding_idx, or -1
   int passes, bits;
-  uint4* zero;        // dweight
+  uint8_t* zero;      // dweight
   long long zero_vecs;
-  int zero_tail;      // bytes behind the last whole 16
+  int zero_tail;      // bytes behind the last whole 32
 };
 
 // shared memory of another CTA of the cluster
@@ -77,21 +79,28 @@ __device__ __forceinline__ int ld_cluster_s32(uint32_t addr) {
 template <typename I>
 __global__ void __cluster_dims__(kSortCtas, 1, 1) __launch_bounds__(kSortThreads) embedding_sort_kernel(const EmbSortArgs p) {
   if (blockIdx.x >= kSortCtas) {
-    const long long n = static_cast<long long>(gridDim.x - kSortCtas) * kSortThreads;
-    const long long me = static_cast<long long>(blockIdx.x - kSortCtas) * kSortThreads + threadIdx.x;
-    for (long long i = me; i < p.zero_vecs; i += n) p.zero[i] = make_uint4(0u, 0u, 0u, 0u);
-    if (me < p.zero_tail) reinterpret_cast<uint8_t*>(p.zero + p.zero_vecs)[me] = 0;
+    const uint32_t none[8] = {0u, 0u, 0u, 0u, 0u, 0u, 0u, 0u};
+    const long long first = static_cast<long long>(blockIdx.x - kSortCtas) * kZeroVecs;
+#pragma unroll
+    for (int i = 0; i < kZeroVecs; i += kSortThreads) {
+      const long long at = first + i + threadIdx.x;
+      if (at < p.zero_vecs) store_32_bytes(p.zero + 32 * at, none);
+    }
+    if (first == 0 && static_cast<int>(threadIdx.x) < p.zero_tail) p.zero[32 * p.zero_vecs + threadIdx.x] = 0;
     return;
   }
   __shared__ int hist[kSortWarps][kSortBins];   // per warp: counts, then where the warp's next element of a digit goes
   __shared__ int total[kSortBins];              // of this CTA, read by the others
-  __shared__ int scan[kSortBins];
+  __shared__ int scan[kSortBins / 32];
   const int cta = blockIdx.x, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const I* ids = static_cast<const I*>(p.ids);
-  // a warp owns a contiguous piece, a multiple of 32 elements long: the order of elements is (CTA, warp, step, lane)
-  const int per = ((p.tokens + kSortCtas * kSortWarps - 1) / (kSortCtas * kSortWarps) + 31) / 32 * 32;
-  const long long begin = static_cast<long long>(cta * kSortWarps + warp) * per;
-  const int a = static_cast<int>(begin < p.tokens ? begin : p.tokens), b = static_cast<int>(begin + per < p.tokens ? begin + per : p.tokens);
+  // A CTA owns a contiguous piece, a warp a contiguous part of it, multiples of 32 long: elements are in the order of (CTA, warp,
+  // step, lane). Few tokens are few warps' work, since the counts of all warps are added up one after the other.
+  const long long cta_per = (static_cast<long long>(p.tokens + kSortCtas - 1) / kSortCtas + 31) / 32 * 32;
+  const int warps = static_cast<int>(cta_per / 32 < kSortWarps ? cta_per / 32 : kSortWarps);
+  const long long per = (cta_per / 32 + warps - 1) / warps * 32;
+  const long long cta_end = min((cta + 1) * cta_per, static_cast<long long>(p.tokens));
+  const int a = static_cast<int>(min(cta * cta_per + warp * per, cta_end)), b = warp < warps ? static_cast<int>(min(a + per, cta_end)) : a;
   const int bins = 1 << p.bits;
   for (int pass = 0; pass < p.passes; ++pass) {
     const int shift = pass * p.bits;
@@ -115,9 +124,9 @@ __global__ void __cluster_dims__(kSortCtas, 1, 1) __launch_bounds__(kSortThreads
       __syncwarp();
     }
     __syncthreads();
+    int sum = 0;                                // of digit `tid` in this CTA
     if (tid < bins) {
-      int sum = 0;
-      for (int w = 0; w < kSortWarps; ++w) {
+      for (int w = 0; w < warps; ++w) {
         const int n = hist[w][tid];
         hist[w][tid] = sum;
         sum += n;
@@ -127,24 +136,26 @@ __global__ void __cluster_dims__(kSortCtas, 1, 1) __launch_bounds__(kSortThreads
     cluster_arrive();
     cluster_wait();
     int before = 0, all = 0;                    // this digit in earlier CTAs, and everywhere
-    if (tid < bins) {
+    if (tid < bins)
+#pragma unroll
       for (int c = 0; c < kSortCtas; ++c) {
         const int n = ld_cluster_s32(mapa_u32(&total[tid], c));
         all += n;
         if (c < cta) before += n;
       }
-      scan[tid] = all;
+    // digits in order: a scan of each warp's 32, then of the warps
+    int inc = all;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int n = __shfl_up_sync(0xffffffffu, inc, o);
+      if (lane >= o) inc += n;
     }
+    if (lane == 31 && warp < kSortBins / 32) scan[warp] = inc;
     __syncthreads();
-    for (int o = 1; o < bins; o <<= 1) {
-      const int n = tid < bins && tid >= o ? scan[tid - o] : 0;
-      __syncthreads();
-      if (tid < bins) scan[tid] += n;
-      __syncthreads();
-    }
     if (tid < bins) {
-      const int base = scan[tid] - all + before;
-      for (int w = 0; w < kSortWarps; ++w) hist[w][tid] += base;
+      int base = inc - all + before;
+      for (int w = 0; w < warp; ++w) base += scan[w];
+      for (int w = 0; w < warps; ++w) hist[w][tid] += base;
     }
     __syncthreads();
     for (int i0 = a; i0 < b; i0 += 32) {
@@ -168,6 +179,31 @@ __global__ void __cluster_dims__(kSortCtas, 1, 1) __launch_bounds__(kSortThreads
 }
 
 // ---------------------------------------------------------------------------------------------- runs
+// N consecutive fp32 values, 16 bytes at a time where they fill that.
+template <int N>
+__device__ __forceinline__ void add_row(float (&acc)[N], const float* p) {
+  if constexpr (N % 4 == 0) {
+#pragma unroll
+    for (int k = 0; k < N; k += 4) {
+      const float4 v = *reinterpret_cast<const float4*>(p + k);
+      acc[k] += v.x, acc[k + 1] += v.y, acc[k + 2] += v.z, acc[k + 3] += v.w;
+    }
+  } else {
+#pragma unroll
+    for (int k = 0; k < N; ++k) acc[k] += p[k];
+  }
+}
+template <int N>
+__device__ __forceinline__ void put_row(float* p, const float (&acc)[N]) {
+  if constexpr (N % 4 == 0) {
+#pragma unroll
+    for (int k = 0; k < N; k += 4) *reinterpret_cast<float4*>(p + k) = make_float4(acc[k], acc[k + 1], acc[k + 2], acc[k + 3]);
+  } else {
+#pragma unroll
+    for (int k = 0; k < N; ++k) p[k] = acc[k];
+  }
+}
+
 template <typename T, int N>
 __global__ void __launch_bounds__(kEmbThreads) embedding_chunk_kernel(const int* __restrict__ key, const int* __restrict__ pos,
                                                                       const T* __restrict__ dout, T* __restrict__ dweight,
@@ -210,9 +246,7 @@ __global__ void __launch_bounds__(kEmbThreads) embedding_chunk_kernel(const int*
         for (int k = 0; k < N; ++k) o.set(k, acc[k] * scale);
         o.store(dweight + static_cast<long long>(r) * H + c);
       } else {                                     // `head` where the run came in from the left, `tail` where it began here
-        float* part = (from_left ? head : tail) + static_cast<long long>(blockIdx.x) * H + c;
-#pragma unroll
-        for (int k = 0; k < N; ++k) part[k] = acc[k];
+        put_row(((from_left ? head : tail) + static_cast<long long>(blockIdx.x) * H + c), acc);
       }
       from_left = false;
 #pragma unroll
@@ -223,7 +257,7 @@ __global__ void __launch_bounds__(kEmbThreads) embedding_chunk_kernel(const int*
 
 // One CTA per chunk in which a run begins that crosses the chunk's right border.
 template <typename T, int N>
-__global__ void __launch_bounds__(kEmbThreads) embedding_join_kernel(const int* __restrict__ key, T* __restrict__ dweight,
+__global__ void __launch_bounds__(kEmbJoinThreads) embedding_join_kernel(const int* __restrict__ key, T* __restrict__ dweight,
                                                                      const float* __restrict__ head, const float* __restrict__ tail,
                                                                      int tokens, int H, int rows, float scale) {
   const int chunk = blockIdx.x;
@@ -234,21 +268,20 @@ __global__ void __launch_bounds__(kEmbThreads) embedding_join_kernel(const int* 
   if (key[first] == r && first > 0 && key[first - 1] == r) return;          // it began earlier: that chunk's CTA adds it up
   // the chunks that the run goes on in: sorted, so the number of chunks that begin with r; looked for by the whole block at once
   int more = 0;
-  for (int base = 0;; base += kEmbThreads) {
+  for (int base = 0;; base += kEmbJoinThreads) {
     const long long at = next + static_cast<long long>(base + threadIdx.x) * kEmbChunk;
     const int hit = __syncthreads_count(at < tokens && key[at] == r);
     more += hit;
-    if (hit < kEmbThreads) break;
+    if (hit < kEmbJoinThreads) break;
   }
-  const int c = (blockIdx.y * kEmbThreads + threadIdx.x) * N;
+  const int c = (blockIdx.y * kEmbJoinThreads + threadIdx.x) * N;
   if (c >= H) return;
   float acc[N];
 #pragma unroll
-  for (int k = 0; k < N; ++k) acc[k] = tail[static_cast<long long>(chunk) * H + c + k];
+  for (int k = 0; k < N; ++k) acc[k] = 0.f;
+  add_row(acc, tail + static_cast<long long>(chunk) * H + c);
 #pragma unroll 8
-  for (int i = 1; i <= more; ++i)
-#pragma unroll
-    for (int k = 0; k < N; ++k) acc[k] += head[static_cast<long long>(chunk + i) * H + c + k];
+  for (int i = 1; i <= more; ++i) add_row(acc, head + static_cast<long long>(chunk + i) * H + c);
   Vec<T, N> o;
 #pragma unroll
   for (int k = 0; k < N; ++k) o.set(k, acc[k] * scale);
@@ -277,7 +310,7 @@ static int launch_embedding_runs(const EmbSortArgs& s, const void* dout, void* d
   const dim3 grid(chunks, (H / N + kEmbThreads - 1) / kEmbThreads);
   embedding_chunk_kernel<T, N><<<grid, kEmbThreads, 0, stream>>>(key, pos, static_cast<const T*>(dout), static_cast<T*>(dweight), parts,
                                                                tail, s.tokens, H, s.rows, scale);
-  embedding_join_kernel<T, N><<<grid, kEmbThreads, 0, stream>>>(key, static_cast<T*>(dweight), parts, tail, s.tokens, H, s.rows, scale);
+  embedding_join_kernel<T, N><<<dim3(chunks, (H / N + kEmbJoinThreads - 1) / kEmbJoinThreads), kEmbJoinThreads, 0, stream>>>(key, static_cast<T*>(dweight), parts, tail, s.tokens, H, s.rows, scale);
   count_launch(2);
   MB_CHECK_CUDA(cudaGetLastError());
   return 0;
@@ -326,8 +359,8 @@ MB_API int mb_embedding_bwd(const void* ids, int wide, const void* dout, void* d
     set_last_error(what);
     return -1;
   }
-  if ((reinterpret_cast<uintptr_t>(dweight) | reinterpret_cast<uintptr_t>(scratch)) & 15) {
-    set_last_error("mb_embedding_bwd: dweight and scratch must be 16-byte aligned");
+  if ((reinterpret_cast<uintptr_t>(dweight) | reinterpret_cast<uintptr_t>(scratch)) & 31) {
+    set_last_error("mb_embedding_bwd: dweight and scratch must be 32-byte aligned");
     return -3;
   }
   EmbSortArgs s;
@@ -340,12 +373,13 @@ MB_API int mb_embedding_bwd(const void* ids, int wide, const void* dout, void* d
   s.passes = (width + 7) / 8;
   s.bits = (width + s.passes - 1) / s.passes;
   const long long bytes = rows * H * (dtype == 2 ? 4 : 2);
-  s.zero = static_cast<uint4*>(dweight);
-  s.zero_vecs = bytes / 16, s.zero_tail = static_cast<int>(bytes % 16);
-  long long fill = (bytes / 16 + kSortThreads * 8 - 1) / (kSortThreads * 8);
-  const long long cap = 2ll * sm_count() - kSortCtas;
-  if (fill > cap) fill = cap;
-  if (fill < 1) fill = 1;
+  s.zero = static_cast<uint8_t*>(dweight);
+  s.zero_vecs = bytes / 32, s.zero_tail = static_cast<int>(bytes % 32);
+  const long long fill = bytes / 32 / kZeroVecs + 1;
+  if (fill >= (1ll << 31) - 65536) {
+    set_last_error("mb_embedding_bwd: the table is too large");
+    return -1;
+  }
   const unsigned grid = static_cast<unsigned>(kSortCtas + (fill + kSortCtas - 1) / kSortCtas * kSortCtas);
   if (wide) embedding_sort_kernel<long long><<<grid, kSortThreads, 0, stream>>>(s);
   else embedding_sort_kernel<int><<<grid, kSortThreads, 0, stream>>>(s);

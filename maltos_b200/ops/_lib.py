@@ -106,6 +106,7 @@ class _RangedLibrary:
 _PROTOTYPES = {
     "mb_document_bounds": "pippiip",
     "mb_window_attn_fwd": "pllpllpll" "ppppp" "iiiiiiii" "fp",
+    "mb_window_attn_token": "pllpllpll" "ppp" "iiiiiiii" "fp",
     "mb_window_attn_bwd_scratch_words": "iiiiiiiii",
     "mb_window_attn_bwd": "pllpllpll" "pppll" "pppp" "ppp" "iiiiiiii" "fp",
     "mb_embedding_fwd": "pippilil" "fp",

@@ -12,6 +12,15 @@ from maltos_b200.utils.activation_checkpoint import current_checkpoint_stash
 from . import _lib
 
 
+def _few_queries(B: int, Hkv: int, rows: int) -> bool:
+    """Whether a forward without gradients takes ``csrc/window_token.cu``: ``rows`` (queries x heads of a group) of each key/value
+    head in groups of 8, K and V read once a group. Up to one group it always wins (8 rows of 2048 visible keys, 8 key/value
+    heads: 20 us against 48 us in tiles of 128 rows); up to four while the groups fit the SMs (4 groups x 16 heads: 20 against
+    92 us, 2 x 64: 40 against 48 us; 4 x 64 lose, 76 against 48 us)."""
+    groups = -(-rows // 8)
+    return groups == 1 or (groups <= 4 and B * Hkv * groups <= 148)
+
+
 def _addressable(t: torch.Tensor) -> tuple[torch.Tensor, int, int]:
     """``[B, S, h, D]`` as the kernels address it (heads contiguous inside a token, 16-byte aligned, token and batch strides
     positive multiples of 8 elements), with the token and the batch stride; copied only where its strides do not fit."""
@@ -48,6 +57,13 @@ def window_forward(q, k, v, *, window: int, sinks: int, starts, scale: float, ke
     k, k_t, k_b = _addressable(k)
     v, v_t, v_b = _addressable(v)
     out = torch.empty((B, Sq, Hq, D), dtype=torch.bfloat16, device=q.device)
+    if not keep and _few_queries(B, Hkv, Sq * (Hq // Hkv)):
+        lse = torch.empty((B, Hq, Sq), dtype=torch.float32, device=q.device) if want_lse else None
+        with _lib.on_device_of(q):
+            _lib.check(_lib.lib().mb_window_attn_token(q.data_ptr(), q_t, q_b, k.data_ptr(), k_t, k_b, v.data_ptr(), v_t, v_b, out.data_ptr(),
+                                                       _lib.address(lse), _lib.address(starts), B, Sq, Sk, Hq, Hkv, D, window, sinks, scale,
+                                                       _lib.stream_of(q)), "mb_window_attn_token")
+        return out, None, None, lse
     out_lo = torch.empty_like(out) if keep else None
     lse2 = torch.empty((B, Hq, Sq), dtype=torch.float32, device=q.device) if keep else None
     lse = torch.empty((B, Hq, Sq), dtype=torch.float32, device=q.device) if want_lse else None

@@ -235,3 +235,25 @@ def test_other_types_and_head_sizes_run_the_restatement():
         (value, _), *_ = _expect(q, k, v, torch.zeros_like(q), 20, 2, None, 1 / math.sqrt(D))
         eps = torch.finfo(dtype).eps
         assert out.dtype == dtype and (out.double() - value).abs().max() <= (eps / 2 + 2e-6) * 4 + 1e-5
+
+
+@pytest.mark.parametrize("Sq,Sk,Hq,Hkv,D,window,sinks", [(1, 1, 1, 1, 64, 1, 0), (1, 700, 8, 2, 128, 300, 4), (1, 700, 4, 4, 64, 1000, 0), (2, 517, 6, 2, 128, 100, 130),
+                                                         (1, 5000, 16, 2, 64, 4096, 16), (3, 33, 10, 1, 128, 7, 2), (8, 400, 4, 1, 64, 60, 3),
+                                                         (5, 3, 2, 1, 128, 2, 1), (1, 1300, 32, 1, 128, 1200, 4), (4, 200, 12, 4, 128, 1, 0)])
+def test_few_queries_without_gradients(Sq, Sk, Hq, Hkv, D, window, sinks):
+    ids = _documents(3, Sk, [Sk // 2, Sk // 3], 1) if Sk > 30 else None
+    for seq in (None, ids):
+        for packed in (False, True):
+            if packed and Sq > Sk:
+                continue
+            q, k, v = _qkv(3, Sq, Sk, Hq, Hkv, D, seed=Sk, packed=packed)
+            with torch.no_grad():
+                out, lse = sliding_window_attention(q, k, v, window=window, sinks=sinks, sequence_ids=seq, return_lse=True)
+            _lib.fetch_status()
+            (value, bound), w_lse, *_ = _expect(q, k, v, torch.zeros_like(q), window, sinks, seq, 1 / math.sqrt(D))
+            _near("out", out, (value, bound))
+            finite = torch.isfinite(w_lse)
+            assert torch.equal(torch.isfinite(lse), finite) and torch.isneginf(lse[~finite]).all()
+            assert not finite.any() or (lse[finite].double() - w_lse[finite]).abs().max() < 1e-4
+            again = sliding_window_attention(q, k, v, window=window, sinks=sinks, sequence_ids=seq)
+            assert torch.equal(out, again)
