@@ -29,7 +29,7 @@ def _contiguous(t: torch.Tensor) -> torch.Tensor:
 
 def _lookup(ids: torch.Tensor, w: torch.Tensor, scale: float) -> torch.Tensor:
     rows, H = w.shape
-    out = torch.empty((*ids.shape, H), dtype=w.dtype, device=w.device)
+    out = w.new_empty((*ids.shape, H))
     with _lib.on_device_of(w):
         _lib.check(_lib.lib().mb_embedding_fwd(ids.data_ptr(), 1 if ids.dtype == torch.int64 else 0, w.data_ptr(), out.data_ptr(),
                                                _DTYPES[w.dtype], ids.numel(), H, rows, scale, _lib.stream_of(w)), "mb_embedding_fwd")
@@ -49,9 +49,9 @@ class _Embedding(torch.autograd.Function):
         (ids,) = ctx.saved_tensors
         H, n, dout = dout.shape[-1], ids.numel(), _contiguous(dout)
         L = _lib.lib()
-        dweight = torch.empty((ctx.rows, H), dtype=dout.dtype, device=dout.device)
+        dweight = dout.new_empty((ctx.rows, H))
         with _lib.on_device_of(dout):
-            scratch = torch.empty((L.mb_embedding_bwd_scratch_words(n, H),), dtype=torch.int32, device=dout.device)
+            scratch = ids.new_empty(L.mb_embedding_bwd_scratch_words(n, H) // (1 if ids.dtype == torch.int32 else 2) + 1)   # 4-byte words
             _lib.check(L.mb_embedding_bwd(ids.data_ptr(), 1 if ids.dtype == torch.int64 else 0, dout.data_ptr(), dweight.data_ptr(),
                                           scratch.data_ptr(), _DTYPES[dout.dtype], n, H, ctx.rows,
                                           -1 if ctx.padding_idx is None else ctx.padding_idx, ctx.scale, _lib.stream_of(dout)),

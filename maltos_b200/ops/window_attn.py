@@ -56,7 +56,7 @@ def window_forward(q, k, v, *, window: int, sinks: int, starts, scale: float, ke
     q, q_t, q_b = _addressable(q)
     k, k_t, k_b = _addressable(k)
     v, v_t, v_b = _addressable(v)
-    out = torch.empty((B, Sq, Hq, D), dtype=torch.bfloat16, device=q.device)
+    out = q.new_empty((B, Sq, Hq, D))
     if not keep and _few_queries(B, Hkv, Sq * (Hq // Hkv)):
         lse = torch.empty((B, Hq, Sq), dtype=torch.float32, device=q.device) if want_lse else None
         with _lib.on_device_of(q):
@@ -82,13 +82,11 @@ def window_backward(q, k, v, out, out_lo, lse2, dout, *, window: int, sinks: int
     k, k_t, k_b = _addressable(k)
     v, v_t, v_b = _addressable(v)
     dout, do_t, do_b = _addressable(dout)
-    dq = torch.empty((B, Sq, Hq, D), dtype=torch.bfloat16, device=q.device)
-    dk = torch.empty((B, Sk, Hkv, D), dtype=torch.bfloat16, device=q.device)
-    dv = torch.empty((B, Sk, Hkv, D), dtype=torch.bfloat16, device=q.device)
+    dq, dk, dv = q.new_empty((B, Sq, Hq, D)), q.new_empty((B, Sk, Hkv, D)), q.new_empty((B, Sk, Hkv, D))
     L = _lib.lib()
     with _lib.on_device_of(q):
         words = L.mb_window_attn_bwd_scratch_words(B, Sq, Sk, Hq, Hkv, D, window, sinks, 0 if starts is None else 1)
-        scratch = torch.empty((words,), dtype=torch.int32, device=q.device)
+        scratch = lse2.new_empty(words)
         _lib.check(L.mb_window_attn_bwd(q.data_ptr(), q_t, q_b, k.data_ptr(), k_t, k_b, v.data_ptr(), v_t, v_b, out.data_ptr(),
                                         out_lo.data_ptr(), dout.data_ptr(), do_t, do_b, lse2.data_ptr(), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(),
                                         _lib.address(starts), _lib.address(ends), scratch.data_ptr(), B, Sq, Sk, Hq, Hkv, D, window, sinks,
