@@ -13,6 +13,7 @@ import torch.nn as nn
 from torch.utils.checkpoint import checkpoint
 
 from maltos_b200.ops.cross_entropy import linear_cross_entropy
+from maltos_b200.ops.embedding import ScaledEmbedding
 from maltos_b200.ops.gemm import linear
 from maltos_b200.ops.grouped import grouped_linear
 from maltos_b200.utils.activation_checkpoint import activation_checkpoint_context_fn
@@ -70,6 +71,34 @@ def project_group(x: torch.Tensor, modules: Sequence[nn.Module]) -> tuple[torch.
 
         x = copy_to_group(x, modules[0].tp_group)
     return grouped_linear(x, weights)
+
+
+def check_block_options(config) -> None:
+    """The options of a decoder block that LLaMA and OLMo-2 share."""
+    if config.sliding_window is not None and config.sliding_window < 1:
+        raise ValueError(f"sliding_window must be at least 1, got {config.sliding_window}")
+    if config.sink_tokens < 0 or (config.sink_tokens and config.sliding_window is None):
+        raise ValueError(f"sink_tokens={config.sink_tokens} must not be negative and needs a sliding_window")
+    if config.full_attention_every is not None and (config.full_attention_every < 1 or config.sliding_window is None):
+        raise ValueError(f"full_attention_every={config.full_attention_every} must be at least 1 and needs a sliding_window")
+    if config.embedding_scale is not None and not config.embedding_scale > 0:
+        raise ValueError(f"embedding_scale must be positive, got {config.embedding_scale}")
+
+
+def layer_window(config, layer: int) -> int | None:
+    """The attention window of a layer, None where it sees all keys (``full_attention_every=n``: layers n - 1, 2n - 1, ...)."""
+    every = config.full_attention_every
+    return None if every is not None and layer % every == every - 1 else config.sliding_window
+
+
+def attention_span(config) -> int:
+    """Keys that a query of the longest row attends to at most, summed over the layers (for FLOP counts)."""
+    windows = [layer_window(config, i) for i in range(config.num_hidden_layers)]
+    return sum(config.max_position_embeddings if w is None else min(w + config.sink_tokens, config.max_position_embeddings) for w in windows)
+
+
+def token_embedding(vocab_size: int, hidden_size: int, scale: float | None) -> nn.Embedding:
+    return nn.Embedding(vocab_size, hidden_size) if scale is None else ScaledEmbedding(vocab_size, hidden_size, scale)
 
 
 class Linear(nn.Linear):

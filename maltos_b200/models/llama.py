@@ -13,15 +13,16 @@ from dataclasses import dataclass, field
 import torch
 import torch.nn as nn
 
-from maltos_b200.ops.attention import causal_attention
-from maltos_b200.ops.norm import add_rms_norm, rms_norm
+from maltos_b200.ops.attention import causal_attention, sliding_window_attention
+from maltos_b200.ops.norm import add_rms_norm, block_norm, rms_norm
 from maltos_b200.ops.rope import build_rope_cache, rope_qkv_split
 from maltos_b200.ops.swiglu import swiglu_packed, swiglu
 from maltos_b200.parallel.specs import (ContextParallelSpec, PipelineParallelSpec, TpSpParallelSpec, TpSpShardAxis,
                                         TpSpShardRule)
 
 from .activation_checkpointing import ActivationCheckpointConfig
-from .common import Linear, ParsedBatch, lm_logits, lm_loss, project_group, project_out, run_layer
+from .common import (Linear, ParsedBatch, attention_span, check_block_options, layer_window, lm_logits, lm_loss, project_group, project_out,
+                     run_layer, token_embedding)
 
 
 @dataclass(frozen=True)
@@ -38,11 +39,19 @@ class LlamaConfig:
     tie_word_embeddings: bool = False
     attention_backend: str = "sdpa_auto"
     activation_checkpointing: ActivationCheckpointConfig = field(default_factory=ActivationCheckpointConfig)
+    sliding_window: int | None = None             # keys a query sees behind itself; None: all
+    sink_tokens: int = 0                          # first tokens of a document that stay visible beyond the window
+    full_attention_every: int | None = None       # with a window: every n-th layer sees all keys
+    embedding_scale: float | None = None          # token embeddings are multiplied by this
+    post_block_norm: bool = False                 # a norm after attention and MLP too, before they join the residual stream
+    residual_scale: float = 1.0                   # what a block adds to the stream is multiplied by this
+    residual_gate: bool = False                   # ... and by a learned gate per channel
 
     def __post_init__(self) -> None:
         from maltos_b200.utils.attention_backend import validate_attention_backend
 
         validate_attention_backend(self.attention_backend)
+        check_block_options(self)
 
 
 class LlamaRMSNorm(nn.Module):
@@ -57,6 +66,22 @@ class LlamaRMSNorm(nn.Module):
         if residual is None:
             return rms_norm(x, self.weight, self.eps)
         return add_rms_norm(x, residual, self.weight, self.eps)
+
+
+class BlockNorm(nn.Module):
+    """Seam between a block and what follows it in one pass: the block's output ``a`` through its own norm (``after``), a learned
+    gate per channel (``gate``) and the residual scale onto the stream ``x``, and the next block's norm (``before``).
+    ``forward(a, residual=x)`` returns ``(y, x)`` as :class:`LlamaRMSNorm` does, or ``x`` alone without ``before``. ``weight`` is the
+    next block's norm, so a checkpoint keeps that name; ``after_weight`` and ``gate`` exist where asked for."""
+
+    def __init__(self, hidden_size: int, eps: float, *, after: bool, before: bool, gate: bool, scale: float) -> None:
+        super().__init__()
+        for name, wanted in (("weight", before), ("after_weight", after), ("gate", gate)):
+            self.register_parameter(name, nn.Parameter(torch.ones(hidden_size)) if wanted else None)
+        self.eps, self.scale = eps, scale
+
+    def forward(self, a: torch.Tensor, residual: torch.Tensor):
+        return block_norm(a, residual, self.after_weight, self.weight, gate=self.gate, scale=self.scale, eps=self.eps)
 
 
 class LlamaRotaryEmbedding(nn.Module):
@@ -83,11 +108,14 @@ class _LlamaAttentionCore(nn.Module):
     preserves_native_gqa = True
     layout = "bshd"
 
-    def __init__(self, attention_backend: str = "sdpa_auto") -> None:
+    def __init__(self, attention_backend: str = "sdpa_auto", window: int | None = None, sinks: int = 0) -> None:
         super().__init__()
         self.attention_backend = attention_backend
+        self.window, self.sinks = window, sinks
 
     def forward(self, q, k, v, position_offset: int = 0, position_ids=None, sequence_ids=None):
+        if self.window is not None:
+            return sliding_window_attention(q, k, v, window=self.window, sinks=self.sinks, sequence_ids=sequence_ids)
         return causal_attention(q, k, v, position_ids=position_ids, sequence_ids=sequence_ids)
 
 
@@ -95,7 +123,7 @@ class LlamaAttention(nn.Module):
     handles_sequence_parallel_input = True
     rope_interleaved = True
 
-    def __init__(self, config: LlamaConfig) -> None:
+    def __init__(self, config: LlamaConfig, layer: int = 0) -> None:
         super().__init__()
         if config.hidden_size % config.num_attention_heads:
             raise ValueError("hidden_size must be divisible by num_attention_heads")
@@ -111,7 +139,7 @@ class LlamaAttention(nn.Module):
         self.k_proj = Linear(config.hidden_size, self.num_kv_heads * self.head_dim, bias=False)
         self.v_proj = Linear(config.hidden_size, self.num_kv_heads * self.head_dim, bias=False)
         self.o_proj = Linear(config.hidden_size, config.hidden_size, bias=False)
-        self.attn_core = _LlamaAttentionCore(config.attention_backend)
+        self.attn_core = _LlamaAttentionCore(config.attention_backend, layer_window(config, layer), config.sink_tokens)
 
     def parameter_fusion_groups(self):
         return [[self.q_proj.weight, self.k_proj.weight, self.v_proj.weight]]
@@ -154,17 +182,25 @@ class LlamaMLP(nn.Module):
 
 
 class LlamaDecoderLayer(nn.Module):
-    def __init__(self, config: LlamaConfig) -> None:
+    def __init__(self, config: LlamaConfig, layer: int = 0) -> None:
         super().__init__()
-        self.self_attn = LlamaAttention(config)
+        self.self_attn = LlamaAttention(config, layer)
         self.mlp = LlamaMLP(config)
         self.input_layernorm = LlamaRMSNorm(config.hidden_size, config.rms_norm_eps)
-        self.post_attention_layernorm = LlamaRMSNorm(config.hidden_size, config.rms_norm_eps)
+        if config.post_block_norm or config.residual_gate or config.residual_scale != 1.0:
+            seam = dict(after=config.post_block_norm, gate=config.residual_gate, scale=config.residual_scale)
+            self.post_attention_layernorm = BlockNorm(config.hidden_size, config.rms_norm_eps, before=True, **seam)
+            self.post_feedforward_layernorm = BlockNorm(config.hidden_size, config.rms_norm_eps, before=False, **seam)
+        else:
+            self.post_attention_layernorm = LlamaRMSNorm(config.hidden_size, config.rms_norm_eps)
+            self.post_feedforward_layernorm = None
 
     def forward(self, x, position_offset: int = 0, position_ids=None, sequence_ids=None):
         a = self.self_attn(self.input_layernorm(x), position_offset=position_offset, position_ids=position_ids,
                            sequence_ids=sequence_ids)
         y, x = self.post_attention_layernorm(a, residual=x)   # x <- x + a ; y = norm(x), one pass
+        if self.post_feedforward_layernorm is not None:
+            return self.post_feedforward_layernorm(self.mlp(y), residual=x)
         return x + self.mlp(y)
 
 
@@ -174,8 +210,8 @@ class LlamaForCausalLM(nn.Module):
     def __init__(self, config: LlamaConfig) -> None:
         super().__init__()
         self.config = config
-        self.embed_tokens = nn.Embedding(config.vocab_size, config.hidden_size)
-        self.layers = nn.ModuleList([LlamaDecoderLayer(config) for _ in range(config.num_hidden_layers)])
+        self.embed_tokens = token_embedding(config.vocab_size, config.hidden_size, config.embedding_scale)
+        self.layers = nn.ModuleList([LlamaDecoderLayer(config, i) for i in range(config.num_hidden_layers)])
         self.norm = LlamaRMSNorm(config.hidden_size, config.rms_norm_eps)
         self.lm_head = Linear(config.hidden_size, config.vocab_size, bias=False)
         if config.tie_word_embeddings:
@@ -216,8 +252,8 @@ class LlamaForCausalLM(nn.Module):
 
     def flops_per_token(self) -> float:
         c = self.config
-        per_layer = 8 * c.hidden_size * c.hidden_size + 6 * c.hidden_size * c.intermediate_size + 4 * c.max_position_embeddings * c.hidden_size
-        return float(3 * (c.num_hidden_layers * per_layer + 2 * c.hidden_size * c.vocab_size))
+        per_layer = 8 * c.hidden_size * c.hidden_size + 6 * c.hidden_size * c.intermediate_size
+        return float(3 * (c.num_hidden_layers * per_layer + 4 * attention_span(c) * c.hidden_size + 2 * c.hidden_size * c.vocab_size))
 
 
 def _tp_rules(n_layers: int, post: str) -> list[TpSpShardRule]:

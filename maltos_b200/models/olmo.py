@@ -13,8 +13,9 @@ from maltos_b200.parallel.specs import (ContextParallelSpec, PipelineParallelSpe
 from maltos_b200.runtime.layers.distributed_rmsnorm import DistributedRMSNorm
 
 from .activation_checkpointing import ActivationCheckpointConfig
-from .common import Linear, ParsedBatch, lm_logits, lm_loss, project_group, project_out, run_layer
-from .llama import LlamaMLP, LlamaRMSNorm, LlamaRotaryEmbedding, _LlamaAttentionCore
+from .common import (Linear, ParsedBatch, attention_span, check_block_options, layer_window, lm_logits, lm_loss, project_group, project_out,
+                     run_layer, token_embedding)
+from .llama import BlockNorm, LlamaMLP, LlamaRMSNorm, LlamaRotaryEmbedding, _LlamaAttentionCore
 
 
 @dataclass(frozen=True)
@@ -32,11 +33,18 @@ class OlmoConfig:
     attention_bias: bool = False
     attention_backend: str = "sdpa_auto"
     activation_checkpointing: ActivationCheckpointConfig = field(default_factory=ActivationCheckpointConfig)
+    sliding_window: int | None = None             # as in LlamaConfig
+    sink_tokens: int = 0
+    full_attention_every: int | None = None
+    embedding_scale: float | None = None
+    residual_scale: float = 1.0
+    residual_gate: bool = False
 
     def __post_init__(self) -> None:
         from maltos_b200.utils.attention_backend import validate_attention_backend
 
         validate_attention_backend(self.attention_backend)
+        check_block_options(self)
 
 
 class OlmoRMSNorm(LlamaRMSNorm):
@@ -50,7 +58,7 @@ class OlmoRotaryEmbedding(LlamaRotaryEmbedding):
 class OlmoAttention(nn.Module):
     handles_sequence_parallel_input = True
 
-    def __init__(self, config: OlmoConfig) -> None:
+    def __init__(self, config: OlmoConfig, layer: int = 0) -> None:
         super().__init__()
         if config.hidden_size % config.num_attention_heads:
             raise ValueError("hidden_size must be divisible by num_attention_heads")
@@ -68,7 +76,7 @@ class OlmoAttention(nn.Module):
         self.o_proj = Linear(config.hidden_size, config.hidden_size, bias=b)
         self.q_norm = DistributedRMSNorm(self.num_heads * self.head_dim, config.rms_norm_eps)
         self.k_norm = DistributedRMSNorm(self.num_kv_heads * self.head_dim, config.rms_norm_eps)
-        self.attn_core = _LlamaAttentionCore(config.attention_backend)
+        self.attn_core = _LlamaAttentionCore(config.attention_backend, layer_window(config, layer), config.sink_tokens)
 
     def parameter_fusion_groups(self):
         return [[self.q_proj.weight, self.k_proj.weight, self.v_proj.weight]]
@@ -93,14 +101,24 @@ class OlmoAttention(nn.Module):
 
 
 class OlmoDecoderLayer(nn.Module):
-    def __init__(self, config: OlmoConfig) -> None:
+    def __init__(self, config: OlmoConfig, layer: int = 0) -> None:
         super().__init__()
-        self.self_attn = OlmoAttention(config)
+        self.self_attn = OlmoAttention(config, layer)
         self.mlp = LlamaMLP(config)
-        self.post_attention_layernorm = OlmoRMSNorm(config.hidden_size, config.rms_norm_eps)
-        self.post_feedforward_layernorm = OlmoRMSNorm(config.hidden_size, config.rms_norm_eps)
+        self.joined = config.residual_gate or config.residual_scale != 1.0
+        if self.joined:
+            seam = dict(after=True, before=False, gate=config.residual_gate, scale=config.residual_scale)
+            self.post_attention_layernorm = BlockNorm(config.hidden_size, config.rms_norm_eps, **seam)
+            self.post_feedforward_layernorm = BlockNorm(config.hidden_size, config.rms_norm_eps, **seam)
+        else:
+            self.post_attention_layernorm = OlmoRMSNorm(config.hidden_size, config.rms_norm_eps)
+            self.post_feedforward_layernorm = OlmoRMSNorm(config.hidden_size, config.rms_norm_eps)
 
     def forward(self, x, position_offset: int = 0, position_ids=None, sequence_ids=None, rotary=None):
+        if self.joined:
+            a = self.self_attn(x, position_offset=position_offset, position_ids=position_ids, sequence_ids=sequence_ids, rotary=rotary)
+            x = self.post_attention_layernorm(a, residual=x)
+            return self.post_feedforward_layernorm(self.mlp(x), residual=x)
         x = x + self.post_attention_layernorm(self.self_attn(x, position_offset=position_offset, position_ids=position_ids,
                                                              sequence_ids=sequence_ids, rotary=rotary))
         return x + self.post_feedforward_layernorm(self.mlp(x))
@@ -112,11 +130,11 @@ class OlmoForCausalLM(nn.Module):
     def __init__(self, config: OlmoConfig) -> None:
         super().__init__()
         self.config = config
-        self.embed_tokens = nn.Embedding(config.vocab_size, config.hidden_size)
+        self.embed_tokens = token_embedding(config.vocab_size, config.hidden_size, config.embedding_scale)
         head_dim = config.hidden_size // config.num_attention_heads
         # one model-level table shared by all layers
         self.rotary_emb = OlmoRotaryEmbedding(head_dim, config.max_position_embeddings, config.rope_theta)
-        self.layers = nn.ModuleList([OlmoDecoderLayer(config) for _ in range(config.num_hidden_layers)])
+        self.layers = nn.ModuleList([OlmoDecoderLayer(config, i) for i in range(config.num_hidden_layers)])
         self.norm = OlmoRMSNorm(config.hidden_size, config.rms_norm_eps)
         self.lm_head = Linear(config.hidden_size, config.vocab_size, bias=False)
         if config.tie_word_embeddings:
@@ -157,8 +175,8 @@ class OlmoForCausalLM(nn.Module):
 
     def flops_per_token(self) -> float:
         c = self.config
-        per_layer = 8 * c.hidden_size * c.hidden_size + 6 * c.hidden_size * c.intermediate_size + 4 * c.max_position_embeddings * c.hidden_size
-        return float(3 * (c.num_hidden_layers * per_layer + 2 * c.hidden_size * c.vocab_size))
+        per_layer = 8 * c.hidden_size * c.hidden_size + 6 * c.hidden_size * c.intermediate_size
+        return float(3 * (c.num_hidden_layers * per_layer + 4 * attention_span(c) * c.hidden_size + 2 * c.hidden_size * c.vocab_size))
 
 
 def _olmo_rules(n_layers: int, sequence_parallel: bool) -> list[TpSpShardRule]:

@@ -27,3 +27,10 @@ def canonical_sequence_ids(sequence_ids, *, batch_size: int, seq_len: int, devic
 
 def build_example_causal_mask(*, q_positions, k_positions, q_sequence_ids=None, k_sequence_ids=None) -> torch.Tensor:
     return build_visibility_mask(q_positions, k_positions, q_sequence_ids, k_sequence_ids)
+
+
+def refuse_windowed_core(path: str, core) -> None:
+    """The context-parallel attention cores know causal and document masks only; putting one in the place of a core with a
+    sliding window would silently widen the model's attention."""
+    if getattr(core, "window", None) is not None:
+        raise ValueError(f"{path} has a sliding window of {core.window}; context parallelism and HDP do not support sliding_window")

@@ -20,6 +20,7 @@ from maltos_b200.parallel.context_interfaces import ContextParallelAttentionCore
 from maltos_b200.parallel.context_token_planner import ContextTokenPlannerType, build_context_token_planner
 from maltos_b200.parallel.protocols import ContextParallelizableModule
 from maltos_b200.runtime.layers.all_gather_attention import AllGatherKvAttentionCore
+from maltos_b200.runtime.layers.attn_masking_utils import refuse_windowed_core
 from maltos_b200.runtime.layers.ring_attention import RingAttentionCore
 from maltos_b200.runtime.mesh import MeshAxis
 from maltos_b200.runtime.plugin import PluginId, RuntimePlugin
@@ -69,6 +70,7 @@ class ContextParallelPlugin(RuntimePlugin):
                     continue
                 if block is None or not hasattr(block, "attn_core"):
                     continue
+                refuse_windowed_core(path, block.attn_core)
                 backend = getattr(block.attn_core, "attention_backend", "eager")
                 if kind is ContextParallelAttentionCoreType.RING:
                     core = RingAttentionCore(self.cp_group, backend)

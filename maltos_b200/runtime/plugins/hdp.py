@@ -17,6 +17,7 @@ import torch.nn as nn
 from maltos_b200.parallel.hdp_helper import (BYTESCALE_HDP_SCHEDULE_KEY, BYTESCALE_HDP_WAVES_KEY, ByteScaleHdpBalancedConfig,
                                              ByteScaleHdpLocalLayout)
 from maltos_b200.parallel.protocols import ContextParallelizableModule
+from maltos_b200.runtime.layers.attn_masking_utils import refuse_windowed_core
 from maltos_b200.runtime.layers.hdp_attention import HdpBalancedAttentionCore
 from maltos_b200.runtime.mesh import MeshAxis
 from maltos_b200.runtime.plugin import PluginId, RuntimePlugin
@@ -115,6 +116,7 @@ class ByteScaleHdpPlugin(RuntimePlugin):
             block = model.get_submodule(path)
             if not hasattr(block, "attn_core"):
                 raise TypeError(f"attention module path={path} has no attn_core")
+            refuse_windowed_core(path, block.attn_core)
             core = HdpBalancedAttentionCore(self.hdp_group, attention_backend=getattr(block.attn_core, "attention_backend", AttentionBackend.EAGER))
             block.attn_core = core
             self._attention_cores.append(core)

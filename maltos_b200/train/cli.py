@@ -75,6 +75,11 @@ def validate_args(args: argparse.Namespace, world_size: int) -> None:
                          "(the pipeline runner cuts every micro-batch into that many pieces)")
     if getattr(args, "token_weighted_loss", False) and args.hdp_balanced:
         raise ValueError("--token-weighted-loss is implied by --hdp-balanced (HDP weights every rank's loss by its targets)")
+    for name, default in _BLOCK_OPTIONS.items():
+        if getattr(args, name, default) != default and args.model not in (("llama",) if name == "post_block_norm" else ("llama", "olmo", "olmo2")):
+            raise ValueError(f"--{name.replace('_', '-')} is not an option of --model {args.model}")
+    if getattr(args, "sliding_window", None) is not None and (args.cp_size > 1 or args.hdp_balanced):
+        raise ValueError("--sliding-window is not supported with --cp-size > 1 or --hdp-balanced")
     if args.ep_size > 1 and args.dp_size % args.ep_size:
         raise ValueError("--ep-size must divide --dp-size")
     if args.ep_size > 1 and args.model != "tiny_moe":
@@ -128,6 +133,11 @@ def resolve_resume_path(resume_from, checkpoint_dir, *, rank: int):
 
 
 # ------------------------------------------------------------------------------------------------ model
+#: options of the decoder block (``LlamaConfig``, ``OlmoConfig``) that are flags too, with the flags' defaults
+_BLOCK_OPTIONS = {"sliding_window": None, "sink_tokens": 0, "full_attention_every": None, "embedding_scale": None, "post_block_norm": False,
+                  "residual_scale": 1.0, "residual_gate": False}
+
+
 def _variant(base, tp, sp, args):
     return sp if args.use_sp else (tp if args.tp_size > 1 else base)
 
@@ -137,6 +147,7 @@ def _build_model(args: argparse.Namespace) -> nn.Module:
 
     ckpt = M.ActivationCheckpointConfig(enabled=bool(args.activation_checkpointing), every_n_layers=args.activation_checkpoint_every_n_layers)
     name = args.model
+    block = {k: getattr(args, k, d) for k, d in _BLOCK_OPTIONS.items()}
     if name == "tiny":
         cls = _variant(M.TinyTransformer, M.TinyTransformerTp, M.TinyTransformerTpSp, args)
         model = cls(args.dim, args.n_heads, args.n_kv_heads or args.n_heads, args.hidden_size, args.eps, args.n_layers,
@@ -154,14 +165,15 @@ def _build_model(args: argparse.Namespace) -> nn.Module:
                                   num_hidden_layers=args.n_layers, num_attention_heads=args.n_heads, num_key_value_heads=args.n_kv_heads,
                                   max_position_embeddings=args.seq_len, rms_norm_eps=args.eps,
                                   rope_theta=getattr(args, "rope_theta", None) or 10000.0,
-                                  attention_backend=args.attention_backend, activation_checkpointing=ckpt))
+                                  attention_backend=args.attention_backend, activation_checkpointing=ckpt, **block))
     elif name in ("olmo", "olmo2"):
         cls = _variant(M.OlmoForCausalLM, M.OlmoForCausalLMTp, M.OlmoForCausalLMTpSp, args)
+        block.pop("post_block_norm")          # its norms stand after the blocks anyway
         model = cls(M.OlmoConfig(vocab_size=args.vocab_size, hidden_size=args.dim, intermediate_size=args.hidden_size,
                                  num_hidden_layers=args.n_layers, num_attention_heads=args.n_heads, num_key_value_heads=args.n_kv_heads,
                                  max_position_embeddings=args.seq_len, rms_norm_eps=args.eps,
                                  rope_theta=getattr(args, "rope_theta", None) or 500000.0,
-                                 attention_backend=args.attention_backend, activation_checkpointing=ckpt))
+                                 attention_backend=args.attention_backend, activation_checkpointing=ckpt, **block))
     else:
         raise ValueError(f"unknown model={name}")
     std = getattr(args, "init_std", None)
@@ -173,11 +185,11 @@ def _build_model(args: argparse.Namespace) -> nn.Module:
 
 
 def _zero3_wrap_classes() -> set[type]:
-    from maltos_b200.models.llama import LlamaRMSNorm
+    from maltos_b200.models.llama import BlockNorm, LlamaRMSNorm
     from maltos_b200.models.tiny_transformer import RmsNorm
     from maltos_b200.runtime.layers.distributed_rmsnorm import DistributedRMSNorm
 
-    return {nn.Linear, nn.Embedding, nn.LayerNorm, RmsNorm, LlamaRMSNorm, DistributedRMSNorm}
+    return {nn.Linear, nn.Embedding, nn.LayerNorm, RmsNorm, LlamaRMSNorm, BlockNorm, DistributedRMSNorm}
 
 
 def _build_hdp_config(args: argparse.Namespace):

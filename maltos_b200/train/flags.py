@@ -5,8 +5,9 @@ for it); the argparse parser, the recipe->flag mapping and the spec field lists 
 pre-parsed from ``--config`` and becomes parser *defaults*, so explicit flags win. Flag names, defaults, the alias set and
 the spec layout (``format = "train_cli_args"``, ``version = 3``, 16 model + 22 runtime fields, strict field check) are
 those of the reference (``train/flags.py:12-403``) because recipes and checkpoints carry them. Additional flags of this
-framework: ``--pp-schedule``, ``--rope-theta``, ``--moe-top-k``, ``--moe-capacity-factor``, ``--init-std``; they are
-deliberately NOT part of the spec so that spec files stay interchangeable.
+framework: ``--pp-schedule``, ``--rope-theta``, ``--moe-top-k``, ``--moe-capacity-factor``, ``--init-std`` and the block options
+(``--sliding-window``, ``--sink-tokens``, ``--full-attention-every``, ``--embedding-scale``, ``--post-block-norm``,
+``--residual-scale``, ``--residual-gate``); they are deliberately NOT part of the spec so that spec files stay interchangeable.
 """
 from __future__ import annotations
 
@@ -74,6 +75,13 @@ FLAGS: tuple[Flag, ...] = (
     Flag("rope_theta", float, None, yaml=("model.rope_theta",), help="RoPE base (default: 10000 for llama, 500000 for olmo)"),
     Flag("moe_top_k", int, 1, yaml=("model.moe_top_k",)),
     Flag("moe_capacity_factor", float, None, yaml=("model.moe_capacity_factor",)),
+    Flag("sliding_window", int, None, yaml=("model.sliding_window",), help="llama, olmo: keys a query sees behind itself (default: all)"),
+    Flag("sink_tokens", int, 0, yaml=("model.sink_tokens",), help="with --sliding-window: first tokens of a document that stay visible"),
+    Flag("full_attention_every", int, None, yaml=("model.full_attention_every",), help="with --sliding-window: every n-th layer sees all keys"),
+    Flag("embedding_scale", float, None, yaml=("model.embedding_scale",), help="llama, olmo: factor on the token embeddings"),
+    Flag("post_block_norm", BOOL, False, yaml=("model.post_block_norm",), help="llama: a norm after attention and MLP too"),
+    Flag("residual_scale", float, 1.0, yaml=("model.residual_scale",), help="llama, olmo: factor on what a block adds to the residual stream"),
+    Flag("residual_gate", BOOL, False, yaml=("model.residual_gate",), help="llama, olmo: a learned gate per channel on what a block adds"),
     Flag("init_std", float, None, yaml=("model.init_std",), help="re-initialise matrices with normal(0, std)"),
     # parallelism
     Flag("dp_size", int, 1, yaml=("parallel.dp_size",)),
