@@ -3,10 +3,11 @@
 // softmax of one tile runs under the matrix products of the other:
 //   warp 0       TMA producer: the tiles' queries and a ring of K and V blocks,
 //   warps 1, 2   one per tile: issue S = Q K^T and O += P V as UMMAs; S, P and O stay in tensor memory (P overwrites the scores it
-//                came from). A wait that is already satisfied still costs some 250 cycles while UMMAs saturate shared memory, so
+//                came from). A wait that is already satisfied still costs up to 250 cycles while UMMAs saturate shared memory, so
 //                each tile has an issuer of its own and no barrier is asked twice,
-//   warps 4-7 and 8-11  one warpgroup per tile, a thread per query row: running maximum and sum, P in bf16, output. P is handed
-//                over in halves of 64 keys, so that O += P V begins under the second half's exponentials.
+//   warps 3-18   eight per tile, two threads per query row with 64 keys of a block each: running maximum and sum, P in bf16, output.
+//                With one thread per row a scheduler has one warp of a tile to run, which takes 14 cycles an exponential where
+//                the special-function unit needs 8; the price of two is an exchange of their maxima in every block.
 // The two tiles are two query heads of one key/value head on the same rows where the group is even, else neighbouring rows of
 // one head. O is rescaled only when a row's maximum has grown by more than 2^8 since the last rescale: P then stays below 2^8
 // and its bf16 rounding is relative, so nothing is lost, and after the first blocks the rescale hardly ever happens.
@@ -21,11 +22,9 @@
 
 namespace mb {
 
-constexpr int kWfThreads = 384;
+constexpr int kWfSoftmaxWarps = 16;
+constexpr int kWfThreads = 32 * (3 + kWfSoftmaxWarps);
 constexpr int kWfStages = 5;                       // K and V blocks in flight
-// registers: the launch gives 168 x 384 = 64512; after the split 128 x 56 + 256 x 224 = 64512
-constexpr int kWfLaunchRegs = 168, kWfOtherRegs = 56, kWfSoftmaxRegs = 224;
-static_assert(128 * kWfOtherRegs + 256 * kWfSoftmaxRegs <= kWfThreads * kWfLaunchRegs, "register split exceeds the launch");
 constexpr float kWfLog2e = 1.4426950408889634f, kWfLn2 = 0.6931471805599453f;
 constexpr float kWfGrowth = 8.f;                   // log2 of how far P may exceed 1 before O is rescaled
 
@@ -96,32 +95,39 @@ window_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
   constexpr int ATOM_BYTES = kWinBlock * 128;
   constexpr uint32_t TMEM_COLS = 512, O_COL = 0, S_COL = 256;   // O of tile t at t * 128, its scores at 256 + t * 128
 
-  extern __shared__ uint8_t smem_raw[];
-  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  extern __shared__ __align__(1024) uint8_t smem_raw[];   // with head_dim 128 the tiles fill it: its start has to be aligned
+  uint8_t* smem = smem_raw;
   uint8_t* sQ = smem;                              // 2 tiles
   uint8_t* sKV = sQ + 2 * TILE_BYTES;              // kWfStages blocks
   uint64_t* bars = reinterpret_cast<uint64_t*>(sKV + kWfStages * TILE_BYTES);
   uint64_t* q_full = bars;                         // 2
   uint64_t* q_empty = bars + 2;                    // 2
   uint64_t* s_full = bars + 4;                     // 2
-  uint64_t* p_full = bars + 6;                     // 2 tiles x 2 halves
-  uint64_t* o_full = bars + 10;                    // 2
-  uint64_t* kv_full = bars + 12;                   // kWfStages
+  uint64_t* p_full = bars + 6;                     // 2
+  uint64_t* o_full = bars + 8;                     // 2
+  uint64_t* kv_full = bars + 10;                   // kWfStages
   uint64_t* kv_empty = kv_full + kWfStages;        // kWfStages
   uint64_t* turn = kv_empty + kWfStages;           // 2: the exponentials of a block are tile t's turn
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(turn + 2);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  float* exchange = reinterpret_cast<float*>(smem + (2 + kWfStages) * TILE_BYTES + 256);   // [tile][half][row]
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (smem_u32(smem_raw) & 1023u) {   // uniform over the CTA: nothing has been set up yet
+    if (threadIdx.x == 0) {
+      atomicOr(&p.status[0], MB_ERR_BAD_INDEX);
+      p.status[2] = 1015;
+    }
+    return;
+  }
   if (threadIdx.x == 0) {
     for (int t = 0; t < 2; ++t) {
       mbar_init(&q_full[t], 1);
       mbar_init(&q_empty[t], 1);
       mbar_init(&s_full[t], 1);
-      mbar_init(&p_full[2 * t], 4);
-      mbar_init(&p_full[2 * t + 1], 4);
+      mbar_init(&p_full[t], 8);
       mbar_init(&o_full[t], 1);
-      mbar_init(&turn[t], 4);
+      mbar_init(&turn[t], 8);
     }
     for (int i = 0; i < kWfStages; ++i) {
       mbar_init(&kv_full[i], 1);
@@ -143,8 +149,7 @@ window_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
   tc_fence_after();
   const uint32_t tmem_base = *tmem_slot;
 
-  if (warp < 4) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kWfOtherRegs));
+  if (warp < 3) {
     if (warp == 0) {
       // ---------------------------------------------------------------- TMA producer
       int slot = 0, round = 0;                     // ring position and how often it has gone round
@@ -191,7 +196,7 @@ window_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
         ok = __shfl_sync(0xffffffffu, static_cast<int>(ok), 0) != 0;
         if (!ok) break;
       }
-    } else if (warp <= 2) {
+    } else {
       // ---------------------------------------------------------------- UMMA issuer of tile t
       // Step u: O += P V of block u - 1, then the scores of block u over that P. The scores' commit therefore also says that the
       // product before them is complete, which is what a rescale of O waits for.
@@ -228,19 +233,13 @@ window_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
             if (pending) {
               const uint32_t v_lo = smem_desc_lo(smem_u32(sKV + vs * TILE_BYTES), ATOM_BYTES);
               const uint32_t acc0 = has_o ? 1u : 0u;
-#pragma unroll
-              for (int half = 0; half < 2; ++half) {
-                ok = ok && mbar_wait(&p_full[2 * t + half], p_phase & 1, abort_flag);
-                if (!ok) break;
-                tc_fence_after();
-#pragma unroll
-                for (int k2 = 0; k2 < kWinBlock / 32; ++k2) {
-                  const int kk = half * (kWinBlock / 32) + k2;
-                  umma_bf16_ts_lh(o_tmem, s_tmem + static_cast<uint32_t>(kk * 8), v_lo + static_cast<uint32_t>(kk * 128), hi, idesc_pv,
-                                  kk != 0 ? 1u : acc0);
-                }
-              }
+              ok = mbar_wait(&p_full[t], p_phase & 1, abort_flag);
               if (!ok) break;
+              tc_fence_after();
+#pragma unroll
+              for (int kk = 0; kk < kWinBlock / 16; ++kk)   // the 64 keys of a half sit packed in the first 32 of their 64 columns
+                umma_bf16_ts_lh(o_tmem, s_tmem + static_cast<uint32_t>((kk >> 2) * 64 + (kk & 3) * 8), v_lo + static_cast<uint32_t>(kk * 128), hi,
+                                idesc_pv, kk != 0 ? 1u : acc0);
               ++p_phase;
               has_o = true;
             }
@@ -277,17 +276,30 @@ window_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
     }
     __syncwarp();
   } else {
-    // ------------------------------------------------------------------ softmax and output: a thread per query row
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kWfSoftmaxRegs));
-    const int t = (warp - 4) >> 2;
+    // ------------------------------------------------------------------ softmax and output: two threads per query row
+    const int t = (warp - 3) >> 3, half = ((warp - 3) >> 2) & 1;
     const int row = (warp & 3) * 32 + lane;
     const uint32_t t_lane = static_cast<uint32_t>((warp & 3) * 32) << 16;
-    const uint32_t s_tmem = tmem_base + S_COL + static_cast<uint32_t>(t) * 128u + t_lane;
-    const uint32_t o_tmem = tmem_base + O_COL + static_cast<uint32_t>(t) * 128u + t_lane;
+    const uint32_t s_tmem = tmem_base + S_COL + static_cast<uint32_t>(t * 128 + half * 64) + t_lane;
+    constexpr int HALF_D = D / 2;                  // columns of O that this thread rescales and stores
+    const uint32_t o_tmem = tmem_base + O_COL + static_cast<uint32_t>(t * 128 + half * HALF_D) + t_lane;
+    // The two threads of a row exchange a value through shared memory and a barrier of their two warps. NaN says that a wait of
+    // one of them ran out: both then leave at the same place, so that neither is left behind at the barrier (a maximum is never
+    // NaN, and a sum that is NaN stops nothing but the output loop of its own rows, for which `stop` is not looked at).
+    // A slot is written again only after the partner has read it: between two blocks that follows from the P of both, which the
+    // next scores wait for; at the end of an item the barrier is passed once more.
+    float* slot = exchange + (t * 2 + half) * kWinBlock + row;
+    const float* partner = exchange + (t * 2 + (half ^ 1)) * kWinBlock + row;
+    auto pair_barrier = [&] { asm volatile("bar.sync %0, 64;" ::"r"(1 + t * 4 + (warp & 3)) : "memory"); };
+    auto swap = [&](float mine) {
+      *slot = mine;
+      pair_barrier();
+      return *const_cast<const volatile float*>(partner);
+    };
     int s_count = 0, o_count = 0;
     uint32_t turn_phase = 0;
     bool owed = false;                             // tile 0: the other tile had its last block too, and hands the turn back
-    bool ok = true;
+    bool ok = true, stop = false;
     for (int item = blockIdx.x; item < p.items; item += gridDim.x) {
       WindowItem it;
       window_item(p, item, it);
@@ -299,38 +311,46 @@ window_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
       const int n = tile.count();
       const int qi = q0 + row;
       const WindowRow w = window_row(p.rule, it.batch, p.Sk, qi + p.Sk - p.Sq, qi < p.Sq);
-      // m_run: the power of two that P is relative to; l_run: sum of the rounded P; x_run: of P as it was before
+      // m_run: the power of two that P is relative to; l_run: this half's sum of the rounded P; x_run: of P as it was before
       float m_run = -INFINITY, l_run = 0.f, x_run = 0.f;
       for (int j = 0; j < n; ++j) {
-        ok = mbar_wait(&s_full[t], s_count & 1, abort_flag);
+        ok = ok && mbar_wait(&s_full[t], s_count & 1, abort_flag);
         ok = __all_sync(0xffffffffu, ok);
-        if (!ok) break;
         ++s_count;
         tc_fence_after();
-        const int key0 = tile.block(j) * kWinBlock;
-        uint32_t s[128];
-#pragma unroll
-        for (int c = 0; c < 4; ++c) tmem_ld_32x32b_x32(s_tmem + c * 32, reinterpret_cast<uint32_t(&)[32]>(s[c * 32]));
-        tmem_ld_wait();
-        uint32_t none = 0;                         // bit c: no row of the warp sees a key of chunk c (of 32)
-        if (key0 < tile.full_lo || key0 + kWinBlock - 1 > tile.full_hi) {
-#pragma unroll
-          for (int c = 0; c < 4; ++c) {
-            const uint32_t seen = window_bits(w, key0 + c * 32);
-            if (__all_sync(0xffffffffu, seen == 0xffffffffu)) continue;
-            if (__all_sync(0xffffffffu, seen == 0u)) none |= 1u << c;
+        const int blk = tile.block(j), key0 = blk * kWinBlock + half * 64;
+        // The scores are read twice rather than kept: 32 of them at a time, the second chunk last, so that it is still there after
+        // the maximum.
+        uint32_t s[32], seen[2] = {0xffffffffu, 0xffffffffu};
+        float m_blk = -INFINITY;
+        if (blk * kWinBlock < tile.full_lo || blk * kWinBlock + kWinBlock - 1 > tile.full_hi)
+          seen[0] = window_bits(w, key0), seen[1] = window_bits(w, key0 + 32);
+        auto read = [&](int c) {
+          tmem_ld_32x32b_x32(s_tmem + c * 32, s);
+          tmem_ld_wait();
+          if (__any_sync(0xffffffffu, seen[c] != 0xffffffffu)) {
 #pragma unroll
             for (int i = 0; i < 32; ++i)
-              if (!((seen >> i) & 1u)) s[c * 32 + i] = __float_as_uint(-INFINITY);
+              if (!((seen[c] >> i) & 1u)) s[i] = __float_as_uint(-INFINITY);
           }
+        };
+        if (ok) {
+          float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+          for (int c = 0; c < 2; ++c) {
+            read(c);
+#pragma unroll
+            for (int i = 0; i < 32; i += 8)
+#pragma unroll
+              for (int k = 0; k < 4; ++k) mx[k] = fmaxf(fmaxf(mx[k], __uint_as_float(s[i + 2 * k])), __uint_as_float(s[i + 2 * k + 1]));
+          }
+          m_blk = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * p.scale_log2;
         }
-        float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll
-        for (int i = 0; i < 128; i += 8)
-#pragma unroll
-          for (int k = 0; k < 4; ++k) mx[k] = fmaxf(fmaxf(mx[k], __uint_as_float(s[i + 2 * k])), __uint_as_float(s[i + 2 * k + 1]));
-        const float m_blk = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * p.scale_log2;
-        if (__any_sync(0xffffffffu, m_blk > m_run + kWfGrowth)) {
+        const float m_other = swap(ok ? m_blk : NAN);
+        stop = __any_sync(0xffffffffu, !ok || m_other != m_other);
+        if (stop) break;
+        m_blk = fmaxf(m_blk, m_other);
+        if (__any_sync(0xffffffffu, m_blk > m_run + kWfGrowth)) {   // the same for the two warps of these rows
           const float m_new = fmaxf(m_run, ceilf(m_blk));
           const float alpha = m_run == -INFINITY ? 0.f : wf_exp2(m_run - m_new);   // a power of two
           m_run = m_new;
@@ -338,7 +358,7 @@ window_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
           if (LSE) x_run *= alpha;
           if (j > 0) {
 #pragma unroll 1
-            for (int c = 0; c < D; c += 16) {
+            for (int c = 0; c < HALF_D; c += 16) {
               uint32_t r[16];
               tmem_ld_32x32b_x16(o_tmem + c, r);
               tmem_ld_wait();
@@ -350,48 +370,43 @@ window_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
         }
         // The two tiles take turns with their exponentials: block by block, tile 0 first. Left alone they fall into step, both on
         // the exponentials and then both on the tensor cores, and neither is hidden.
-        const int blk = tile.block(j);
         const bool both = paired && other.has(blk);
         if (t == 0 ? owed : both) {
-          ok = mbar_wait(&turn[t], turn_phase & 1, abort_flag);
-          ok = __all_sync(0xffffffffu, ok);
-          if (!ok) break;
+          ok = mbar_wait(&turn[t], turn_phase & 1, abort_flag);   // a wait that runs out is acted on at the next exchange
           ++turn_phase;
         }
         const float m_safe = m_run == -INFINITY ? 0.f : m_run;
         const uint64_t scale2 = f32x2(p.scale_log2, p.scale_log2), shift2 = f32x2(-m_safe, -m_safe);
         uint64_t sum[2] = {0, 0}, sum_x[2] = {0, 0};
-#pragma unroll
-        for (int c = 0; c < 4; ++c) {              // 32 keys: 16 columns of packed P
-          uint32_t pk[16];
-          if ((none >> c) & 1u) {
-#pragma unroll
-            for (int i = 0; i < 16; ++i) pk[i] = 0u;
-          } else {
+        uint32_t pk[16];
+        auto weights = [&](int c) {                // P of the chunk in s
+          if (__any_sync(0xffffffffu, seen[c] != 0u)) {
 #pragma unroll
             for (int i = 0; i < 16; ++i) {
               float a, b;
-              const uint64_t x = fma_f32x2(f32x2(__uint_as_float(s[c * 32 + 2 * i]), __uint_as_float(s[c * 32 + 2 * i + 1])), scale2, shift2);
-              f32x2_split(x, a, b);
+              f32x2_split(fma_f32x2(f32x2(__uint_as_float(s[2 * i]), __uint_as_float(s[2 * i + 1])), scale2, shift2), a, b);
               a = wf_exp2(a), b = wf_exp2(b);
               pk[i] = pack_bf16x2(a, b);
               sum[i & 1] = add_f32x2(sum[i & 1], bf16x2_as_f32x2(pk[i]));
               if (LSE) sum_x[i & 1] = add_f32x2(sum_x[i & 1], f32x2(a, b));
             }
+          } else {                                 // no row of the warp sees a key of this chunk
+#pragma unroll
+            for (int i = 0; i < 16; ++i) pk[i] = 0u;
           }
-          tmem_st_32x32b_x16(s_tmem + c * 16, pk);
-          if (c == 3) {
-            // one arrival and one wait each way for every block that both have, so neither barrier gets two phases ahead
-            owed = both;
-            if (both && lane == 0) mbar_arrive(&turn[t ^ 1]);
-          }
-          if (c & 1) {
-            tmem_st_wait();
-            tc_fence_before();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&p_full[2 * t + (c >> 1)]);
-          }
-        }
+        };
+        weights(1);
+        read(0);                                   // before its scores are overwritten
+        tmem_st_32x32b_x16(s_tmem + 16, pk);
+        weights(0);
+        tmem_st_32x32b_x16(s_tmem, pk);
+        // one arrival and one wait each way for every block that both have, so neither barrier gets two phases ahead
+        owed = both;
+        if (both && lane == 0) mbar_arrive(&turn[t ^ 1]);
+        tmem_st_wait();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&p_full[t]);
         float lo, hi;
         f32x2_split(add_f32x2(sum[0], sum[1]), lo, hi);
         l_run += lo + hi;
@@ -400,44 +415,45 @@ window_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
           x_run += lo + hi;
         }
       }
-      if (!ok) break;
+      if (stop) break;
       // ---------------------------------------------------------------- output
       if (n > 0) {
-        ok = mbar_wait(&o_full[t], o_count & 1, abort_flag);
+        ok = ok && mbar_wait(&o_full[t], o_count & 1, abort_flag);
         ok = __all_sync(0xffffffffu, ok);
-        if (!ok) break;
         ++o_count;
         tc_fence_after();
       }
+      l_run += swap(l_run);
+      pair_barrier();
+      if (LSE) {
+        x_run += swap(x_run);
+        pair_barrier();
+      }
       const float inv = l_run > 0.f ? 1.f / l_run : 0.f;
-      const long long at = ((static_cast<long long>(it.batch) * p.Sq + qi) * p.Hq + head) * D;
+      const long long at = ((static_cast<long long>(it.batch) * p.Sq + qi) * p.Hq + head) * D + half * HALF_D;
 #pragma unroll 1
-      for (int c = 0; c < D; c += 32) {
-        uint32_t r[32];
-        if (n > 0) {                               // warp-collective: every lane takes part, rows inside the sequence are stored
-          tmem_ld_32x32b_x32(o_tmem + c, r);
-          tmem_ld_wait();
-        } else {
+      for (int c = 0; c < HALF_D; c += 16) {
+        uint32_t r[16];
 #pragma unroll
-          for (int i = 0; i < 32; ++i) r[i] = 0u;
+        for (int i = 0; i < 16; ++i) r[i] = 0u;
+        if (n > 0 && ok) {                         // warp-collective: every lane takes part, rows inside the sequence are stored
+          tmem_ld_32x32b_x16(o_tmem + c, r);
+          tmem_ld_wait();
         }
         if (qi < p.Sq) {
+          uint32_t v[8], lo[8];
 #pragma unroll
-          for (int i = 0; i < 32; i += 8) {
-            uint32_t v[4], w[4];
-#pragma unroll
-            for (int k = 0; k < 4; ++k) {
-              const float a = __uint_as_float(r[i + 2 * k]) * inv, b = __uint_as_float(r[i + 2 * k + 1]) * inv;
-              v[k] = pack_bf16x2(a, b);
-              w[k] = pack_bf16x2(a - __uint_as_float(v[k] << 16), b - __uint_as_float(v[k] & 0xffff0000u));
-            }
-            *reinterpret_cast<uint4*>(p.out + at + c + i) = make_uint4(v[0], v[1], v[2], v[3]);
-            if (p.out_lo) *reinterpret_cast<uint4*>(p.out_lo + at + c + i) = make_uint4(w[0], w[1], w[2], w[3]);
+          for (int k = 0; k < 8; ++k) {
+            const float a = __uint_as_float(r[2 * k]) * inv, b = __uint_as_float(r[2 * k + 1]) * inv;
+            v[k] = pack_bf16x2(a, b);
+            lo[k] = pack_bf16x2(a - __uint_as_float(v[k] << 16), b - __uint_as_float(v[k] & 0xffff0000u));
           }
+          store_32_bytes(p.out + at + c, v);
+          if (p.out_lo) store_32_bytes(p.out_lo + at + c, lo);
         }
       }
       tc_fence_before();                           // these reads of O come before the next item's first product (via p_full)
-      if (qi < p.Sq) {
+      if (qi < p.Sq && half == 0) {
         const long long stat = (static_cast<long long>(it.batch) * p.Hq + head) * p.Sq + qi;
         if (p.lse2) p.lse2[stat] = l_run > 0.f ? m_run + log2f(l_run) : -INFINITY;
         if (LSE) p.lse[stat] = x_run > 0.f ? (m_run + log2f(x_run)) * kWfLn2 : -INFINITY;
@@ -464,17 +480,11 @@ window_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
 template <int D, bool LSE>
 static int launch_window_fwd(const CUtensorMap& tmQ, const CUtensorMap& tmK, const CUtensorMap& tmV, const WindowFwdArgs& args,
                              cudaStream_t stream) {
-  constexpr size_t smem = 1024 + (2 + kWfStages) * (kWinBlock * D * 2) + 256;
+  constexpr size_t smem = (2 + kWfStages) * (kWinBlock * D * 2) + 256 + 4 * kWinBlock * sizeof(float);
   static bool configured[64] = {false};
   int dev = 0;
   MB_CHECK_CUDA(cudaGetDevice(&dev));
   if (!configured[dev & 63]) {
-    cudaFuncAttributes at;
-    MB_CHECK_CUDA(cudaFuncGetAttributes(&at, window_fwd_kernel<D, LSE>));
-    if (at.numRegs != kWfLaunchRegs) {             // the split of the register file is made for this launch size
-      set_last_error("mb_window_attn_fwd: built with another register count than the register split assumes");
-      return -6;
-    }
     MB_CHECK_CUDA(cudaFuncSetAttribute(window_fwd_kernel<D, LSE>, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem)));
     configured[dev & 63] = true;
   }
@@ -571,6 +581,10 @@ MB_API int mb_window_attn_fwd(const void* q, long long q_tstride, long long q_bs
   if (const char* what = window_attn_problem(B, Sq, Sk, Hq, Hkv, D, window, sinks, strides, 6, pointers, 5)) {
     set_last_error(what);
     return -1;
+  }
+  if ((reinterpret_cast<uintptr_t>(out) | reinterpret_cast<uintptr_t>(out_lo)) & 31) {
+    set_last_error("mb_window_attn_fwd: outputs must be 32-byte aligned");
+    return -3;
   }
   int* status = status_ptr();
   if (!status) return -4;
