@@ -58,6 +58,9 @@ __device__ __forceinline__ uint32_t window_bits(const WindowRow& w, int key0) {
 struct WindowTile {
   int sa, ea, b0, b1;
   int full_lo, full_hi;
+  int lo, last, far, far_end;   // keys that some row sees: [lo, last] and [far, far_end)
+  // whether some row sees a key of the 64 from `key0`
+  __device__ __forceinline__ bool sees64(int key0) const { return (key0 <= last && key0 + 63 >= lo) || (key0 < far_end && key0 + 63 >= far); }
   __device__ __forceinline__ int count() const { return (ea - sa) + (b1 - b0); }
   __device__ __forceinline__ bool has(int blk) const { return (blk >= sa && blk < ea) || (blk >= b0 && blk < b1); }
   __device__ __forceinline__ int block(int n) const { return n < ea - sa ? sa + n : b0 + n - (ea - sa); }
@@ -67,6 +70,7 @@ __device__ __forceinline__ WindowTile window_tile(const WindowRule& r, int batch
   WindowTile t;
   t.sa = t.ea = t.b0 = t.b1 = 0;
   t.full_lo = kWinNone, t.full_hi = -1;
+  t.lo = t.far = kWinNone, t.last = t.far_end = -1;
   const int off = Sk - Sq;
   const int first = q0 + off, p1 = min(q0 + kWinBlock, Sq) - 1 + off;
   if (q0 >= Sq || p1 < 0) return t;
@@ -99,6 +103,7 @@ __device__ __forceinline__ WindowTile window_tile(const WindowRule& r, int batch
   t.sa = start / kWinBlock;
   t.ea = min((min(start + r.sinks, lo) + kWinBlock - 1) / kWinBlock, t.b0);
   if (t.ea <= t.sa) t.sa = t.ea = 0;
+  t.lo = lo, t.last = last, t.far = start, t.far_end = min(start + r.sinks, lo);
   if (whole) t.full_lo = lo_max, t.full_hi = p0;
   return t;
 }

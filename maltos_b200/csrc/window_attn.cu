@@ -3,11 +3,12 @@
 // softmax of one tile runs under the matrix products of the other:
 //   warp 0       TMA producer: the tiles' queries and a ring of K and V blocks,
 //   warps 1, 2   one per tile: issue S = Q K^T and O += P V as UMMAs; S, P and O stay in tensor memory (P overwrites the scores it
-//                came from). A wait that is already satisfied still costs up to 250 cycles while UMMAs saturate shared memory, so
-//                each tile has an issuer of its own and no barrier is asked twice,
-//   warps 3-18   eight per tile, two threads per query row with 64 keys of a block each: running maximum and sum, P in bf16, output.
-//                With one thread per row a scheduler has one warp of a tile to run, which takes 14 cycles an exponential where
-//                the special-function unit needs 8; the price of two is an exchange of their maxima in every block.
+//                came from),
+//   warps 3-18   eight per tile, two threads per query row with 32 keys each: running maximum and sum, P in bf16, output.
+// A block's keys are worked on in two halves of 64 with buffers of their own, so that a tile hides its products itself: while the
+// arithmetic is at one half, O += P V of the other and the other's next scores are formed. (With whole blocks a tile alternates
+// between 2600 cycles of arithmetic and 1800 of products and their waits, and the two tiles hide only part of that from one
+// another: 4400 cycles for the pair, of 2048 of UMMAs.) Halves of which no row sees a key are left out.
 // The two tiles are two query heads of one key/value head on the same rows where the group is even, else neighbouring rows of
 // one head. O is rescaled only when a row's maximum has grown by more than 2^8 since the last rescale: P then stays below 2^8
 // and its bf16 rounding is relative, so nothing is lost, and after the first blocks the rescale hardly ever happens.
@@ -102,13 +103,12 @@ window_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
   uint64_t* bars = reinterpret_cast<uint64_t*>(sKV + kWfStages * TILE_BYTES);
   uint64_t* q_full = bars;                         // 2
   uint64_t* q_empty = bars + 2;                    // 2
-  uint64_t* s_full = bars + 4;                     // 2
-  uint64_t* p_full = bars + 6;                     // 2
-  uint64_t* o_full = bars + 8;                     // 2
-  uint64_t* kv_full = bars + 10;                   // kWfStages
+  uint64_t* s_full = bars + 4;                     // 2 tiles x 2 halves
+  uint64_t* p_full = bars + 8;                     // 2 x 2
+  uint64_t* o_done = bars + 12;                    // 2 x 2: the tile's product k (odd, even) is in O; two may be on their way
+  uint64_t* kv_full = bars + 16;                   // kWfStages
   uint64_t* kv_empty = kv_full + kWfStages;        // kWfStages
-  uint64_t* turn = kv_empty + kWfStages;           // 2: the exponentials of a block are tile t's turn
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(turn + 2);
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(kv_empty + kWfStages);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   float* exchange = reinterpret_cast<float*>(smem + (2 + kWfStages) * TILE_BYTES + 256);   // [tile][half][row]
 
@@ -124,10 +124,11 @@ window_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
     for (int t = 0; t < 2; ++t) {
       mbar_init(&q_full[t], 1);
       mbar_init(&q_empty[t], 1);
-      mbar_init(&s_full[t], 1);
-      mbar_init(&p_full[t], 8);
-      mbar_init(&o_full[t], 1);
-      mbar_init(&turn[t], 8);
+      for (int h = 0; h < 2; ++h) {
+        mbar_init(&s_full[2 * t + h], 1);
+        mbar_init(&p_full[2 * t + h], 8);
+        mbar_init(&o_done[2 * t + h], 1);
+      }
     }
     for (int i = 0; i < kWfStages; ++i) {
       mbar_init(&kv_full[i], 1);
@@ -198,16 +199,16 @@ window_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
       }
     } else {
       // ---------------------------------------------------------------- UMMA issuer of tile t
-      // Step u: O += P V of block u - 1, then the scores of block u over that P. The scores' commit therefore also says that the
-      // product before them is complete, which is what a rescale of O waits for.
+      // Step (u, h): O += P V of what half h holds from block u - 1, then the scores of half h of block u in its place. The products
+      // thus come in the order of the arithmetic, none later than one block after its scores.
       const int t = warp - 1;
-      const uint32_t idesc_qk = make_idesc_bf16(kWinBlock, kWinBlock, 0, 0);
+      const uint32_t idesc_qk = make_idesc_bf16(kWinBlock, 64, 0, 0);
       const uint32_t idesc_pv = make_idesc_bf16(kWinBlock, D, 0, 1);
       constexpr uint32_t hi = smem_desc_hi_sw128(1024);
       const uint32_t s_tmem = tmem_base + S_COL + static_cast<uint32_t>(t) * 128u, o_tmem = tmem_base + O_COL + static_cast<uint32_t>(t) * 128u;
       const uint32_t q_lo = smem_desc_lo(smem_u32(sQ + t * TILE_BYTES), 16);
       int ring = 0, ring_round = 0;                // position of the block's K in the ring
-      uint32_t p_phase = 0, q_phase = 0;
+      uint32_t p_phase[2] = {0, 0}, q_phase = 0, products = 0;
       bool ok = true;
       for (int item = blockIdx.x; item < p.items; item += gridDim.x) {
         WindowItem it;
@@ -216,12 +217,12 @@ window_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
         if (lane == 0) {
           const WindowTile tile = t ? it.tile[1] : it.tile[0];
           int left = tile.count();                 // blocks whose scores are not issued yet
-          bool pending = false, begun = false, has_o = false;
+          bool pending[2] = {false, false}, begun = false, has_o = false;
           int vs = 0, v_round = 0;                 // ring position of V of the block before
           for (int u = 0; u <= it.n; ++u) {
-            const int ks = ring;
-            const bool mine = u < it.n && tile.has(it.block(u));
-            // what was loaded long ago is waited for first, the only wait that matters (for P) comes last
+            const int ks = ring, blk = u < it.n ? it.block(u) : 0;
+            const bool mine = u < it.n && tile.has(blk), used = pending[0] || pending[1];
+            // what was loaded long ago is waited for first, the waits that matter (for P) come last
             ok = (u == 0 || mbar_wait(&kv_full[vs], v_round & 1, abort_flag)) && (u == it.n || mbar_wait(&kv_full[ks], ring_round & 1, abort_flag));
             if (!ok) break;
             if (mine && !begun) {
@@ -230,39 +231,46 @@ window_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
               ++q_phase;
               begun = true;
             }
-            if (pending) {
-              const uint32_t v_lo = smem_desc_lo(smem_u32(sKV + vs * TILE_BYTES), ATOM_BYTES);
-              const uint32_t acc0 = has_o ? 1u : 0u;
-              ok = mbar_wait(&p_full[t], p_phase & 1, abort_flag);
-              if (!ok) break;
-              tc_fence_after();
+            const uint32_t v_lo = smem_desc_lo(smem_u32(sKV + vs * TILE_BYTES), ATOM_BYTES), k_lo = smem_desc_lo(smem_u32(sKV + ks * TILE_BYTES), 16);
 #pragma unroll
-              for (int kk = 0; kk < kWinBlock / 16; ++kk)   // the 64 keys of a half sit packed in the first 32 of their 64 columns
-                umma_bf16_ts_lh(o_tmem, s_tmem + static_cast<uint32_t>((kk >> 2) * 64 + (kk & 3) * 8), v_lo + static_cast<uint32_t>(kk * 128), hi,
-                                idesc_pv, kk != 0 ? 1u : acc0);
-              ++p_phase;
-              has_o = true;
-            }
-            if (mine) {
-              tc_fence_after();
-              const uint32_t k_lo = smem_desc_lo(smem_u32(sKV + ks * TILE_BYTES), 16);
+            for (int h = 0; h < 2; ++h) {
+              if (pending[h]) {
+                ok = ok && mbar_wait(&p_full[2 * t + h], p_phase[h] & 1, abort_flag);
+                if (!ok) continue;
+                ++p_phase[h];
+                tc_fence_after();
+                const uint32_t acc0 = has_o ? 1u : 0u;
 #pragma unroll
-              for (int kk = 0; kk < D / 16; ++kk) {
-                const uint32_t off = static_cast<uint32_t>(((kk >> 2) * ATOM_BYTES + (kk & 3) * 32) >> 4);
-                umma_bf16_ss_lh(s_tmem, q_lo + off, hi, k_lo + off, hi, idesc_qk, kk != 0 ? 1u : 0u);
+                for (int k2 = 0; k2 < 4; ++k2)     // the 32 keys of a thread sit packed in the first 16 of their 32 columns
+                  umma_bf16_ts_lh(o_tmem, s_tmem + static_cast<uint32_t>(h * 64 + (k2 >> 1) * 32 + (k2 & 1) * 8),
+                                  v_lo + static_cast<uint32_t>((h * 4 + k2) * 128), hi, idesc_pv, k2 != 0 ? 1u : acc0);
+                umma_commit(&o_done[2 * t + (products++ & 1)]);
+                has_o = true;
+                pending[h] = false;
               }
-              umma_commit(&s_full[t]);
+              if (mine && tile.sees64(blk * kWinBlock + h * 64)) {
+                tc_fence_after();
+#pragma unroll
+                for (int kk = 0; kk < D / 16; ++kk) {
+                  const uint32_t off = static_cast<uint32_t>(((kk >> 2) * ATOM_BYTES + (kk & 3) * 32) >> 4);
+                  umma_bf16_ss_lh(s_tmem + static_cast<uint32_t>(h * 64), q_lo + off, hi, k_lo + off + static_cast<uint32_t>(h * (64 * 128 >> 4)), hi,
+                                  idesc_qk, kk != 0 ? 1u : 0u);
+                }
+                umma_commit(&s_full[2 * t + h]);
+                pending[h] = true;
+              }
+            }
+            if (!ok) break;
+            if (mine) {
               umma_commit(&kv_empty[ks]);
               if (--left == 0) umma_commit(&q_empty[t]);
             } else if (u < it.n) {
               mbar_arrive(&kv_empty[ks]);          // the other tile's block
             }
             if (u > 0) {
-              if (pending) umma_commit(&kv_empty[vs]);
+              if (used) umma_commit(&kv_empty[vs]);
               else mbar_arrive(&kv_empty[vs]);
-              if (pending && !mine && left == 0) umma_commit(&o_full[t]);
             }
-            pending = mine;
             if (u < it.n) {
               if (++ring == kWfStages) ring = 0, ++ring_round;
               vs = ring, v_round = ring_round;
@@ -277,28 +285,30 @@ window_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
     __syncwarp();
   } else {
     // ------------------------------------------------------------------ softmax and output: two threads per query row
-    const int t = (warp - 3) >> 3, half = ((warp - 3) >> 2) & 1;
+    const int t = (warp - 3) >> 3, half = ((warp - 3) >> 2) & 1;   // half: which 32 of a buffer's 64 keys, which half of O's columns
     const int row = (warp & 3) * 32 + lane;
     const uint32_t t_lane = static_cast<uint32_t>((warp & 3) * 32) << 16;
-    const uint32_t s_tmem = tmem_base + S_COL + static_cast<uint32_t>(t * 128 + half * 64) + t_lane;
+    const uint32_t s_tmem = tmem_base + S_COL + static_cast<uint32_t>(t * 128 + half * 32) + t_lane;
     constexpr int HALF_D = D / 2;                  // columns of O that this thread rescales and stores
     const uint32_t o_tmem = tmem_base + O_COL + static_cast<uint32_t>(t * 128 + half * HALF_D) + t_lane;
     // The two threads of a row exchange a value through shared memory and a barrier of their two warps. NaN says that a wait of
     // one of them ran out: both then leave at the same place, so that neither is left behind at the barrier (a maximum is never
     // NaN, and a sum that is NaN stops nothing but the output loop of its own rows, for which `stop` is not looked at).
-    // A slot is written again only after the partner has read it: between two blocks that follows from the P of both, which the
-    // next scores wait for; at the end of an item the barrier is passed once more.
     float* slot = exchange + (t * 2 + half) * kWinBlock + row;
-    const float* partner = exchange + (t * 2 + (half ^ 1)) * kWinBlock + row;
+    const volatile float* partner = exchange + (t * 2 + (half ^ 1)) * kWinBlock + row;
     auto pair_barrier = [&] { asm volatile("bar.sync %0, 64;" ::"r"(1 + t * 4 + (warp & 3)) : "memory"); };
     auto swap = [&](float mine) {
       *slot = mine;
       pair_barrier();
-      return *const_cast<const volatile float*>(partner);
+      const float theirs = *partner;
+      pair_barrier();                              // both have read: the slot may be written again
+      return theirs;
     };
-    int s_count = 0, o_count = 0;
-    uint32_t turn_phase = 0;
-    bool owed = false;                             // tile 0: the other tile had its last block too, and hands the turn back
+    uint32_t s_phase[2] = {0, 0}, products = 0;    // products: of this tile so far, its halves in all items
+    auto product_done = [&] {                      // the last one
+      const bool there = mbar_wait(&o_done[2 * t + ((products - 1) & 1)], ((products - 1) >> 1) & 1, abort_flag);
+      return __all_sync(0xffffffffu, there) != 0;
+    };
     bool ok = true, stop = false;
     for (int item = blockIdx.x; item < p.items; item += gridDim.x) {
       WindowItem it;
@@ -306,81 +316,71 @@ window_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
       const int q0 = it.q0[t], head = it.head[t];
       if (q0 >= p.Sq) continue;                    // the missing second tile
       const WindowTile tile = window_tile(p.rule, it.batch, p.Sq, p.Sk, q0);
-      const WindowTile other = p.pair == 1 ? tile : window_tile(p.rule, it.batch, p.Sq, p.Sk, it.q0[t ^ 1]);
-      const bool paired = p.pair != 0;
       const int n = tile.count();
       const int qi = q0 + row;
       const WindowRow w = window_row(p.rule, it.batch, p.Sk, qi + p.Sk - p.Sq, qi < p.Sq);
-      // m_run: the power of two that P is relative to; l_run: this half's sum of the rounded P; x_run: of P as it was before
+      // m_run: the power of two that P is relative to; l_run: this thread's sum of the rounded P; x_run: of P as it was before
       float m_run = -INFINITY, l_run = 0.f, x_run = 0.f;
+      bool first = true;
       for (int j = 0; j < n; ++j) {
-        ok = ok && mbar_wait(&s_full[t], s_count & 1, abort_flag);
-        ok = __all_sync(0xffffffffu, ok);
-        ++s_count;
-        tc_fence_after();
-        const int blk = tile.block(j), key0 = blk * kWinBlock + half * 64;
-        // The scores are read twice rather than kept: 32 of them at a time, the second chunk last, so that it is still there after
-        // the maximum.
-        uint32_t s[32], seen[2] = {0xffffffffu, 0xffffffffu};
-        float m_blk = -INFINITY;
-        if (blk * kWinBlock < tile.full_lo || blk * kWinBlock + kWinBlock - 1 > tile.full_hi)
-          seen[0] = window_bits(w, key0), seen[1] = window_bits(w, key0 + 32);
-        auto read = [&](int c) {
-          tmem_ld_32x32b_x32(s_tmem + c * 32, s);
-          tmem_ld_wait();
-          if (__any_sync(0xffffffffu, seen[c] != 0xffffffffu)) {
+        const int blk0 = tile.block(j) * kWinBlock;
+        const bool edge = blk0 < tile.full_lo || blk0 + kWinBlock - 1 > tile.full_hi;
 #pragma unroll
-            for (int i = 0; i < 32; ++i)
-              if (!((seen[c] >> i) & 1u)) s[i] = __float_as_uint(-INFINITY);
-          }
-        };
-        if (ok) {
-          float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+        for (int h = 0; h < 2; ++h) {
+          if (stop || !tile.sees64(blk0 + h * 64)) continue;
+          ok = ok && mbar_wait(&s_full[2 * t + h], s_phase[h] & 1, abort_flag);
+          ok = __all_sync(0xffffffffu, ok);
+          ++s_phase[h];
+          tc_fence_after();
+          uint32_t s[32], seen = 0xffffffffu;
+          float m_blk = -INFINITY;
+          if (ok) {
+            tmem_ld_32x32b_x32(s_tmem + h * 64, s);
+            if (edge) seen = window_bits(w, blk0 + h * 64 + half * 32);
+            tmem_ld_wait();
+            if (__any_sync(0xffffffffu, seen != 0xffffffffu)) {
 #pragma unroll
-          for (int c = 0; c < 2; ++c) {
-            read(c);
+              for (int i = 0; i < 32; ++i)
+                if (!((seen >> i) & 1u)) s[i] = __float_as_uint(-INFINITY);
+            }
+            float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
             for (int i = 0; i < 32; i += 8)
 #pragma unroll
               for (int k = 0; k < 4; ++k) mx[k] = fmaxf(fmaxf(mx[k], __uint_as_float(s[i + 2 * k])), __uint_as_float(s[i + 2 * k + 1]));
+            m_blk = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * p.scale_log2;
           }
-          m_blk = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * p.scale_log2;
-        }
-        const float m_other = swap(ok ? m_blk : NAN);
-        stop = __any_sync(0xffffffffu, !ok || m_other != m_other);
-        if (stop) break;
-        m_blk = fmaxf(m_blk, m_other);
-        if (__any_sync(0xffffffffu, m_blk > m_run + kWfGrowth)) {   // the same for the two warps of these rows
-          const float m_new = fmaxf(m_run, ceilf(m_blk));
-          const float alpha = m_run == -INFINITY ? 0.f : wf_exp2(m_run - m_new);   // a power of two
-          m_run = m_new;
-          l_run *= alpha;
-          if (LSE) x_run *= alpha;
-          if (j > 0) {
+          const float m_other = swap(ok ? m_blk : NAN);
+          stop = __any_sync(0xffffffffu, !ok || m_other != m_other);
+          if (stop) continue;
+          m_blk = fmaxf(m_blk, m_other);
+          if (__any_sync(0xffffffffu, m_blk > m_run + kWfGrowth)) {   // the same for the two warps of these rows
+            const float m_new = fmaxf(m_run, ceilf(m_blk));
+            const float alpha = m_run == -INFINITY ? 0.f : wf_exp2(m_run - m_new);   // a power of two
+            m_run = m_new;
+            l_run *= alpha;
+            if (LSE) x_run *= alpha;
+            if (!first) {                          // once the product before is in O (a wait that runs out is acted on at the next exchange)
+              ok = product_done();
+              tc_fence_after();
 #pragma unroll 1
-            for (int c = 0; c < HALF_D; c += 16) {
-              uint32_t r[16];
-              tmem_ld_32x32b_x16(o_tmem + c, r);
-              tmem_ld_wait();
+              for (int c = 0; c < HALF_D; c += 16) {
+                uint32_t r[16];
+                tmem_ld_32x32b_x16(o_tmem + c, r);
+                tmem_ld_wait();
 #pragma unroll
-              for (int i = 0; i < 16; ++i) r[i] = __float_as_uint(__uint_as_float(r[i]) * alpha);
-              tmem_st_32x32b_x16(o_tmem + c, r);
+                for (int i = 0; i < 16; ++i) r[i] = __float_as_uint(__uint_as_float(r[i]) * alpha);
+                tmem_st_32x32b_x16(o_tmem + c, r);
+              }
             }
           }
-        }
-        // The two tiles take turns with their exponentials: block by block, tile 0 first. Left alone they fall into step, both on
-        // the exponentials and then both on the tensor cores, and neither is hidden.
-        const bool both = paired && other.has(blk);
-        if (t == 0 ? owed : both) {
-          ok = mbar_wait(&turn[t], turn_phase & 1, abort_flag);   // a wait that runs out is acted on at the next exchange
-          ++turn_phase;
-        }
-        const float m_safe = m_run == -INFINITY ? 0.f : m_run;
-        const uint64_t scale2 = f32x2(p.scale_log2, p.scale_log2), shift2 = f32x2(-m_safe, -m_safe);
-        uint64_t sum[2] = {0, 0}, sum_x[2] = {0, 0};
-        uint32_t pk[16];
-        auto weights = [&](int c) {                // P of the chunk in s
-          if (__any_sync(0xffffffffu, seen[c] != 0u)) {
+          first = false;
+          ++products;
+          const float m_safe = m_run == -INFINITY ? 0.f : m_run;
+          const uint64_t scale2 = f32x2(p.scale_log2, p.scale_log2), shift2 = f32x2(-m_safe, -m_safe);
+          uint64_t sum[2] = {0, 0}, sum_x[2] = {0, 0};
+          uint32_t pk[16];
+          if (__any_sync(0xffffffffu, seen != 0u)) {
 #pragma unroll
             for (int i = 0; i < 16; ++i) {
               float a, b;
@@ -390,45 +390,33 @@ window_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
               sum[i & 1] = add_f32x2(sum[i & 1], bf16x2_as_f32x2(pk[i]));
               if (LSE) sum_x[i & 1] = add_f32x2(sum_x[i & 1], f32x2(a, b));
             }
-          } else {                                 // no row of the warp sees a key of this chunk
+          } else {                                 // no row of the warp sees one of its keys
 #pragma unroll
             for (int i = 0; i < 16; ++i) pk[i] = 0u;
           }
-        };
-        weights(1);
-        read(0);                                   // before its scores are overwritten
-        tmem_st_32x32b_x16(s_tmem + 16, pk);
-        weights(0);
-        tmem_st_32x32b_x16(s_tmem, pk);
-        // one arrival and one wait each way for every block that both have, so neither barrier gets two phases ahead
-        owed = both;
-        if (both && lane == 0) mbar_arrive(&turn[t ^ 1]);
-        tmem_st_wait();
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&p_full[t]);
-        float lo, hi;
-        f32x2_split(add_f32x2(sum[0], sum[1]), lo, hi);
-        l_run += lo + hi;
-        if (LSE) {
-          f32x2_split(add_f32x2(sum_x[0], sum_x[1]), lo, hi);
-          x_run += lo + hi;
+          tmem_st_32x32b_x16(s_tmem + h * 64, pk);
+          float lo, hi;
+          f32x2_split(add_f32x2(sum[0], sum[1]), lo, hi);
+          l_run += lo + hi;
+          if (LSE) {
+            f32x2_split(add_f32x2(sum_x[0], sum_x[1]), lo, hi);
+            x_run += lo + hi;
+          }
+          tmem_st_wait();
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&p_full[2 * t + h]);
         }
+        if (stop) break;
       }
       if (stop) break;
       // ---------------------------------------------------------------- output
       if (n > 0) {
-        ok = ok && mbar_wait(&o_full[t], o_count & 1, abort_flag);
-        ok = __all_sync(0xffffffffu, ok);
-        ++o_count;
+        ok = ok && product_done();
         tc_fence_after();
       }
       l_run += swap(l_run);
-      pair_barrier();
-      if (LSE) {
-        x_run += swap(x_run);
-        pair_barrier();
-      }
+      if (LSE) x_run += swap(x_run);
       const float inv = l_run > 0.f ? 1.f / l_run : 0.f;
       const long long at = ((static_cast<long long>(it.batch) * p.Sq + qi) * p.Hq + head) * D + half * HALF_D;
 #pragma unroll 1
