@@ -21,6 +21,7 @@ struct Vec {
   static constexpr int kPieces = N == 1 ? 1 : static_cast<int>(N * sizeof(T) / 16);
   union {
     uint4 piece[kPieces];
+    uint32_t word[4 * kPieces];
     T at[N];
   };
   __device__ __forceinline__ Vec() {}
@@ -47,6 +48,10 @@ struct Vec {
                      : "=r"(piece[i].x), "=r"(piece[i].y), "=r"(piece[i].z), "=r"(piece[i].w)
                      : "l"(reinterpret_cast<const uint4*>(p) + i));
     }
+  }
+  __device__ __forceinline__ void load_shared(const T* p) {
+#pragma unroll
+    for (int i = 0; i < kPieces; ++i) piece[i] = reinterpret_cast<const uint4*>(p)[i];
   }
   __device__ __forceinline__ void store(T* p) const {
     if constexpr (N == 1) {

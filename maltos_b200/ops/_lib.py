@@ -113,7 +113,7 @@ _PROTOTYPES = {
     "mb_embedding_bwd_scratch_words": "li",
     "mb_embedding_bwd": "pippp" "ilill" "fp",
     "mb_block_norm_fwd": "pppppi" "pppp" "ili" "ffp",
-    "mb_block_norm_bwd_parts": "li",
+    "mb_block_norm_bwd_parts": "ili",
     "mb_block_norm_bwd": "ppppppp" "i" "ppppppp" "pp" "ili" "fp",
 }
 _KINDS = {"p": c_void_p, "l": c_ll, "i": c_int, "f": c_float}

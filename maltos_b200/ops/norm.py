@@ -149,7 +149,7 @@ class _BlockNorm(torch.autograd.Function):
         dw1, dw2, dg = (None if t is None else torch.empty_like(t) for t in (w1, w2, g))
         L = _lib.lib()
         with _lib.on_device_of(some):
-            size = L.mb_block_norm_bwd_parts(rows, H) * H
+            size = L.mb_block_norm_bwd_parts(_BLOCK_DTYPES[some.dtype], rows, H) * H
             parts = torch.empty(2 * size, dtype=torch.float32, device=some.device)
             r1, part = stats.data_ptr(), parts.data_ptr()
             _lib.check(L.mb_block_norm_bwd(a(dy), a(dh), a(x), a(h), a(w1), a(w2), a(g), mode, r1, r1 + 4 * rows, dx.data_ptr(), dres.data_ptr(),

@@ -6,6 +6,9 @@
     python -m maltos_b200.tools.bench_kernels swiglu --rows 65536 --hidden 14336
     python -m maltos_b200.tools.bench_kernels adamw --numel 500000000
     python -m maltos_b200.tools.bench_kernels attention --seq 8192 --heads 32 --kv-heads 8
+    python -m maltos_b200.tools.bench_kernels window-attention --seq 8192 --window 1024 --sinks 4
+    python -m maltos_b200.tools.bench_kernels embedding --rows 32768 --hidden 4096 --vocab 128256
+    python -m maltos_b200.tools.bench_kernels block-norm --rows 8192 --hidden 4096 --gate channel
 
 Every line reports the achieved rate and, where ``--peaks MEASURED_PEAKS.json`` is given, the fraction of the measured
 copy bandwidth / cuBLAS throughput of the machine. Small ``--iters`` runs are what profiler captures are taken from.
@@ -14,6 +17,7 @@ from __future__ import annotations
 
 import argparse
 import json
+import math
 from pathlib import Path
 
 import torch
@@ -39,6 +43,20 @@ def _time(fn, iters: int, warmup: int = 3, flush: torch.Tensor | None = None) ->
         end.synchronize()
         times.append(start.elapsed_time(end))
     return sorted(times)[len(times) // 2]
+
+
+def _recorded(fn):
+    """``fn`` as the replay of a CUDA graph: its launches without the host's part of them, which is longer than small kernels."""
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        for _ in range(2):
+            fn()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        fn()
+    return graph.replay
 
 
 def _peaks(path: str | None) -> dict:
@@ -205,6 +223,83 @@ def bench_attention(args) -> None:
     _lib.fetch_status()
 
 
+def bench_window_attention(args) -> None:
+    """Sliding-window attention: forward, backward and (one query a row) the forward of a single token."""
+    from maltos_b200.ops import _lib
+    from maltos_b200.ops.attention import sliding_window_attention
+
+    B, S, Hq, Hkv, D, W, sinks = args.batch, args.seq, args.heads, args.kv_heads, args.head_dim, args.window, args.sinks
+    Sq = args.queries or S
+    g = torch.Generator(device="cuda").manual_seed(0)
+    q = torch.randn(B, Sq, Hq, D, device="cuda", generator=g).bfloat16()
+    k, v = (torch.randn(B, S, Hkv, D, device="cuda", generator=g).bfloat16() for _ in range(2))
+    dout = torch.randn(B, Sq, Hq, D, device="cuda", generator=g).bfloat16()
+    ids = None
+    if args.documents:
+        ids = (torch.arange(S, device="cuda") * args.documents // S).expand(B, S)
+    p = torch.arange(S - Sq, S, dtype=torch.int64)
+    start = torch.zeros_like(p) if ids is None else torch.searchsorted(ids[0].cpu(), ids[0].cpu()[p])
+    seen = p - start + 1
+    pairs = int(torch.minimum(seen, W + torch.clamp(torch.minimum(seen - W, torch.full_like(seen, sinks)), min=0)).sum()) * B * Hq
+    flush = torch.empty(256 << 20, dtype=torch.uint8, device="cuda")
+    tag = f"B{B} S{Sq}/{S} h{Hq}/{Hkv} D{D} window {W} first {sinks}" + (f" documents {args.documents}" if ids is not None else "")
+    call = dict(window=W, sinks=sinks, sequence_ids=ids)
+
+    def report(what: str, ms: float, products: int) -> None:
+        flops = 2.0 * products * pairs * D
+        peak = _peaks(args.peaks).get("bf16_tflops")
+        print(f"window attention {what} {tag}: {ms * 1e3:8.1f} us  {flops / ms / 1e9:7.1f} TFLOP/s" +
+              (f"  {flops / ms / 1e9 / peak:.2f} of measured cuBLAS" if peak else ""))
+
+    with torch.no_grad():
+        report("fwd    ", _time(_recorded(lambda: sliding_window_attention(q, k, v, **call)), args.iters, flush=flush), 2)
+    leaves = [t.requires_grad_() for t in (q, k, v)]
+    report("fwd+bwd", _time(_recorded(lambda: torch.autograd.grad(sliding_window_attention(q, k, v, **call), leaves, dout)), args.iters, flush=flush), 7)
+    _lib.fetch_status()
+
+
+def bench_embedding(args) -> None:
+    from maltos_b200.ops import _lib
+    from maltos_b200.ops.embedding import embedding
+
+    T, H, V = args.rows, args.hidden, args.vocab
+    g = torch.Generator(device="cuda").manual_seed(0)
+    weight = torch.randn(V, H, device="cuda", generator=g).bfloat16()
+    # frequencies that fall with the rank, ranks spread over the table
+    ids = ((torch.rand(T, device="cuda", generator=g) * math.log(V)).exp().long().clamp_(1, V) - 1) * 40503 % V
+    dout = torch.randn(T, H, device="cuda", generator=g).bfloat16()
+    flush = torch.empty(256 << 20, dtype=torch.uint8, device="cuda")
+    peaks, used = _peaks(args.peaks), int(ids.unique().numel())
+    with torch.no_grad():
+        _report_bw(f"embedding fwd {T} tokens of [{V},{H}]", (used + T) * H * 2, _time(_recorded(lambda: embedding(ids, weight, scale=2.0)), args.iters, flush=flush), peaks)
+    weight.requires_grad_()
+    _report_bw(f"embedding fwd+bwd {T} tokens of [{V},{H}]", (used + 2 * T + V) * H * 2,
+               _time(_recorded(lambda: torch.autograd.grad(embedding(ids, weight, scale=2.0), weight, dout)), args.iters, flush=flush), peaks)
+    _lib.fetch_status()
+
+
+def bench_block_norm(args) -> None:
+    from maltos_b200.ops import _lib
+    from maltos_b200.ops.norm import block_norm
+
+    rows, H = args.rows, args.hidden
+    g = torch.Generator(device="cuda").manual_seed(0)
+    x, r, dy, dh = (torch.randn(rows, H, device="cuda", generator=g).bfloat16() for _ in range(4))
+    w1, w2 = (torch.ones(H, device="cuda").bfloat16() for _ in range(2))
+    gate = {"none": None, "channel": torch.rand(H, device="cuda").bfloat16(),
+            "element": torch.rand(rows, H, device="cuda").bfloat16()}[args.gate]
+    flush = torch.empty(256 << 20, dtype=torch.uint8, device="cuda")
+    peaks, wide = _peaks(args.peaks), 1 if args.gate == "element" else 0
+    tag = f"[{rows},{H}] gate {args.gate}"
+    with torch.no_grad():
+        _report_bw(f"block norm fwd {tag}", (4 + wide) * rows * H * 2,
+                   _time(_recorded(lambda: block_norm(x, r, w1, w2, gate=gate, scale=0.5)), args.iters, flush=flush), peaks)
+    leaves = [t.requires_grad_() for t in (x, r, w1, w2, gate) if t is not None]
+    _report_bw(f"block norm fwd+bwd {tag}", (10 + 3 * wide) * rows * H * 2,
+               _time(_recorded(lambda: torch.autograd.grad(block_norm(x, r, w1, w2, gate=gate, scale=0.5), leaves, (dy, dh))), args.iters, flush=flush), peaks)
+    _lib.fetch_status()
+
+
 def main(argv=None) -> None:
     p = argparse.ArgumentParser(description=__doc__, formatter_class=argparse.RawDescriptionHelpFormatter)
     p.add_argument("--peaks", default="MEASURED_PEAKS.json", help="JSON with hbm_gbs / bf16_tflops of this machine")
@@ -228,6 +323,24 @@ def main(argv=None) -> None:
     t.add_argument("--head-dim", type=int, default=128)
     t.add_argument("--causal", action=argparse.BooleanOptionalAction, default=True)
     t.add_argument("--libraries", action=argparse.BooleanOptionalAction, default=True, help="also time the library kernels")
+    w = sub.add_parser("window-attention")
+    w.add_argument("--batch", type=int, default=1)
+    w.add_argument("--seq", type=int, default=8192)
+    w.add_argument("--queries", type=int, default=0, help="the last N tokens of the row ask (0: all of them)")
+    w.add_argument("--heads", type=int, default=32)
+    w.add_argument("--kv-heads", type=int, default=8)
+    w.add_argument("--head-dim", type=int, choices=(64, 128), default=128)
+    w.add_argument("--window", type=int, default=1024)
+    w.add_argument("--sinks", type=int, default=4)
+    w.add_argument("--documents", type=int, default=0, help="packed documents of equal length (0: one row, one document)")
+    e = sub.add_parser("embedding")
+    e.add_argument("--rows", type=int, default=32768, help="tokens")
+    e.add_argument("--hidden", type=int, default=4096)
+    e.add_argument("--vocab", type=int, default=128256)
+    b = sub.add_parser("block-norm")
+    b.add_argument("--rows", type=int, default=8192)
+    b.add_argument("--hidden", type=int, default=4096)
+    b.add_argument("--gate", choices=("none", "channel", "element"), default="none")
     a = sub.add_parser("adamw")
     a.add_argument("--numel", type=int, default=500_000_000)
     z = sub.add_parser("shard-paths")
@@ -237,6 +350,7 @@ def main(argv=None) -> None:
     if not torch.cuda.is_available():
         raise SystemExit("bench_kernels needs a CUDA device")
     {"gemm": bench_gemm, "rmsnorm": bench_rmsnorm, "swiglu": bench_swiglu, "adamw": bench_adamw, "attention": bench_attention,
+     "window-attention": bench_window_attention, "embedding": bench_embedding, "block-norm": bench_block_norm,
      "shard-paths": bench_shard_paths}[args.what](args)
 
 

@@ -214,6 +214,23 @@ def test_block_norm_rows(rows):
     _block_norm_case((rows, 2048), torch.float32, True, False, "channel", 0.1)
 
 
+# Many rows to each CTA of the backward, so that its ring of row pieces goes round several times: rings of many rows, of two, of one
+# and a part, of one, and rows that do not fit.
+@pytest.mark.parametrize("shape,dtype,gate", [
+    ((30000, 40), torch.bfloat16, "element"), ((70001, 264), torch.float16, None), ((5001, 1024), torch.bfloat16, "channel"),
+    ((1203, 4096), torch.float16, "element"), ((901, 5120), torch.bfloat16, "channel"), ((750, 8192), torch.bfloat16, "element"),
+    ((449, 8200), torch.bfloat16, None), ((450, 16384), torch.bfloat16, "element"), ((601, 4096), torch.float32, "element"),
+    ((450, 8192), torch.float32, "element"), ((447, 8200), torch.float32, "channel"), ((445, 16384), torch.float32, "element")])
+def test_block_norm_many_rows_to_a_cta(shape, dtype, gate):
+    _block_norm_case(shape, dtype, True, True, gate, 0.7)
+
+
+@pytest.mark.parametrize("after", [True, False])
+def test_block_norm_many_rows_without_the_second_norm(after):
+    _block_norm_case((2100, 2048), torch.bfloat16, after, False, "element", 0.7)
+    _block_norm_case((2100, 2048), torch.bfloat16, after, False, None, 0.7)
+
+
 @pytest.mark.parametrize("gate", [None, "channel", "element"])
 @pytest.mark.parametrize("after,before", [(True, True), (True, False), (False, True), (False, False)])
 @pytest.mark.parametrize("only", [None, "y", "h"])
