@@ -7,8 +7,9 @@
 //   window_bwd_dkdv_kernel    persistent; an item is 128 keys of one key/value head and a piece of the (query head, 128 query rows)
 //                             that see them. Transposed products S^T = K Q^T and dP^T = V dO^T (TMEM lane = key) leave P^T and dS^T
 //                             in tensor memory as the A operands of dV += P^T dO and dK += dS^T Q;
-//   window_bwd_join_kernel    adds up key blocks whose work was cut into pieces, in the pieces' order;
-//   window_bwd_dq_kernel      persistent; an item is 128 query rows of one head, S double-buffered, dS written over S.
+//   window_bwd_dq_kernel      persistent; an item is 128 query rows of one head, S double-buffered, dS written over S. At its end the
+//                             CTAs add up key blocks whose work was cut into pieces, in the pieces' order (in a launch of its own,
+//                             where a few blocks have all the pieces, that took 23 us of the layer's 570).
 // The keys of first tokens are seen by every later query, so a block that holds some has many times the work of the others; and
 // with few heads there are fewer blocks than SMs. Both are met by cutting a block's work into pieces. No atomics: the same bits
 // every time.
@@ -27,8 +28,8 @@ constexpr float kWbLog2e = 1.4426950408889634f;
 struct WindowBwdArgs {
   __nv_bfloat16 *dq, *dk, *dv;   // contiguous [B, S, H, D]
   const float *lse2, *delta;     // [B * Hq, Sq_pad]
-  const int* list;               // [0]: entries; from 4 on: int4 {block, first, one past the last iteration, slot or -1}
-  const int2* pieces;            // [B * key blocks] {first slot, pieces}; pieces 1: no slot
+  const int* list;               // [0]: entries, [1]: cut blocks; from 4 on: int4 {block, first, one past the last iteration, slot or -1}
+  const int4* cuts;              // [list[1]] {block, first slot, pieces, -}: blocks of more than one piece
   float* parts;                  // [slots, Hkv, 2 (dK, dV), 128, D]
   WindowRule rule;
   int B, Sq, Sk, Hq, Hkv, Sq_pad;
@@ -44,7 +45,7 @@ struct WindowBwdPrepArgs {
   const float* lse2_in;          // [B, Hq, Sq]
   float *lse2, *delta;
   int* list;
-  int2* pieces;
+  int4* cuts;
   WindowRule rule;
   int B, Sq, Sk, Hq, Hkv, Sq_pad, key_blocks;
   int piece;                     // iterations of a piece
@@ -99,12 +100,12 @@ constexpr int kWbPrepThreads = 1024;
 // The list of work: every key block's iterations, (query heads of the group) x (query tiles that see it), cut into pieces.
 __device__ void window_bwd_list(const WindowBwdPrepArgs& p) {
   __shared__ int warp_entries[32], warp_slots[32];
-  __shared__ int total_entries, total_slots;
+  __shared__ int total_entries, total_slots, total_cuts;
   __shared__ int found[kWbPrepThreads];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int blocks = p.B * p.key_blocks, group = p.Hq / p.Hkv;
   int4* entry = reinterpret_cast<int4*>(p.list + 4);
-  if (tid == 0) total_entries = total_slots = 0;
+  if (tid == 0) total_entries = total_slots = total_cuts = 0;
   __syncthreads();
   for (int base = 0; base < blocks; base += kWbPrepThreads) {
     // a block per thread; with documents a block's range is a warp's work, the blocks dealt out to the warps
@@ -142,17 +143,18 @@ __device__ void window_bwd_list(const WindowBwdPrepArgs& p) {
       if (tid == 0) total += all;
       __syncthreads();
     };
-    int slot = 0, at = 0;
+    int slot = 0, at = 0, cut = 0;
     scan(n > 1 ? n : 0, warp_slots, total_slots, slot);
     if (n > 1 && slot + n > p.max_slots) n = 1;    // the caller's bound says that this does not happen
     scan(n, warp_entries, total_entries, at);
+    scan(n > 1 ? 1 : 0, warp_slots, total_cuts, cut);
     if (mine < blocks) {
-      p.pieces[mine] = make_int2(slot, n);
+      if (n > 1) p.cuts[cut] = make_int4(mine, slot, n, 0);
       const int per = n > 1 ? p.piece : n_iter;
       for (int i = 0; i < n; ++i) entry[at + i] = make_int4(mine, i * per, min(n_iter, (i + 1) * per), n > 1 ? slot + i : -1);
     }
   }
-  if (tid == 0) p.list[0] = total_entries;
+  if (tid == 0) p.list[0] = total_entries, p.list[1] = total_cuts;
 }
 
 // CTA 0: the list. Others: delta and lse2, D / 8 lanes a row, rows in memory order.
@@ -563,26 +565,27 @@ window_bwd_dkdv_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_con
   }
 }
 
-// dK, dV of key blocks that were cut: one CTA per (block, key/value head), the pieces added in order.
+// Key blocks of several pieces: their sums, the work dealt out to all threads of the grid.
 template <int D>
-__global__ void __launch_bounds__(256) window_bwd_join_kernel(const WindowBwdArgs p) {
-  const int blk = blockIdx.x / p.Hkv, kv_head = blockIdx.x % p.Hkv;
-  const int2 pc = p.pieces[blk];
-  if (pc.y <= 1) return;
-  const int batch = blk / p.key_blocks, k0 = (blk % p.key_blocks) * kWinBlock;
-  for (int i = threadIdx.x + blockIdx.y * 256; i < 2 * kWinBlock * D / 4; i += 256 * gridDim.y) {
-    const int which = i / (kWinBlock * D / 4), row = i % (kWinBlock * D / 4) / (D / 4), c = i % (D / 4) * 4;
-    if (k0 + row >= p.Sk) continue;
+__device__ __forceinline__ void window_bwd_join(const WindowBwdArgs& p) {
+  constexpr long long kQuads = 2 * kWinBlock * D / 4;      // of a block and head: dK, then dV
+  const long long all = p.list[1] * static_cast<long long>(p.Hkv) * kQuads, step = static_cast<long long>(gridDim.x) * kWbThreads;
+  for (long long i = blockIdx.x * static_cast<long long>(kWbThreads) + threadIdx.x; i < all; i += step) {
+    const int e = static_cast<int>(i % kQuads), unit = static_cast<int>(i / kQuads), kv_head = unit % p.Hkv;
+    const int4 cut = p.cuts[unit / p.Hkv];
+    const int which = e / (kWinBlock * D / 4), row = e % (kWinBlock * D / 4) / (D / 4), c = e % (D / 4) * 4;
+    const int batch = cut.x / p.key_blocks, key = cut.x % p.key_blocks * kWinBlock + row;
+    if (key >= p.Sk) continue;
     float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
+    const float* part = p.parts + (static_cast<long long>(cut.y) * p.Hkv + kv_head) * 2 * kWinBlock * D + 4ll * e;
 #pragma unroll 4
-    for (int s = 0; s < pc.y; ++s) {
-      const float4 x = *reinterpret_cast<const float4*>(p.parts + ((static_cast<long long>(pc.x + s) * p.Hkv + kv_head) * 2 + which) * kWinBlock * D +
-                                                        row * D + c);
+    for (int s = 0; s < cut.z; ++s) {
+      const float4 x = *reinterpret_cast<const float4*>(part + s * (static_cast<long long>(p.Hkv) * 2 * kWinBlock * D));
       a.x += x.x, a.y += x.y, a.z += x.z, a.w += x.w;
     }
     uint2 v;
     v.x = pack_bf16x2(a.x, a.y), v.y = pack_bf16x2(a.z, a.w);
-    *reinterpret_cast<uint2*>((which ? p.dv : p.dk) + ((static_cast<long long>(batch) * p.Sk + k0 + row) * p.Hkv + kv_head) * D + c) = v;
+    *reinterpret_cast<uint2*>((which ? p.dv : p.dk) + ((static_cast<long long>(batch) * p.Sk + key) * p.Hkv + kv_head) * D + c) = v;
   }
 }
 
@@ -902,6 +905,7 @@ window_bwd_dq_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
 
   tc_fence_before();
   __syncthreads();
+  window_bwd_join<D>(p);
   if (*abort_flag) {
     __nanosleep(50000);
     if (threadIdx.x == 0) {
@@ -921,7 +925,7 @@ window_bwd_dq_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
 struct WindowBwdPlan {
   int sq_pad, key_blocks, row_tiles, piece;
   long long blocks, max_slots, rows;
-  long long at_delta, at_list, at_pieces, at_parts, words;   // in 4-byte words
+  long long at_delta, at_list, at_cuts, at_parts, words;   // in 4-byte words
 };
 
 static WindowBwdPlan window_bwd_plan(int B, int Sq, int Sk, int Hq, int Hkv, int D, int window, int sinks, bool packed) {
@@ -962,8 +966,8 @@ static WindowBwdPlan window_bwd_plan(int B, int Sq, int Sk, int Hq, int Hkv, int
   w.rows = static_cast<long long>(B) * Hq * w.sq_pad;
   w.at_delta = w.rows;
   w.at_list = 2 * w.rows;
-  w.at_pieces = w.at_list + 4 + 4 * (w.blocks + slots);       // int4 entries: at_list is a multiple of 128 words
-  w.at_parts = (w.at_pieces + 2 * w.blocks + 7) / 8 * 8;     // stored 32 bytes at a time
+  w.at_cuts = w.at_list + 4 + 4 * (w.blocks + slots);       // int4 entries: at_list is a multiple of 128 words
+  w.at_parts = (w.at_cuts + 4 * w.blocks + 7) / 8 * 8;     // stored 32 bytes at a time
   w.words = w.at_parts + slots * Hkv * 2 * kWinBlock * D;
   return w;
 }
@@ -991,10 +995,6 @@ static int launch_window_bwd(const WindowBwdMaps& m, const WindowBwdPrepArgs& pr
   const int grid_kv = static_cast<int>(most < sm_count() ? most : sm_count());
   window_bwd_dkdv_kernel<D><<<grid_kv, kWbThreads, smem_dkdv, stream>>>(m.q, m.dout, m.k, m.v, a);
   count_launch(2);
-  if (plan.max_slots > 0) {
-    window_bwd_join_kernel<D><<<dim3(static_cast<unsigned>(plan.blocks * a.Hkv), 4), 256, 0, stream>>>(a);
-    count_launch();
-  }
   const long long tiles = static_cast<long long>(plan.row_tiles) * a.Hq * a.B;
   window_bwd_dq_kernel<D><<<static_cast<int>(tiles < sm_count() ? tiles : sm_count()), kWbThreads, smem_dq, stream>>>(m.q, m.dout, m.k, m.v, a);
   count_launch();
@@ -1045,17 +1045,17 @@ MB_API int mb_window_attn_bwd(const void* q, long long q_tstride, long long q_bs
   float* lse2_pad = reinterpret_cast<float*>(scratch);
   float* delta = lse2_pad + plan.at_delta;
   int* list = scratch + plan.at_list;
-  int2* pieces = reinterpret_cast<int2*>(scratch + plan.at_pieces);
+  int4* cuts = reinterpret_cast<int4*>(scratch + plan.at_cuts);
   WindowBwdPrepArgs prep;
   prep.out = static_cast<const __nv_bfloat16*>(out), prep.out_lo = static_cast<const __nv_bfloat16*>(out_lo);
   prep.dout = static_cast<const __nv_bfloat16*>(dout);
   prep.do_tstride = do_tstride, prep.do_bstride = do_bstride;
-  prep.lse2_in = lse2, prep.lse2 = lse2_pad, prep.delta = delta, prep.list = list, prep.pieces = pieces, prep.rule = rule;
+  prep.lse2_in = lse2, prep.lse2 = lse2_pad, prep.delta = delta, prep.list = list, prep.cuts = cuts, prep.rule = rule;
   prep.B = B, prep.Sq = Sq, prep.Sk = Sk, prep.Hq = Hq, prep.Hkv = Hkv, prep.Sq_pad = plan.sq_pad, prep.key_blocks = plan.key_blocks;
   prep.piece = plan.piece, prep.max_slots = static_cast<int>(plan.max_slots);
   WindowBwdArgs a;
   a.dq = static_cast<__nv_bfloat16*>(dq), a.dk = static_cast<__nv_bfloat16*>(dk), a.dv = static_cast<__nv_bfloat16*>(dv);
-  a.lse2 = lse2_pad, a.delta = delta, a.list = list, a.pieces = pieces, a.parts = reinterpret_cast<float*>(scratch + plan.at_parts);
+  a.lse2 = lse2_pad, a.delta = delta, a.list = list, a.cuts = cuts, a.parts = reinterpret_cast<float*>(scratch + plan.at_parts);
   a.rule = rule;
   a.B = B, a.Sq = Sq, a.Sk = Sk, a.Hq = Hq, a.Hkv = Hkv, a.Sq_pad = plan.sq_pad;
   a.key_blocks = plan.key_blocks, a.row_tiles = plan.row_tiles;
