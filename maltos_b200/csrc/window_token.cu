@@ -6,7 +6,8 @@
 // head dimension may be permuted in S = Q K^T as long as Q and K agree, and the rows of O^T = V^T P^T may be any 16 dimensions,
 // so no value changes its lane (on the FMA pipe the same loop took 75 us for the case below, 1.4 times the tile kernel). The
 // parts are joined in shared memory, then across the cluster, in one launch and in a fixed order.
-// Bound by HBM: 8 rows x 2052 visible keys x 8 key/value heads of 128 are 67 MB, 10 us at the copy rate.
+// Bound by HBM: 8 rows x 2052 visible keys x 8 key/value heads of 128 are 67 MB, 10 us at the copy rate; it takes 20 us (25 us
+// with a cold L2): a single wave of clusters, whose first loads and last join nothing hides.
 #include "host.h"
 #include "ptx.cuh"
 #include "window.cuh"

@@ -163,10 +163,10 @@ def sliding_window_attention(q, k, v, *, window: int, sinks: int = 0, sequence_i
 
     A query that sees nothing (padding, or ``Sq > Sk``) gets zeros and log-sum-exp -inf. ``return_lse`` adds the log-sum-exp
     ``[B, heads, Sq]`` (fp32, not differentiable). k and v have to be finite everywhere, at padding too: a masked key has
-    weight zero, and zero times infinity is no number. On CUDA bf16 with head_dim 64 or 128 the kernels of
-    ``csrc/window_attn.cu``, ``csrc/window_attn_bwd.cu`` and, for a few queries without
-    gradients, ``csrc/window_token.cu`` run, which visit only the key blocks that the rule reaches; other
-    types and sizes run :func:`sliding_window_reference`."""
+    weight zero, and zero times infinity is no number; for gradients the same goes for q and for the output's gradient. On CUDA
+    bf16 with head_dim 64 or 128 the kernels of ``csrc/window_attn.cu``, ``csrc/window_attn_bwd.cu`` and, for a few queries
+    without gradients, ``csrc/window_token.cu`` run, which visit only the key blocks that the rule reaches; other types and
+    sizes run :func:`sliding_window_reference`."""
     _check_window_arguments(q, k, v, window, sinks, sequence_ids, scale)
     if _kernel_eligible(q, k, v) and q.numel() and k.numel():
         from .window_attn import window_attention
