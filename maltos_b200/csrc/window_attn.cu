@@ -11,7 +11,8 @@
 // another: 4400 cycles for the pair, of 2048 of UMMAs.) Halves of which no row sees a key are left out.
 // Measured (bf16, TFLOP/s of the visible pairs): 8192 rows, 32 / 8 heads of 128, window 1024 206 us / 628; 16384 rows, 8 / 2 heads,
 // window 4096 297 us / 814; the whole causal triangle of 8192 rows 616 us / 890; heads of 64 reach 352, since a product of half the
-// work leaves the same arithmetic. Bound by the tile's arithmetic (exponentials, conversions) between two products.
+// work leaves the same arithmetic. Bound by the tile's arithmetic between two products, by its instructions more than by the
+// exponentials: a quarter of them by polynomial on the multiply-add pipe costs 7 per cent here (the backward gains from that).
 // The two tiles are two query heads of one key/value head on the same rows where the group is even, else neighbouring rows of
 // one head. O is rescaled only when a row's maximum has grown by more than 2^8 since the last rescale: P then stays below 2^8
 // and its bf16 rounding is relative, so nothing is lost, and after the first blocks the rescale hardly ever happens.
@@ -294,12 +295,20 @@ window_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
     const uint32_t s_tmem = tmem_base + S_COL + static_cast<uint32_t>(t * 128 + half * 32) + t_lane;
     constexpr int HALF_D = D / 2;                  // columns of O that this thread rescales and stores
     const uint32_t o_tmem = tmem_base + O_COL + static_cast<uint32_t>(t * 128 + half * HALF_D) + t_lane;
-    // The two threads of a row exchange a value through shared memory and a barrier of their two warps. NaN says that a wait of
+    // The two threads of a row exchange a value through shared memory and barriers of their two warps; maxima only when one of the
+    // 64 threads has to rescale, which one barrier tells them all. NaN says that a wait of
     // one of them ran out: both then leave at the same place, so that neither is left behind at the barrier (a maximum is never
     // NaN, and a sum that is NaN stops nothing but the output loop of its own rows, for which `stop` is not looked at).
     float* slot = exchange + (t * 2 + half) * kWinBlock + row;
     const volatile float* partner = exchange + (t * 2 + (half ^ 1)) * kWinBlock + row;
     auto pair_barrier = [&] { asm volatile("bar.sync %0, 64;" ::"r"(1 + t * 4 + (warp & 3)) : "memory"); };
+    auto pair_any = [&](bool mine) {               // of the 64 threads
+      int any;
+      asm volatile(
+          "{\n.reg .pred p, q;\nsetp.ne.s32 p, %1, 0;\nbar.red.or.pred q, %2, 64, p;\nselp.s32 %0, 1, 0, q;\n}"
+          : "=r"(any) : "r"(static_cast<int>(mine)), "r"(1 + t * 4 + (warp & 3)) : "memory");
+      return any != 0;
+    };
     auto swap = [&](float mine) {
       *slot = mine;
       pair_barrier();
@@ -353,11 +362,11 @@ window_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
               for (int k = 0; k < 4; ++k) mx[k] = fmaxf(fmaxf(mx[k], __uint_as_float(s[i + 2 * k])), __uint_as_float(s[i + 2 * k + 1]));
             m_blk = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * p.scale_log2;
           }
-          const float m_other = swap(ok ? m_blk : NAN);
-          stop = __any_sync(0xffffffffu, !ok || m_other != m_other);
-          if (stop) continue;
-          m_blk = fmaxf(m_blk, m_other);
-          if (__any_sync(0xffffffffu, m_blk > m_run + kWfGrowth)) {   // the same for the two warps of these rows
+          if (pair_any(!ok || m_blk > m_run + kWfGrowth)) {   // seldom, after the first blocks; the same for the two warps of these rows
+            const float m_other = swap(ok ? m_blk : NAN);
+            stop = __any_sync(0xffffffffu, !ok || m_other != m_other);
+            if (stop) continue;
+            m_blk = fmaxf(m_blk, m_other);
             const float m_new = fmaxf(m_run, ceilf(m_blk));
             const float alpha = m_run == -INFINITY ? 0.f : wf_exp2(m_run - m_new);   // a power of two
             m_run = m_new;
