@@ -2,11 +2,11 @@
 //   forward   out[t] = scale * weight[ids[t]]
 //   gradient  dweight[r] = scale * sum of dout[t] over the tokens t of row r, in the order of t and in fp32, rounded once
 // Three launches make the gradient, without atomics on floating-point values, so its bits do not depend on the schedule:
-//   embedding_sort_kernel   cluster 0 (8 CTAs) sorts the pairs (row, t) by row, stably, with digits of up to 8 bits;
-//                           all other CTAs meanwhile write the zeros of dweight, which is most of what there is to write;
+//   embedding_sort_kernel   one cluster sorts the pairs (row, t) by row, stably, with digits of up to 8 bits;
 //   embedding_chunk_kernel  one CTA per 32 sorted tokens (and slice of columns): runs that lie inside go straight to their row,
 //                           the parts of runs that cross a chunk's border go to fp32 buffers. A frequent token is thereby
-//                           spread over as many CTAs as it has chunks;
+//                           spread over as many CTAs as it has chunks. The CTAs behind them write the zeros, of which most of
+//                           dweight consists: each looks its rows up among the sorted ones;
 //   embedding_join_kernel   adds the parts of the crossing runs, in order.
 // Bound by memory: 32768 tokens into a bf16 table of 128256 x 4096 take 70 us forward (4.8 TB/s) and about 300 us backward, of which
 // 217 us are the zeros (1.05 GB at 4.8 TB/s; bulk copies from shared memory write no faster), 59 the runs and 23 the join. With few
@@ -21,7 +21,7 @@ namespace mb {
 constexpr int kEmbThreads = 256;
 constexpr int kSortCtas = 8, kSortThreads = 1024, kSortWarps = kSortThreads / 32, kSortBins = 256;
 constexpr int kEmbChunk = 32;
-constexpr int kZeroVecs = 8 * kSortThreads;   // 32-byte pieces that a CTA writes: short pieces, since clusters leave some SMs out at first
+constexpr int kZeroRows = 32;     // rows that a CTA of zeros looks up
 constexpr int kEmbJoinThreads = 64;   // narrow blocks: a frequent token's parts are added by several SMs
 
 template <typename I>
@@ -59,7 +59,7 @@ __global__ void __launch_bounds__(kEmbThreads) embedding_fwd_kernel(const I* __r
   }
 }
 
-// ---------------------------------------------------------------------------------------------- sort + zeros
+// ---------------------------------------------------------------------------------------------- sort
 struct EmbSortArgs {
   const void* ids;
   int* key[2];        // ping-pong pairs; the sorted ones end in [passes & 1 ? 0 : 1]
@@ -67,9 +67,6 @@ struct EmbSortArgs {
   int tokens, rows;   // rows: also the key of tokens that get no gradient (outside the table, or padding_idx)
   int pad;            // padding_idx, or -1
   int passes, bits;
-  uint8_t* zero;      // dweight
-  long long zero_vecs;
-  int zero_tail;      // bytes behind the last whole 32
 };
 
 // shared memory of another CTA of the cluster
@@ -81,17 +78,6 @@ __device__ __forceinline__ int ld_cluster_s32(uint32_t addr) {
 
 template <typename I>
 __global__ void __cluster_dims__(kSortCtas, 1, 1) __launch_bounds__(kSortThreads) embedding_sort_kernel(const EmbSortArgs p) {
-  if (blockIdx.x >= kSortCtas) {
-    const uint32_t none[8] = {0u, 0u, 0u, 0u, 0u, 0u, 0u, 0u};
-    const long long first = static_cast<long long>(blockIdx.x - kSortCtas) * kZeroVecs;
-#pragma unroll
-    for (int i = 0; i < kZeroVecs; i += kSortThreads) {
-      const long long at = first + i + threadIdx.x;
-      if (at < p.zero_vecs) store_32_bytes(p.zero + 32 * at, none);
-    }
-    if (first == 0 && static_cast<int>(threadIdx.x) < p.zero_tail) p.zero[32 * p.zero_vecs + threadIdx.x] = 0;
-    return;
-  }
   __shared__ int hist[kSortWarps][kSortBins];   // per warp: counts, then where the warp's next element of a digit goes
   __shared__ int total[kSortBins];              // of this CTA, read by the others
   __shared__ int scan[kSortBins / 32];
@@ -211,8 +197,31 @@ template <typename T, int N>
 __global__ void __launch_bounds__(kEmbThreads) embedding_chunk_kernel(const int* __restrict__ key, const int* __restrict__ pos,
                                                                       const T* __restrict__ dout, T* __restrict__ dweight,
                                                                       float* __restrict__ head, float* __restrict__ tail, int tokens, int H,
-                                                                      int rows, float scale) {
+                                                                      int rows, int chunks, float scale) {
   __shared__ int s_key[kEmbChunk + 2], s_pos[kEmbChunk];
+  const int c = (blockIdx.y * kEmbThreads + threadIdx.x) * N;
+  if (static_cast<int>(blockIdx.x) >= chunks) {    // zeros of the rows that no token has
+    const long long row0 = static_cast<long long>(blockIdx.x - chunks) * kZeroRows;
+    const int n = static_cast<int>(rows - row0 < kZeroRows ? rows - row0 : kZeroRows);
+    if (threadIdx.x < n) {
+      const int r = static_cast<int>(row0) + threadIdx.x;
+      int lo = 0, hi = tokens;                     // the first token whose row is r or a later one
+      while (lo < hi) {
+        const int mid = lo + (hi - lo) / 2;
+        if (key[mid] < r) lo = mid + 1;
+        else hi = mid;
+      }
+      s_pos[threadIdx.x] = lo < tokens && key[lo] == r;
+    }
+    __syncthreads();
+    if (c >= H) return;
+    Vec<T, N> none;
+#pragma unroll
+    for (int k = 0; k < N; ++k) none.set(k, 0.f);
+    for (int i = 0; i < n; ++i)
+      if (!s_pos[i]) none.store(dweight + (row0 + i) * H + c);
+    return;
+  }
   const long long first = static_cast<long long>(blockIdx.x) * kEmbChunk;
   const int n = static_cast<int>(tokens - first < kEmbChunk ? tokens - first : kEmbChunk);
   if (threadIdx.x < kEmbChunk + 2) {               // the chunk's rows with one neighbour on either side, -1 beyond the ends
@@ -221,7 +230,6 @@ __global__ void __launch_bounds__(kEmbThreads) embedding_chunk_kernel(const int*
     if (threadIdx.x < n) s_pos[threadIdx.x] = pos[first + threadIdx.x];
   }
   __syncthreads();
-  const int c = (blockIdx.y * kEmbThreads + threadIdx.x) * N;
   if (c >= H) return;
   float acc[N];
 #pragma unroll
@@ -310,9 +318,10 @@ static int launch_embedding_runs(const EmbSortArgs& s, const void* dout, void* d
   const int* pos = s.pos[(s.passes - 1) & 1];
   const int chunks = (s.tokens + kEmbChunk - 1) / kEmbChunk;
   float* tail = parts + static_cast<long long>(chunks) * H;
-  const dim3 grid(chunks, (H / N + kEmbThreads - 1) / kEmbThreads);
+  const long long zeros = (static_cast<long long>(s.rows) + kZeroRows - 1) / kZeroRows;
+  const dim3 grid(static_cast<unsigned>(chunks + zeros), (H / N + kEmbThreads - 1) / kEmbThreads);
   embedding_chunk_kernel<T, N><<<grid, kEmbThreads, 0, stream>>>(key, pos, static_cast<const T*>(dout), static_cast<T*>(dweight), parts,
-                                                               tail, s.tokens, H, s.rows, scale);
+                                                               tail, s.tokens, H, s.rows, chunks, scale);
   embedding_join_kernel<T, N><<<dim3(chunks, (H / N + kEmbJoinThreads - 1) / kEmbJoinThreads), kEmbJoinThreads, 0, stream>>>(key, static_cast<T*>(dweight), parts, tail, s.tokens, H, s.rows, scale);
   count_launch(2);
   MB_CHECK_CUDA(cudaGetLastError());
@@ -362,8 +371,8 @@ MB_API int mb_embedding_bwd(const void* ids, int wide, const void* dout, void* d
     set_last_error(what);
     return -1;
   }
-  if ((reinterpret_cast<uintptr_t>(dweight) | reinterpret_cast<uintptr_t>(scratch)) & 31) {
-    set_last_error("mb_embedding_bwd: dweight and scratch must be 32-byte aligned");
+  if ((reinterpret_cast<uintptr_t>(dweight) | reinterpret_cast<uintptr_t>(scratch)) & 15) {
+    set_last_error("mb_embedding_bwd: dweight and scratch must be 16-byte aligned");
     return -3;
   }
   EmbSortArgs s;
@@ -375,17 +384,8 @@ MB_API int mb_embedding_bwd(const void* ids, int wide, const void* dout, void* d
   while ((rows >> width) != 0) ++width;            // bits of the largest key, `rows`
   s.passes = (width + 7) / 8;
   s.bits = (width + s.passes - 1) / s.passes;
-  const long long bytes = rows * H * (dtype == 2 ? 4 : 2);
-  s.zero = static_cast<uint8_t*>(dweight);
-  s.zero_vecs = bytes / 32, s.zero_tail = static_cast<int>(bytes % 32);
-  const long long fill = bytes / 32 / kZeroVecs + 1;
-  if (fill >= (1ll << 31) - 65536) {
-    set_last_error("mb_embedding_bwd: the table is too large");
-    return -1;
-  }
-  const unsigned grid = static_cast<unsigned>(kSortCtas + (fill + kSortCtas - 1) / kSortCtas * kSortCtas);
-  if (wide) embedding_sort_kernel<long long><<<grid, kSortThreads, 0, stream>>>(s);
-  else embedding_sort_kernel<int><<<grid, kSortThreads, 0, stream>>>(s);
+  if (wide) embedding_sort_kernel<long long><<<kSortCtas, kSortThreads, 0, stream>>>(s);
+  else embedding_sort_kernel<int><<<kSortCtas, kSortThreads, 0, stream>>>(s);
   count_launch();
   MB_CHECK_CUDA(cudaGetLastError());
   const bool aligned = (reinterpret_cast<uintptr_t>(dout) & 15) == 0;
