@@ -2,15 +2,17 @@
 //   forward   out[t] = scale * weight[ids[t]]
 //   gradient  dweight[r] = scale * sum of dout[t] over the tokens t of row r, in the order of t and in fp32, rounded once
 // Three launches make the gradient, without atomics on floating-point values, so its bits do not depend on the schedule:
-//   embedding_sort_kernel   one cluster sorts the pairs (row, t) by row, stably, with digits of up to 8 bits;
+//   embedding_sort_kernel   one cluster sorts the pairs (row, t) by row, stably, with digits of up to 9 bits (two passes
+//                           up to 2^18 rows; of 8 bits three from 2^16 on: 33 us for 32768 tokens, where two take 28);
 //   embedding_chunk_kernel  one CTA per 32 sorted tokens (and slice of columns): runs that lie inside go straight to their row,
 //                           the parts of runs that cross a chunk's border go to fp32 buffers. A frequent token is thereby
 //                           spread over as many CTAs as it has chunks. The CTAs behind them write the zeros, of which most of
 //                           dweight consists: each looks its rows up among the sorted ones;
 //   embedding_join_kernel   adds the parts of the crossing runs, in order.
-// Bound by memory: 32768 tokens into a bf16 table of 128256 x 4096 take 70 us forward (4.8 TB/s) and about 300 us backward, of which
-// 217 us are the zeros (1.05 GB at 4.8 TB/s; bulk copies from shared memory write no faster), 59 the runs and 23 the join. With few
-// tokens the launches are what counts: 1024 tokens of a 32000 x 512 table 4 + 29 us.
+// Bound by memory: 32768 tokens into a bf16 table of 128256 x 4096 take 70 us forward and 250 us backward: sort 28, runs and zeros
+// 198 (1.3 GB at 6.7 TB/s), join 23. (Zeros of the whole table, written under the sort by the other CTAs of its grid, took 217 us:
+// a grid of clusters does not keep the SMs full.) With few tokens the launches are what counts: 1024 tokens of a 32000 x 512 table
+// 4 + 27 us.
 // Ids outside the table set the status word (index out of bounds), read as zero rows and get no gradient.
 #include "host.h"
 #include "ptx.cuh"
@@ -19,7 +21,7 @@
 namespace mb {
 
 constexpr int kEmbThreads = 256;
-constexpr int kSortCtas = 8, kSortThreads = 1024, kSortWarps = kSortThreads / 32, kSortBins = 256;
+constexpr int kSortCtas = 8, kSortThreads = 1024, kSortWarps = kSortThreads / 32, kSortBins = 512;
 constexpr int kEmbChunk = 32;
 constexpr int kZeroRows = 32;     // rows that a CTA of zeros looks up
 constexpr int kEmbJoinThreads = 64;   // narrow blocks: a frequent token's parts are added by several SMs
@@ -78,7 +80,8 @@ __device__ __forceinline__ int ld_cluster_s32(uint32_t addr) {
 
 template <typename I>
 __global__ void __cluster_dims__(kSortCtas, 1, 1) __launch_bounds__(kSortThreads) embedding_sort_kernel(const EmbSortArgs p) {
-  __shared__ int hist[kSortWarps][kSortBins];   // per warp: counts, then where the warp's next element of a digit goes
+  extern __shared__ int hist_all[];             // per warp: counts, then where the warp's next element of a digit goes
+  int(*hist)[kSortBins] = reinterpret_cast<int(*)[kSortBins]>(hist_all);
   __shared__ int total[kSortBins];              // of this CTA, read by the others
   __shared__ int scan[kSortBins / 32];
   const int cta = blockIdx.x, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -382,10 +385,19 @@ MB_API int mb_embedding_bwd(const void* ids, int wide, const void* dout, void* d
   s.tokens = static_cast<int>(tokens), s.rows = static_cast<int>(rows), s.pad = static_cast<int>(padding_idx);
   int width = 1;
   while ((rows >> width) != 0) ++width;            // bits of the largest key, `rows`
-  s.passes = (width + 7) / 8;
+  s.passes = (width + 8) / 9;
   s.bits = (width + s.passes - 1) / s.passes;
-  if (wide) embedding_sort_kernel<long long><<<kSortCtas, kSortThreads, 0, stream>>>(s);
-  else embedding_sort_kernel<int><<<kSortCtas, kSortThreads, 0, stream>>>(s);
+  constexpr int kSortBytes = kSortWarps * kSortBins * static_cast<int>(sizeof(int));
+  static bool configured[64] = {false};
+  int dev = 0;
+  MB_CHECK_CUDA(cudaGetDevice(&dev));
+  if (!configured[dev & 63]) {
+    MB_CHECK_CUDA(cudaFuncSetAttribute(embedding_sort_kernel<long long>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSortBytes));
+    MB_CHECK_CUDA(cudaFuncSetAttribute(embedding_sort_kernel<int>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSortBytes));
+    configured[dev & 63] = true;
+  }
+  if (wide) embedding_sort_kernel<long long><<<kSortCtas, kSortThreads, kSortBytes, stream>>>(s);
+  else embedding_sort_kernel<int><<<kSortCtas, kSortThreads, kSortBytes, stream>>>(s);
   count_launch();
   MB_CHECK_CUDA(cudaGetLastError());
   const bool aligned = (reinterpret_cast<uintptr_t>(dout) & 15) == 0;
