@@ -333,8 +333,8 @@ static int launch_embedding_runs(const EmbSortArgs& s, const void* dout, void* d
 
 static const char* embedding_problem(int dtype, long long tokens, long long rows, int H) {
   if (dtype < 0 || dtype > 2) return "embedding: the table is bf16, fp16 or fp32";
-  if (tokens < 1 || tokens >= (1ll << 31) - 65536 || rows < 1 || rows >= (1ll << 31) - 1 || H < 1 || H > (1 << 24))
-    return "embedding: tokens and rows below 2^31, hidden size up to 2^24, all positive";
+  if (tokens < 1 || tokens >= (1ll << 31) - 65536 || rows < 1 || rows >= (1ll << 31) - 1 || H < 1 || H > (1 << 21))
+    return "embedding: tokens and rows below 2^31, hidden size up to 2^21, all positive";
   return nullptr;
 }
 

@@ -3,6 +3,7 @@ import pytest
 import torch
 import torch.nn.functional as F
 
+from maltos_b200.ops import _lib
 from maltos_b200.ops.embedding import ScaledEmbedding, embedding
 from maltos_b200.ops.norm import add_rms_norm, block_norm
 
@@ -81,3 +82,18 @@ def test_embedding_refusals():
             embedding(*args, **kw)
     with pytest.raises(IndexError):
         embedding(torch.tensor([5]), w)
+
+
+def test_entry_points_refuse_sizes_before_touching_the_device():
+    """Sizes whose launches would not fit the grid (2^21 columns and more are 65536 blocks of the narrowest join) and sizes that no
+    kernel takes come back as errors; no pointer is read."""
+    lib = _lib.lib()
+    a = 4096
+    for tokens, H, rows in ((1, 2 ** 21 + 1, 4), (0, 8, 4), (2 ** 31, 8, 4), (1, 0, 4), (1, 8, 0), (1, 8, 2 ** 31)):
+        assert lib.mb_embedding_fwd(a, 1, a, a, 0, tokens, H, rows, 1.0, None) == -1
+        assert lib.mb_embedding_bwd(a, 1, a, a, a, 0, tokens, H, rows, -1, 1.0, None) == -1
+    assert lib.mb_embedding_bwd(a, 1, a, a, a, 3, 1, 8, 4, -1, 1.0, None) == -1          # no such type
+    for rows, H in ((0, 8), (1, 4), (1, 12), (1, 16392), (2 ** 31, 8)):
+        assert lib.mb_block_norm_fwd(a, a, None, None, None, 0, a, None, None, None, 0, rows, H, 1.0, 1e-6, None) == -1
+        assert lib.mb_block_norm_bwd(None, a, None, None, None, None, None, 0, None, None, a, a, None, None, None, None, None, 0, rows, H, 1.0, None) == -1
+    assert lib.mb_block_norm_fwd(a + 8, a, None, None, None, 0, a, None, None, None, 0, 1, 8, 1.0, 1e-6, None) == -1     # 8 bytes off
