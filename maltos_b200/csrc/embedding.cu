@@ -23,7 +23,7 @@ namespace mb {
 constexpr int kEmbThreads = 256;
 constexpr int kSortCtas = 8, kSortThreads = 1024, kSortWarps = kSortThreads / 32, kSortBins = 512;
 constexpr int kEmbChunk = 32;
-constexpr int kZeroRows = 32;     // rows that a CTA of zeros looks up
+constexpr int kZeroBytes = 128 * 1024;   // of a CTA of zeros, which looks up 32 rows (wide tables) to 256 (narrow ones)
 constexpr int kEmbJoinThreads = 64;   // narrow blocks: a frequent token's parts are added by several SMs
 
 template <typename I>
@@ -200,12 +200,13 @@ template <typename T, int N>
 __global__ void __launch_bounds__(kEmbThreads) embedding_chunk_kernel(const int* __restrict__ key, const int* __restrict__ pos,
                                                                       const T* __restrict__ dout, T* __restrict__ dweight,
                                                                       float* __restrict__ head, float* __restrict__ tail, int tokens, int H,
-                                                                      int rows, int chunks, float scale) {
+                                                                      int rows, int chunks, int zero_rows, float scale) {
   __shared__ int s_key[kEmbChunk + 2], s_pos[kEmbChunk];
+  __shared__ bool s_used[kEmbThreads];
   const int c = (blockIdx.y * kEmbThreads + threadIdx.x) * N;
   if (static_cast<int>(blockIdx.x) >= chunks) {    // zeros of the rows that no token has
-    const long long row0 = static_cast<long long>(blockIdx.x - chunks) * kZeroRows;
-    const int n = static_cast<int>(rows - row0 < kZeroRows ? rows - row0 : kZeroRows);
+    const long long row0 = static_cast<long long>(blockIdx.x - chunks) * zero_rows;
+    const int n = static_cast<int>(rows - row0 < zero_rows ? rows - row0 : zero_rows);
     if (threadIdx.x < n) {
       const int r = static_cast<int>(row0) + threadIdx.x;
       int lo = 0, hi = tokens;                     // the first token whose row is r or a later one
@@ -214,15 +215,21 @@ __global__ void __launch_bounds__(kEmbThreads) embedding_chunk_kernel(const int*
         if (key[mid] < r) lo = mid + 1;
         else hi = mid;
       }
-      s_pos[threadIdx.x] = lo < tokens && key[lo] == r;
+      s_used[threadIdx.x] = lo < tokens && key[lo] == r;
     }
     __syncthreads();
-    if (c >= H) return;
+    // vector by vector of this slice of columns, row after row, so that narrow rows keep all threads busy
+    const int c0 = blockIdx.y * kEmbThreads * N, width = min(kEmbThreads, (H - c0) / N);
     Vec<T, N> none;
 #pragma unroll
     for (int k = 0; k < N; ++k) none.set(k, 0.f);
-    for (int i = 0; i < n; ++i)
-      if (!s_pos[i]) none.store(dweight + (row0 + i) * H + c);
+    int i = threadIdx.x / width, v = threadIdx.x % width;
+    const int down = kEmbThreads / width, right = kEmbThreads % width;
+    while (i < n) {
+      if (!s_used[i]) none.store(dweight + (row0 + i) * H + c0 + v * N);
+      i += down, v += right;
+      if (v >= width) v -= width, ++i;
+    }
     return;
   }
   const long long first = static_cast<long long>(blockIdx.x) * kEmbChunk;
@@ -321,10 +328,12 @@ static int launch_embedding_runs(const EmbSortArgs& s, const void* dout, void* d
   const int* pos = s.pos[(s.passes - 1) & 1];
   const int chunks = (s.tokens + kEmbChunk - 1) / kEmbChunk;
   float* tail = parts + static_cast<long long>(chunks) * H;
-  const long long zeros = (static_cast<long long>(s.rows) + kZeroRows - 1) / kZeroRows;
+  const int slice = (H / N < kEmbThreads ? H / N : kEmbThreads) * N * static_cast<int>(sizeof(T));   // bytes of a row in a CTA of zeros
+  const int zero_rows = kZeroBytes / slice < 32 ? 32 : kZeroBytes / slice < kEmbThreads ? kZeroBytes / slice : kEmbThreads;
+  const long long zeros = (static_cast<long long>(s.rows) + zero_rows - 1) / zero_rows;
   const dim3 grid(static_cast<unsigned>(chunks + zeros), (H / N + kEmbThreads - 1) / kEmbThreads);
   embedding_chunk_kernel<T, N><<<grid, kEmbThreads, 0, stream>>>(key, pos, static_cast<const T*>(dout), static_cast<T*>(dweight), parts,
-                                                               tail, s.tokens, H, s.rows, chunks, scale);
+                                                               tail, s.tokens, H, s.rows, chunks, zero_rows, scale);
   embedding_join_kernel<T, N><<<dim3(chunks, (H / N + kEmbJoinThreads - 1) / kEmbJoinThreads), kEmbJoinThreads, 0, stream>>>(key, static_cast<T*>(dweight), parts, tail, s.tokens, H, s.rows, scale);
   count_launch(2);
   MB_CHECK_CUDA(cudaGetLastError());

@@ -70,6 +70,24 @@ def test_embedding_frequent_tokens(pad):
         _embedding_case(ids, 3 * len(lengths) + 7, 136, torch.bfloat16, 1.0, pad)
 
 
+@pytest.mark.parametrize("rows,H", [(70001, 8), (70001, 1), (40000, 64), (3001, 513), (5000, 2056), (777, 4104), (33, 30000)])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_embedding_writes_every_element_of_the_gradient(rows, H, dtype):
+    """What the gradient's memory held before does not show: it is NaN, in tables of narrow and wide rows and several slices."""
+    ids = torch.randint(0, rows, (50,), device=DEV, generator=_gen(H))
+    ids[:4] = torch.tensor([0, rows - 1, 1, rows - 1], device=DEV)
+    w = torch.randn(rows, H, device=DEV, generator=_gen(1)).to(dtype).requires_grad_()
+    out = embedding(ids, w)
+    want = torch.bincount(ids, minlength=rows).to(dtype).unsqueeze(1).expand(rows, H)
+    ones = torch.ones_like(out)
+    for _ in range(3):                                                 # the allocator hands the freed memory out again
+        stale = torch.full((rows, H), float("nan"), dtype=dtype, device=DEV)
+        del stale
+        (dw,) = torch.autograd.grad(out, w, ones, retain_graph=True)
+        assert torch.equal(dw, want)
+        del dw
+
+
 def test_embedding_many_tokens_and_narrow_ids():
     ids = (torch.rand(3, 30011, device=DEV, generator=_gen(5)) ** 4 * 5000).long()
     a = _embedding_case(ids, 5000, 64, torch.float32, 2.0, 0)
