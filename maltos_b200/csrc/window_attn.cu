@@ -429,7 +429,9 @@ window_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
       }
       l_run += swap(l_run);
       if (LSE) x_run += swap(x_run);
-      const float inv = l_run > 0.f ? 1.f / l_run : 0.f;
+      // A row that sees nothing is told by its visibility, not by its sum: a query that is no number has to stay one.
+      const bool sees = w.hi >= 0;
+      const float inv = sees ? 1.f / l_run : 0.f;
       const long long at = ((static_cast<long long>(it.batch) * p.Sq + qi) * p.Hq + head) * D + half * HALF_D;
 #pragma unroll 1
       for (int c = 0; c < HALF_D; c += 16) {
@@ -455,8 +457,8 @@ window_fwd_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant
       tc_fence_before();                           // these reads of O come before the next item's first product (via p_full)
       if (qi < p.Sq && half == 0) {
         const long long stat = (static_cast<long long>(it.batch) * p.Hq + head) * p.Sq + qi;
-        if (p.lse2) p.lse2[stat] = l_run > 0.f ? m_run + log2f(l_run) : -INFINITY;
-        if (LSE) p.lse[stat] = x_run > 0.f ? (m_run + log2f(x_run)) * kWfLn2 : -INFINITY;
+        if (p.lse2) p.lse2[stat] = sees ? m_run + log2f(l_run) : -INFINITY;
+        if (LSE) p.lse[stat] = sees ? (m_run + log2f(x_run)) * kWfLn2 : -INFINITY;
       }
     }
   }

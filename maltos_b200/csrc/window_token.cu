@@ -196,9 +196,11 @@ __global__ void __launch_bounds__(kWtThreads, 4) window_token_kernel(const Windo
       sum += a * cl[i], sum_x += a * cx[i], val += a * co[i];
     }
     if (out_row < rows) {
-      p.out[((static_cast<long long>(batch) * p.Sq + oq) * p.Hq + head) * D + d] = __float2bfloat16(sum > 0.f ? val / sum : 0.f);
+      // told by the row's visibility, not by its sum: a query that is no number has to stay one
+      const bool sees = window_row(p.rule, batch, p.Sk, oq + p.Sk - p.Sq, true).hi >= 0;
+      p.out[((static_cast<long long>(batch) * p.Sq + oq) * p.Hq + head) * D + d] = __float2bfloat16(sees ? val / sum : 0.f);
       if (d == 0 && p.lse)
-        p.lse[(static_cast<long long>(batch) * p.Hq + head) * p.Sq + oq] = sum_x > 0.f ? (top + log2f(sum_x)) * 0.6931471805599453f : -INFINITY;
+        p.lse[(static_cast<long long>(batch) * p.Hq + head) * p.Sq + oq] = sees ? (top + log2f(sum_x)) * 0.6931471805599453f : -INFINITY;
     }
   }
   cluster_arrive();                                 // nobody leaves while its shared memory is read

@@ -162,7 +162,7 @@ def sliding_window_attention(q, k, v, *, window: int, sinks: int = 0, sequence_i
         key j is visible  <=>  s(p) <= j <= p  and  (p - j < window  or  j - s(p) < sinks).
 
     A query that sees nothing (padding, or ``Sq > Sk``) gets zeros and log-sum-exp -inf. ``return_lse`` adds the log-sum-exp
-    ``[B, heads, Sq]`` (fp32, not differentiable). k and v have to be finite everywhere, at padding too: a masked key has
+    ``[B, heads, Sq]`` (fp32, not differentiable). A query that holds NaN or an infinity gets NaN, and spoils no other. k and v have to be finite everywhere, at padding too: a masked key has
     weight zero, and zero times infinity is no number; for gradients the same goes for q and for the output's gradient. On CUDA
     bf16 with head_dim 64 or 128 the kernels of ``csrc/window_attn.cu``, ``csrc/window_attn_bwd.cu`` and, for a few queries
     without gradients, ``csrc/window_token.cu`` run, which visit only the key blocks that the rule reaches; other types and
