@@ -5,9 +5,11 @@
 // The forward keeps r1 and r2, the backward needs x, h and the two of them:
 //   dn2 = dy * w2, hn = h * r2, c2 = mean(dn2 * hn);  dt = dh + r2 * (dn2 - hn * c2)      = dresidual
 //   dg = scale * dt * u;  dn1 = scale * gate * dt * w1, xn = x * r1, c1 = mean(dn1 * xn);  dx = r1 * (dn1 - xn * c1)
-// c1 is linear in dt: with e = scale * gate * w1 * xn it is mean(e * (dh + r2 * dn2)) - c2 * mean(e * r2 * hn), so ONE round of
-// sums (c2 and the two means) serves both norms. For a gate a channel, dw1 and dgate are gate and w1 times the same column
-// sum of scale * dt * xn, so two column sums cover three gradients.
+// c1 is linear in dt: with a = gate * w1 * xn it is scale * (mean(a * (dh + r2 * dn2)) - r2 * c2 * mean(a * hn)), so ONE round of
+// sums (c2 and the two means) serves both norms. Products are formed around xn and hn, which are of order one: with r1 * r1 or
+// r2 * r2 taken out of the sums, rows of 1e15 and more (or 1e-13 and less, with a small eps) left the range of fp32 on the way,
+// and dx lost its second term or was infinite although the gradient itself is well inside. For a gate a channel, dw1 and dgate are
+// gate and w1 times the same column sum of scale * dt * xn, so two column sums cover three gradients.
 // The forward is bound by memory, rows in registers between the sums and the write-back: 8192 rows of 4096 in bf16 take 46 us
 // (5.8 TB/s). The backward (91 us, 4.4 TB/s, and 8 us for the column sums; with a gate a channel 4093 rows of 5120 50 us) is held
 // up by its instructions and by the sums in the middle of a row.
@@ -259,7 +261,7 @@ __global__ void __launch_bounds__(bn_bwd_threads(sizeof(T), V), 1) block_norm_bw
       if (p.w1) next_r1 = p.r1[row + gridDim.x];
       if (PRE) next_r2 = p.r2[row + gridDim.x];
     }
-    const uint64_t r2_2 = f32x2(r2, r2);
+    const uint64_t r1_2 = f32x2(r1, r1), r2_2 = f32x2(r2, r2);
     // of a piece: x, h, the gate and b = dh + r2 * dn2
     Vec<T, kBnVec> x, h, g;
     uint64_t b[KEEP ? V : 1][kBnPairs], acc[3] = {0, 0, 0};
@@ -303,7 +305,7 @@ __global__ void __launch_bounds__(bn_bwd_threads(sizeof(T), V), 1) block_norm_bw
         }
       }
     };
-    // sums over the row of r2 * dn2 * h, a * b and a * h with a = gate * w1 * x; what is the same for the whole row comes in later
+    // sums over the row of r2 * dn2 * h, a * b and a * h with a = gate * w1 * xn; what is the same for the whole row comes in later
 #pragma unroll
     for (int j = 0; j < V; ++j) {
       const int s = slot0 + j, m = KEEP ? j : 0, c = tid * kBnVec + j * width;
@@ -314,7 +316,7 @@ __global__ void __launch_bounds__(bn_bwd_threads(sizeof(T), V), 1) block_norm_bw
         if (w1) {
 #pragma unroll
           for (int i = 0; i < kBnPairs; ++i) {
-            const uint64_t a = gated(mul_f32x2(pair_of(x, i), pair_of(v1[KEEP ? j : 0], i)), j, i);
+            const uint64_t a = gated(mul_f32x2(mul_f32x2(pair_of(x, i), r1_2), pair_of(v1[KEEP ? j : 0], i)), j, i);
             acc[1] = fma_f32x2(a, b[m][i], acc[1]);
             if (PRE) acc[2] = fma_f32x2(a, pair_of(h, i), acc[2]);
           }
@@ -327,9 +329,9 @@ __global__ void __launch_bounds__(bn_bwd_threads(sizeof(T), V), 1) block_norm_bw
     __syncwarp();                                  // a row of one warp has no barrier
     const bool beside = ring.slots >= 2 * V;       // the next row fits beside this one
     if (tid == 0 && beside && it > 0) refill(slot0 >= V ? slot0 - V : slot0 - V + ring.slots, it - 1);   // everyone is done with the row before
-    // c2 = mean(dn2 * hn), c1 = mean(scale * a * r1 * (b - r2 * hn * c2)); k2 = r2 * r2 * c2, k1 = r1 * r1 * c1
-    const float k2 = r2 * r2 * sums[0] * inv, sr1 = p.scale * r1;
-    const float k1 = r1 * r1 * sr1 * (sums[1] - k2 * sums[2]) * inv;
+    // with c2 = mean(dn2 * hn) and c1 = mean(scale * a * (b - r2 * hn * c2)): k2 = r2 * c2, k1 = r1 * c1
+    const float k2 = r2 * (sums[0] * inv), sr1 = p.scale * r1;
+    const float k1 = sr1 * ((sums[1] - k2 * (r2 * sums[2])) * inv);
     const uint64_t minus_k2 = f32x2(-k2, -k2), minus_k1 = f32x2(-k1, -k1), sr1_2 = f32x2(sr1, sr1);
 #pragma unroll
     for (int j = 0; j < V; ++j) {
@@ -339,14 +341,14 @@ __global__ void __launch_bounds__(bn_bwd_threads(sizeof(T), V), 1) block_norm_bw
         Vec<T, kBnVec> ox, or_, og;
 #pragma unroll
         for (int i = 0; i < kBnPairs; ++i) {
-          const uint64_t dt = PRE ? fma_f32x2(pair_of(h, i), minus_k2, b[m][i]) : b[m][i];
+          const uint64_t dt = PRE ? fma_f32x2(mul_f32x2(pair_of(h, i), r2_2), minus_k2, b[m][i]) : b[m][i];
           set_pair(or_, i, dt);
           const uint64_t sdt = mul_f32x2(dt, sr1_2), xi = pair_of(x, i);   // scale * dt * r1; r1 is 1 without w1
           uint64_t du = w1 ? mul_f32x2(sdt, pair_of(v1[wm], i)) : sdt;
           if (GATE == 2) set_pair(og, i, mul_f32x2(du, xi));
           s1[j][i] = fma_f32x2(GATE == 2 ? gated(sdt, j, i) : sdt, xi, s1[j][i]);
           du = gated(du, j, i);
-          if (w1) du = fma_f32x2(xi, minus_k1, du);
+          if (w1) du = fma_f32x2(mul_f32x2(xi, r1_2), minus_k1, du);
           set_pair(ox, i, du);
         }
         or_.store(static_cast<T*>(p.dres) + base + c);
