@@ -929,6 +929,19 @@ struct WindowBwdPlan {
   long long at_delta, at_list, at_cuts, at_parts, words;   // in 4-byte words
 };
 
+// Pieces that packed rows can need at most, beside those of blocks that the window alone makes too long. A block is cut for its
+// first tokens only if the queries behind them fill more tiles than a piece takes, so their document is long, and a row has few
+// such documents: with m tiles to exceed, T queries fill at most (T - 1) / 128 + 2 tiles, and up to 127 of them come from before the
+// document. Each of its blocks (of first tokens) takes at most its iterations over the piece, and one more.
+// (4 rows of 8192 tokens, 32 heads of 128, window 512, 4 first tokens: 112 pieces of up to 11 iterations, 448 MiB beside 512 MiB of
+// gradients. A bound by iterations alone, without the documents' lengths, asked for 2.2 GiB.)
+static long long window_bwd_packed_slots(long long B, long long Sq, long long sinks, long long group, long long near, long long piece) {
+  const long long row_tiles = (Sq + kWinBlock - 1) / kWinBlock, m = (piece > near ? piece : near) / group + 1;
+  const long long shortest = (m - 2) * kWinBlock - 126, documents = shortest < 1 ? Sq : Sq / shortest;
+  const long long blocks = (sinks + kWinBlock - 2) / kWinBlock + 1;
+  return B * blocks * ((row_tiles + 3 * documents) * group / piece + documents);
+}
+
 static WindowBwdPlan window_bwd_plan(int B, int Sq, int Sk, int Hq, int Hkv, int D, int window, int sinks, bool packed) {
   WindowBwdPlan w{};
   const long long group = Hq / Hkv;
@@ -948,20 +961,20 @@ static WindowBwdPlan window_bwd_plan(int B, int Sq, int Sk, int Hq, int Hkv, int
     piece = (near + share - 1) / share;
     if (piece < 2) piece = 2;
   }
-  const long long ordinary = (near + piece - 1) / piece;
-  long long slots = ordinary > 1 ? w.blocks * ordinary : 0;
-  if (sinks > 0 && all > piece) {
-    const long long sink_blocks = (sinks + kWinBlock - 1) / kWinBlock;
-    if (!packed) {
-      const long long n = sink_blocks < w.key_blocks ? sink_blocks : w.key_blocks;
-      slots += B * n * ((all + piece - 1) / piece);
-    } else {
-      // a row tile sees far first tokens of one document, which lie in at most sink_blocks + 1 blocks
-      const long long far = B * all * (sink_blocks + 1);
-      const long long cut = piece > near ? far / (piece - near) : w.blocks;   // blocks that far queries make too long
-      slots += far / piece + 2 * (cut < w.blocks ? cut : w.blocks);
-    }
+  // Pieces of blocks that hold first tokens. Their parts may take as much as dK and dV themselves (half a slot a block), or two pieces
+  // an SM if that is more; where they would take more, pieces get longer, which costs nothing when every SM has several.
+  const long long sink_blocks = (sinks + kWinBlock - 1) / kWinBlock;
+  const long long limit = w.blocks / 2 > 2 * sm_count() / Hkv ? w.blocks / 2 : 2 * sm_count() / Hkv;
+  long long sink_slots = 0;
+  while (sinks > 0 && all > piece) {
+    sink_slots = packed ? window_bwd_packed_slots(B, Sq, sinks, group, near, piece)
+                        : B * (sink_blocks < w.key_blocks ? sink_blocks : w.key_blocks) * ((all + piece - 1) / piece);
+    if (sink_slots <= limit) break;
+    sink_slots = 0;
+    piece += piece / 4 + 1;
   }
+  const long long ordinary = (near + piece - 1) / piece;
+  const long long slots = sink_slots + (ordinary > 1 ? w.blocks * ordinary : 0);
   w.piece = static_cast<int>(piece < (1 << 30) ? piece : (1 << 30));
   w.max_slots = slots;
   w.rows = static_cast<long long>(B) * Hq * w.sq_pad;

@@ -6,7 +6,7 @@ import torch
 
 from maltos_b200.ops import _lib
 from maltos_b200.ops.attention import sliding_window_attention, sliding_window_reference
-from tests.test_window_attention_gpu import DEV, _expect, _qkv
+from tests.test_window_attention_gpu import DEV, _case, _documents, _expect, _qkv
 
 pytestmark = pytest.mark.gpu
 
@@ -39,3 +39,29 @@ def test_a_query_that_is_no_number_spoils_its_own_row_only(Sq, Hq, Hkv, D, keep)
     assert ((out.double() - value).abs() - bound)[~bad].max() <= 1e-9
     good = ~bad[:2]
     assert (lse[:2][good].double() - w_lse.transpose(1, 2)[:2][good]).abs().max() < 1e-4
+
+
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("lengths", [[2900], [1000, 30, 1700, 5, 200], [1400, 1400]])
+def test_long_documents_whose_first_blocks_are_cut(lengths, D):
+    """Long lists of queries of the blocks that hold first tokens, of one head (pieces for want of blocks) and of many."""
+    ids = _documents(1, 3001, lengths, 40)
+    _case(1, 3001, 3001, 2, 1, D, 64, 4, ids=ids)
+    _case(1, 3001, 3001, 10, 10, D, 130, 200, ids=ids)
+
+
+@pytest.mark.parametrize("packed", [False, True])
+def test_more_key_blocks_than_the_list_takes_at_a_time(packed):
+    """1120 key blocks, the first of each row cut into pieces; rows on both sides of the list's steps against the formula."""
+    B, S, D, window, sinks = 70, 2000, 64, 64, 4
+    q, k, v = (t.requires_grad_() for t in _qkv(B, S, S, 1, 1, D, seed=3))
+    ids = _documents(B, S, [700, 1000], 0) if packed else None
+    dout = torch.randn(B, S, 1, D, device=DEV, generator=torch.Generator(device=DEV).manual_seed(4)).bfloat16()
+    out = sliding_window_attention(q, k, v, window=window, sinks=sinks, sequence_ids=ids)
+    grads = torch.autograd.grad(out, (q, k, v), dout)
+    _lib.fetch_status()
+    for b in (0, 62, 63, 64, 69):
+        at = slice(b, b + 1)
+        w_out, _, *w_grads = _expect(*(t.detach()[at] for t in (q, k, v)), dout[at], window, sinks, None if ids is None else ids[at], 1 / math.sqrt(D))
+        for got, (value, bound) in zip((out.detach(), *grads), (w_out, *w_grads)):
+            assert ((got[at].double() - value).abs() - bound).max() <= 1e-9
