@@ -100,10 +100,13 @@ __device__ __forceinline__ WindowTile window_tile(const WindowRule& r, int batch
     if (last < 0) return t;
   }
   t.b0 = lo / kWinBlock, t.b1 = last / kWinBlock + 1;
-  t.sa = start / kWinBlock;
-  t.ea = min((min(start + r.sinks, lo) + kWinBlock - 1) / kWinBlock, t.b0);
-  if (t.ea <= t.sa) t.sa = t.ea = 0;
-  t.lo = lo, t.last = last, t.far = start, t.far_end = min(start + r.sinks, lo);
+  t.lo = lo, t.last = last;
+  const int far_end = min(start + r.sinks, lo);
+  if (far_end > start) {                           // else nothing lies before the window (no first tokens, or all inside it)
+    t.far = start, t.far_end = far_end;
+    t.sa = start / kWinBlock, t.ea = min((far_end + kWinBlock - 1) / kWinBlock, t.b0);
+    if (t.ea <= t.sa) t.sa = t.ea = 0;
+  }
   if (whole) t.full_lo = lo_max, t.full_hi = p0;
   return t;
 }

@@ -65,3 +65,22 @@ def test_more_key_blocks_than_the_list_takes_at_a_time(packed):
         w_out, _, *w_grads = _expect(*(t.detach()[at] for t in (q, k, v)), dout[at], window, sinks, None if ids is None else ids[at], 1 / math.sqrt(D))
         for got, (value, bound) in zip((out.detach(), *grads), (w_out, *w_grads)):
             assert ((got[at].double() - value).abs() - bound).max() <= 1e-9
+
+
+@pytest.mark.parametrize("D", [64, 128])
+def test_without_first_tokens_no_block_before_the_window_is_read(D):
+    """A document that starts inside a block, and a value in that block that only the rows near it may see: NaN tells who reads it."""
+    q, k, v = _qkv(1, 643, 643, 4, 2, D)
+    ids = _documents(1, 643, [560], 70)
+    dout = torch.randn_like(q)
+
+    def run(v):
+        leaves = [t.clone().requires_grad_() for t in (q, k, v)]
+        out = sliding_window_attention(*leaves, window=50, sequence_ids=ids)
+        return out.detach(), torch.autograd.grad(out, leaves, dout)[0]
+
+    want = run(v)
+    v[0, 72] = float("nan")
+    for got, clean in zip(run(v), want):
+        assert torch.isnan(got[0, 72:122]).all()
+        assert torch.equal(got[0, 256:], clean[0, 256:])      # the row tiles whose windows begin in a later block
