@@ -248,3 +248,12 @@ def fetch_status(raise_on_error: bool = True) -> tuple[int, int, int, int]:
             raise CommTimeoutError(msg, peer=vals[2], block=vals[1])
         raise DeviceStatusError(msg)
     return vals  # type: ignore[return-value]
+
+
+def raise_recorded_errors(device) -> None:
+    """Raise what kernels recorded on a CUDA device since the last look (nothing on the CPU). Kernels record and go on - an id outside
+    its table reads as zeros, a wait that ran out leaves wrong sums - so whoever drives them has to ask; waits for the current stream."""
+    device = torch.device(device)
+    if device.type == "cuda":
+        with torch.cuda.device(device):
+            fetch_status()

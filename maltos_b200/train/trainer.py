@@ -3,7 +3,8 @@
 ``fit`` pulls micro-batches until ``max_steps`` optimizer steps are done; metrics are collected once per optimizer step
 and flushed asynchronously (the numbers of interval k are printed at interval k+1), checkpoints are written every
 ``checkpoint_every`` steps into ``checkpoint_dir/step_XXXXXXXX`` with optional retention (``keep_last`` /
-``keep_every_n_steps``) and a free-space guard. Interface of the reference's ``train/trainer.py:25-183``.
+``keep_every_n_steps``) and a free-space guard. A step in which a kernel met an index outside its table, or a wait that ran
+out, ends the run with an error before anything of it is saved. Interface of the reference's ``train/trainer.py:25-183``.
 """
 from __future__ import annotations
 
@@ -16,6 +17,7 @@ from typing import Any
 import torch.distributed as dist
 
 from maltos_b200.data.prefetch import PrefetchDataLoader
+from maltos_b200.ops import _lib
 from maltos_b200.runtime.mesh import MeshAxis
 from maltos_b200.state.checkpoint import save_runtime_spec, save_sharded_checkpoint
 from maltos_b200.utils.distributed import raise_if_any_rank_failed
@@ -190,6 +192,7 @@ class Trainer:
                     rt.step_optimizer()
                 with span("maltos::metrics.aggregate"):
                     self.metric_aggregator.update(rt.collect_metrics())   # one host read of the loss per optimizer step
+                _lib.raise_recorded_errors(rt.device)     # after that read, so it waits for nothing more; before a checkpoint keeps the step
                 self._maybe_log()
                 self._maybe_checkpoint()
                 if self._stop_agreed():
