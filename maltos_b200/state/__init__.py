@@ -1,15 +1,15 @@
 """Checkpointable state: the state index, sharded runtime checkpoints and logical (safetensors) checkpoints."""
 from .checkpoint import (CheckpointArtifact, CheckpointManifest, RankCheckpointMetadata, load_checkpoint_manifest,
-                         load_runtime_spec, load_sharded_checkpoint, save_runtime_spec, save_sharded_checkpoint,
-                         save_sharded_checkpoint_from_model_state)
+                         load_model_options, load_runtime_spec, load_sharded_checkpoint, save_model_options,
+                         save_runtime_spec, save_sharded_checkpoint, save_sharded_checkpoint_from_model_state)
 from .state import (BufferEntry, ModelStateMeta, OptimizerState, ParamEntry, RngState, RuntimeParamAttrs, StateManager,
                     TrainerState)
 
 __all__ = [
     "BufferEntry", "CheckpointArtifact", "CheckpointManifest", "ModelStateMeta", "OptimizerState", "ParamEntry",
     "RankCheckpointMetadata", "RngState", "RuntimeParamAttrs", "StateManager", "TrainerState",
-    "load_checkpoint_manifest", "load_runtime_spec", "load_sharded_checkpoint", "save_runtime_spec",
-    "save_sharded_checkpoint", "save_sharded_checkpoint_from_model_state",
+    "load_checkpoint_manifest", "load_model_options", "load_runtime_spec", "load_sharded_checkpoint", "save_model_options",
+    "save_runtime_spec", "save_sharded_checkpoint", "save_sharded_checkpoint_from_model_state",
 ]
 
 

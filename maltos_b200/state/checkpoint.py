@@ -3,6 +3,7 @@
 Layout (identical to the reference, ``state/checkpoint.py:86-250``, so either implementation loads the other's):
 
     <root>/runtime_spec.json
+    <root>/model_options.json      options of the model that the spec does not carry, where there are any
     <root>/step_XXXXXXXX/manifest.json          rank 0; json.dump(indent=2)
     <root>/step_XXXXXXXX/model_rank_R.pt        dict[state_key -> CPU tensor]
     <root>/step_XXXXXXXX/optim_rank_R.pt        only ranks that are their own optimizer source
@@ -345,6 +346,37 @@ def load_runtime_spec(checkpoint) -> dict[str, Any]:
                 raise ValueError("runtime_spec.json must contain a non-empty mapping")
             return spec
     raise ValueError(f"runtime spec not found for {p}; expected runtime_spec.json in the checkpoint root")
+
+
+def save_model_options(checkpoint_root, options: dict[str, Any]) -> None:
+    """``model_options.json`` beside the runtime spec: model options that the spec does not carry. Without any there is no file."""
+    root = Path(checkpoint_root)
+    target = root / "model_options.json"
+    if target.exists():
+        if load_model_options(root) != options:
+            raise ValueError(f"model options already exist with different contents: {target}")
+        return
+    if not options:
+        return
+    root.mkdir(parents=True, exist_ok=True)
+    tmp = root / "model_options.json.tmp"
+    with tmp.open("w", encoding="utf-8") as f:
+        json.dump(options, f, indent=2)
+        f.write("\n")
+    tmp.replace(target)
+
+
+def load_model_options(checkpoint) -> dict[str, Any] | None:
+    """The options recorded for a checkpoint (its directory or the root), None where none were."""
+    p = Path(checkpoint)
+    for cand in (p / "model_options.json", p.parent / "model_options.json"):
+        if cand.is_file():
+            with cand.open("r", encoding="utf-8") as f:
+                options = json.load(f)
+            if not isinstance(options, dict):
+                raise ValueError("model_options.json must contain a mapping")
+            return options
+    return None
 
 
 def _check_min_free_space(path: Path, min_free_gb: float) -> None:

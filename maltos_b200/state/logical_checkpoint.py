@@ -390,6 +390,10 @@ def iter_logical_tensors_from_runtime_checkpoint(checkpoint_dir: str | Path, *, 
     missing = sorted(set(reference_state) - set(pieces))
     if missing:
         raise ValueError(f"runtime checkpoint missing logical tensors: {missing[:8]}{' ...' if len(missing) > 8 else ''}")
+    extra = sorted(set(pieces) - set(reference_state))
+    if extra:               # a recipe without the options that made them: converting would drop them without a word
+        raise ValueError(f"runtime checkpoint has tensors that the recipe's model has not: {extra[:8]}{' ...' if len(extra) > 8 else ''} "
+                         "(are its block options recorded in model_options.json beside runtime_spec.json?)")
     for name in sorted(reference_state):
         full = _assemble_logical_tensor(name=name, pieces=pieces[name], shard_rules=rules, target_shape=tuple(reference_state[name].shape))
         yield name, full.to(dtype=reference_state[name].dtype).cpu().contiguous()

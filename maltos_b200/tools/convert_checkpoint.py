@@ -1,7 +1,7 @@
 """Convert between runtime checkpoints (per-rank, layout-specific) and logical checkpoints (whole tensors, safetensors).
 
 ``runtime-to-logical --checkpoint <step dir> --output <dir>``: single process; the recipe is read from the runtime spec
-stored next to the checkpoint.
+(and the model options, where there are any) stored next to the checkpoint.
 
 ``logical-to-runtime --config recipe.yaml --checkpoint <logical dir> --output <root> [-- overrides]``: run with the
 target layout's world size (``torchrun``); every rank writes its own model artifact of a weights-only checkpoint
@@ -15,11 +15,12 @@ from pathlib import Path
 import torch
 import torch.distributed as dist
 
-from maltos_b200.state.checkpoint import load_runtime_spec, save_runtime_spec, save_sharded_checkpoint_from_model_state
+from maltos_b200.state.checkpoint import (load_model_options, load_runtime_spec, save_model_options, save_runtime_spec,
+                                          save_sharded_checkpoint_from_model_state)
 from maltos_b200.state.logical_checkpoint import (LogicalCheckpointTensorReader, _build_runtime_model_state_from_logical_tensors,
                                                   iter_logical_tensors_from_runtime_checkpoint, save_logical_checkpoint)
 from maltos_b200.train import cli as train_cli
-from maltos_b200.train.flags import build_runtime_spec, parse_args_from, parse_runtime_spec_args
+from maltos_b200.train.flags import apply_model_options, build_model_options, build_runtime_spec, parse_args_from, parse_runtime_spec_args
 from maltos_b200.utils.distributed import distributed_barrier
 
 
@@ -39,7 +40,7 @@ def build_arg_parser_for_convert() -> argparse.ArgumentParser:
 
 def _recipe_args(args: argparse.Namespace) -> argparse.Namespace:
     if args.command == "runtime-to-logical":
-        return parse_runtime_spec_args(load_runtime_spec(args.checkpoint))
+        return apply_model_options(parse_runtime_spec_args(load_runtime_spec(args.checkpoint)), load_model_options(args.checkpoint) or {})
     overrides = list(args.recipe_overrides)
     if overrides[:1] == ["--"]:
         overrides = overrides[1:]
@@ -60,6 +61,7 @@ def logical_to_runtime(runtime, checkpoint_dir: Path, output_dir: Path, *, recip
     model_state, entries = _build_runtime_model_state_from_logical_tensors(runtime, reader)
     if rank == 0:
         save_runtime_spec(output_dir, build_runtime_spec(recipe))
+        save_model_options(output_dir, build_model_options(recipe))
     if dist.is_initialized():
         distributed_barrier()
     save_sharded_checkpoint_from_model_state(runtime.state_manager, output_dir / "step_00000000", model_state=model_state,

@@ -26,8 +26,9 @@ import torch.distributed as dist
 import yaml
 
 from maltos_b200.runtime.mesh import MeshAxis
+from maltos_b200.state.checkpoint import load_model_options
 from maltos_b200.train import cli as train_cli
-from maltos_b200.train.flags import parse_args_from, parse_runtime_spec_args
+from maltos_b200.train.flags import apply_model_options, parse_args_from, parse_runtime_spec_args
 from maltos_b200.utils.constants import IGNORE_INDEX, INPUT_IDS_KEY, LABELS_KEY, PAD_SEQUENCE_ID, POSITION_IDS_KEY, SEQUENCE_IDS_KEY
 
 DEFAULT_CASE_FILE = Path("configs/profile_train_perf_cases.yaml")
@@ -225,7 +226,7 @@ def _training_args(case: CaseDefinition, overrides: list[str]) -> argparse.Names
     if case.recipe:
         return parse_args_from(["--config", case.recipe, *extra], require_data=False)
     spec = json.loads(Path(case.runtime_spec).read_text(encoding="utf-8"))
-    base = parse_runtime_spec_args(spec)
+    base = apply_model_options(parse_runtime_spec_args(spec), load_model_options(case.runtime_spec) or {})
     if not extra:
         return base
     merged = parse_args_from(extra, require_data=False)

@@ -29,7 +29,7 @@ from maltos_b200.runtime.core import RuntimeCore
 from maltos_b200.runtime.mesh import MeshConfig
 from maltos_b200.utils.distributed import distributed_barrier, raise_if_any_rank_failed
 
-from .flags import build_runtime_spec, parse_args
+from .flags import MODEL_OPTION_DEFAULTS, build_model_options, build_runtime_spec, parse_args
 from .trainer import Trainer, TrainerConfig
 
 
@@ -75,8 +75,8 @@ def validate_args(args: argparse.Namespace, world_size: int) -> None:
                          "(the pipeline runner cuts every micro-batch into that many pieces)")
     if getattr(args, "token_weighted_loss", False) and args.hdp_balanced:
         raise ValueError("--token-weighted-loss is implied by --hdp-balanced (HDP weights every rank's loss by its targets)")
-    for name, default in _BLOCK_OPTIONS.items():
-        if getattr(args, name, default) != default and args.model not in (("llama",) if name == "post_block_norm" else ("llama", "olmo", "olmo2")):
+    for name in build_model_options(args):
+        if args.model not in (("llama",) if name == "post_block_norm" else ("llama", "olmo", "olmo2")):
             raise ValueError(f"--{name.replace('_', '-')} is not an option of --model {args.model}")
     if getattr(args, "sliding_window", None) is not None and (args.cp_size > 1 or args.hdp_balanced):
         raise ValueError("--sliding-window is not supported with --cp-size > 1 or --hdp-balanced")
@@ -133,11 +133,6 @@ def resolve_resume_path(resume_from, checkpoint_dir, *, rank: int):
 
 
 # ------------------------------------------------------------------------------------------------ model
-#: options of the decoder block (``LlamaConfig``, ``OlmoConfig``) that are flags too, with the flags' defaults
-_BLOCK_OPTIONS = {"sliding_window": None, "sink_tokens": 0, "full_attention_every": None, "embedding_scale": None, "post_block_norm": False,
-                  "residual_scale": 1.0, "residual_gate": False}
-
-
 def _variant(base, tp, sp, args):
     return sp if args.use_sp else (tp if args.tp_size > 1 else base)
 
@@ -147,7 +142,7 @@ def _build_model(args: argparse.Namespace) -> nn.Module:
 
     ckpt = M.ActivationCheckpointConfig(enabled=bool(args.activation_checkpointing), every_n_layers=args.activation_checkpoint_every_n_layers)
     name = args.model
-    block = {k: getattr(args, k, d) for k, d in _BLOCK_OPTIONS.items()}
+    block = {k: getattr(args, k, d) for k, d in MODEL_OPTION_DEFAULTS.items()}
     if name == "tiny":
         cls = _variant(M.TinyTransformer, M.TinyTransformerTp, M.TinyTransformerTpSp, args)
         model = cls(args.dim, args.n_heads, args.n_kv_heads or args.n_heads, args.hidden_size, args.eps, args.n_layers,
@@ -504,6 +499,7 @@ def _build_run_manifest(*, args, runtime: RuntimeCore, initial_trainable_params:
             "data_format": data_format,
             "data_paths": [str(p) for p in data_paths],
             "runtime_spec": build_runtime_spec(args),
+            "model_options": build_model_options(args),
             "torch": torch.__version__,
         },
     }
@@ -580,6 +576,7 @@ def main(argv: list[str] | None = None) -> None:
     loggers, uploader = (None, None) if args.dry_run else _build_logging(args, rank)
     trainer = Trainer(
         runtime=runtime, dataloader=loader, logger=loggers, checkpoint_uploader=uploader, runtime_spec=build_runtime_spec(args),
+        model_options=build_model_options(args),
         config=TrainerConfig(max_steps=args.max_steps, log_every=args.log_every, checkpoint_every=args.checkpoint_every,
                              checkpoint_dir=args.checkpoint_dir, resume_from=args.resume_from, load_weights_only=args.load_weights_only,
                              checkpoint_keep_last=args.checkpoint_keep_last, checkpoint_keep_every_n_steps=args.checkpoint_keep_every_n_steps,

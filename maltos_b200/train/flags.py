@@ -7,7 +7,8 @@ the spec layout (``format = "train_cli_args"``, ``version = 3``, 16 model + 22 r
 those of the reference (``train/flags.py:12-403``) because recipes and checkpoints carry them. Additional flags of this
 framework: ``--pp-schedule``, ``--rope-theta``, ``--moe-top-k``, ``--moe-capacity-factor``, ``--init-std`` and the block options
 (``--sliding-window``, ``--sink-tokens``, ``--full-attention-every``, ``--embedding-scale``, ``--post-block-norm``,
-``--residual-scale``, ``--residual-gate``); they are deliberately NOT part of the spec so that spec files stay interchangeable.
+``--residual-scale``, ``--residual-gate``); they are deliberately NOT part of the spec so that spec files stay interchangeable. The block
+options that differ from their defaults stand beside the spec, in ``model_options.json`` (:func:`build_model_options`).
 """
 from __future__ import annotations
 
@@ -240,6 +241,31 @@ def build_runtime_spec(args: argparse.Namespace) -> dict[str, Any]:
         "model": {k: getattr(args, k) for k in _RUNTIME_SPEC_MODEL_FIELDS},
         "runtime": {k: getattr(args, k) for k in _RUNTIME_SPEC_RUNTIME_FIELDS},
     }
+
+
+#: options of the decoder block (``LlamaConfig``, ``OlmoConfig``) that are flags: they change the model, and are not in the spec
+MODEL_OPTION_FIELDS = ("sliding_window", "sink_tokens", "full_attention_every", "embedding_scale", "post_block_norm", "residual_scale", "residual_gate")
+MODEL_OPTION_DEFAULTS = {f.name: f.default for f in FLAGS if f.name in MODEL_OPTION_FIELDS}
+
+
+def build_model_options(args: argparse.Namespace) -> dict[str, Any]:
+    """The block options that differ from their defaults; a model without any has ``{}``."""
+    return {k: getattr(args, k, d) for k, d in MODEL_OPTION_DEFAULTS.items() if getattr(args, k, d) != d}
+
+
+def apply_model_options(args: argparse.Namespace, options: dict[str, Any]) -> argparse.Namespace:
+    """``args`` of a runtime spec with the block options that were recorded beside it."""
+    unknown = sorted(set(options) - set(MODEL_OPTION_FIELDS))
+    if unknown:
+        raise ValueError(f"unknown model options: {unknown}")
+    for k, d in MODEL_OPTION_DEFAULTS.items():
+        setattr(args, k, options.get(k, d))
+    return args
+
+
+def describe_model_options(options: dict[str, Any]) -> str:
+    """As flags, for messages."""
+    return " ".join(f"--{k.replace('_', '-')}" + ("" if v is True else f" {v}") for k, v in sorted(options.items())) or "no block options"
 
 
 def _validate_runtime_spec_fields(section: str, values: dict[str, Any], expected: tuple[str, ...]) -> None:

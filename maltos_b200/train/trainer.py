@@ -19,7 +19,8 @@ import torch.distributed as dist
 from maltos_b200.data.prefetch import PrefetchDataLoader
 from maltos_b200.ops import _lib
 from maltos_b200.runtime.mesh import MeshAxis
-from maltos_b200.state.checkpoint import save_runtime_spec, save_sharded_checkpoint
+from maltos_b200.state.checkpoint import load_model_options, save_model_options, save_runtime_spec, save_sharded_checkpoint
+from maltos_b200.train.flags import describe_model_options
 from maltos_b200.utils.distributed import raise_if_any_rank_failed
 from maltos_b200.utils.metrics import MetricAggregator, PendingMetricFlush
 from maltos_b200.utils.profiling import span
@@ -96,7 +97,7 @@ def _validate(config: TrainerConfig, runtime_spec) -> None:
 
 class Trainer:
     def __init__(self, *, runtime, dataloader, config: TrainerConfig, logger=None, metric_aggregator: MetricAggregator | None = None,
-                 checkpoint_uploader=None, runtime_spec: dict[str, Any] | None = None) -> None:
+                 checkpoint_uploader=None, runtime_spec: dict[str, Any] | None = None, model_options: dict[str, Any] | None = None) -> None:
         _validate(config, runtime_spec)
         self.runtime = runtime
         self.dataloader = PrefetchDataLoader(dataloader) if config.data_prefetch_batches else dataloader
@@ -105,6 +106,7 @@ class Trainer:
         self.metric_aggregator = metric_aggregator or MetricAggregator()
         self.checkpoint_uploader = checkpoint_uploader
         self.runtime_spec = runtime_spec
+        self.model_options = model_options      # options the spec does not carry; None: the caller keeps none
         self._last_logged_step = 0
         self._pending_log: PendingMetricFlush | None = None
         self._graceful_stop = False
@@ -115,16 +117,33 @@ class Trainer:
 
     def setup(self) -> None:
         self.runtime.state_manager.bind_dataloader(self.dataloader)
+        self._check_resumed_options()
         self.runtime.setup(checkpoint_path=self.config.resume_from, load_weights_only=self.config.load_weights_only)
         if self.config.checkpoint_every is not None:
             failure = None
             try:
                 if _is_log_rank():
                     save_runtime_spec(self.config.checkpoint_dir, self.runtime_spec)
+                    if self.model_options is not None:
+                        save_model_options(self.config.checkpoint_dir, self.model_options)
             except Exception as exc:  # noqa: BLE001 - an unwritable checkpoint directory must stop every rank, now
                 failure = exc
             raise_if_any_rank_failed(failure, f"writing the runtime spec under {self.config.checkpoint_dir}")
         self._last_logged_step = self.runtime.state.step_context.step
+
+    def _check_resumed_options(self) -> None:
+        """A window or a scale has no parameter, so a checkpoint would load without them and train another model."""
+        if self.config.resume_from is None or self.config.load_weights_only or self.model_options is None:
+            return
+        failure = None
+        try:
+            recorded = load_model_options(self.config.resume_from)
+            if recorded is not None and recorded != self.model_options:
+                raise ValueError(f"{self.config.resume_from} was trained with {describe_model_options(recorded)}, this run has "
+                                 f"{describe_model_options(self.model_options)}: give the same options to resume, or --load-weights-only to start from its weights")
+        except Exception as exc:  # noqa: BLE001 - re-raised on every rank
+            failure = exc
+        raise_if_any_rank_failed(failure, f"checking the model options of {self.config.resume_from}")
 
     # ------------------------------------------------------------------ graceful stop (not in the reference)
     def enable_graceful_stop(self, signals=()) -> None:
