@@ -5,8 +5,8 @@ import pytest
 import torch
 
 from maltos_b200.ops import _lib
-from maltos_b200.ops.attention import sliding_window_attention, sliding_window_reference
-from tests.test_window_attention_gpu import DEV, _case, _documents, _expect, _qkv
+from maltos_b200.ops.attention import build_window_mask, sliding_window_attention, sliding_window_reference
+from tests.test_window_attention_gpu import DEV, U, _case, _documents, _expect, _qkv
 
 pytestmark = pytest.mark.gpu
 
@@ -84,3 +84,72 @@ def test_without_first_tokens_no_block_before_the_window_is_read(D):
     for got, clean in zip(run(v), want):
         assert torch.isnan(got[0, 72:122]).all()
         assert torch.equal(got[0, 256:], clean[0, 256:])      # the row tiles whose windows begin in a later block
+
+
+@pytest.mark.parametrize("D,lean_k,lean_q", [(64, 12.0, 8.0), (128, 20.0, 6.0)])
+def test_dq_of_rows_whose_weight_is_on_the_first_token(D, lean_k, lean_q):
+    """Queries lean towards what the first key holds, as trained models' do: nearly all weight is on one key, and dS there is the small
+    difference dP - delta, so an error e of delta comes out as e * scale * sum P k, far larger than dq's other errors.
+
+    Bound of the norm of dq's error. Weights and dS are rounded to bf16, each off by at most u, relative and independent, so of
+    variance u^2 / 3 at most. With delta taken from the same weights the former enter as
+    sum_j dS_j d_j (k_j - sum P k), the latter as sum_j dS_j d_j k_j; twice the root of the summed variances, and dq's own rounding.
+    What delta from the rounded output alone would add is far outside, which is asserted too."""
+    S, W, N = 300, 100, 1
+    scale = 1 / math.sqrt(D)
+    g = torch.Generator(device=DEV).manual_seed(D)
+    rnd = lambda *s: torch.randn(*s, device=DEV, generator=g)                # noqa: E731
+    lean = torch.nn.functional.normalize(rnd(D), dim=0)
+    q = (rnd(1, S, 2, D) + lean_q * lean).bfloat16().requires_grad_()
+    k = rnd(1, S, 2, D)
+    k[:, :1] += lean_k * lean
+    k, v, dout = k.bfloat16().requires_grad_(), rnd(1, S, 2, D).bfloat16().requires_grad_(), rnd(1, S, 2, D).bfloat16()
+    out = sliding_window_attention(q, k, v, window=W, sinks=N)
+    dq = torch.autograd.grad(out, (q, k, v), dout)[0]
+    _lib.fetch_status()
+    Q, K, V, dO = (t.detach()[0].double().transpose(0, 1) for t in (q, k, v, dout))
+    seen = build_window_mask(S, S, W, N, None, DEV)
+    P = (Q @ K.transpose(1, 2) * scale).masked_fill(~seen, -math.inf).softmax(-1)
+    O, dP = P @ V, dO @ V.transpose(1, 2)
+    delta = (dO * O).sum(-1, keepdim=True)
+    dS, mean_k = P * (dP - delta), P @ K
+    exact = scale * dS @ K
+    spread = ((K.unsqueeze(1) - mean_k.unsqueeze(2)).square() + K.unsqueeze(1).square()).sum(-1)
+    bound = 2 * scale * U / math.sqrt(3) * (dS.square() * spread).sum().sqrt() + U / math.sqrt(3) * exact.norm()
+    from_out = scale * ((dO * O.bfloat16().double()).sum(-1, keepdim=True) - delta) * mean_k
+    assert from_out.norm() > 3 * bound
+    assert (dq[0].double().transpose(0, 1) - exact).norm() <= bound
+
+
+@pytest.mark.parametrize("lengths,pad", [([40, 200, 1, 300, 60], 0), ([128, 128, 128, 128, 100], 5), ([3] * 50, 130), ([], 0)])
+@pytest.mark.parametrize("window,sinks,Hq,Hkv", [(50, 0, 4, 2), (50, 4, 3, 3), (200, 140, 4, 1)])
+def test_documents_at_head_dim_128(lengths, pad, window, sinks, Hq, Hkv):
+    _case(2, 643, 643, Hq, Hkv, 128, window, sinks, ids=_documents(2, 643, lengths, pad))
+
+
+def test_documents_in_captured_graphs_that_share_a_pool():
+    """Two graphs of the same memory pool, replayed in turn with other documents each time."""
+    q, k, v = (t.requires_grad_() for t in _qkv(1, 700, 700, 4, 2, 64))
+    dout = torch.randn_like(q)
+    layouts = [_documents(1, 700, lengths) for lengths in ([300, 390], [40, 600], [650])]
+    ids = [layouts[0].clone(), layouts[0].clone()]
+
+    def step(i):
+        out = sliding_window_attention(q, k, v, window=70, sinks=2, sequence_ids=i)
+        return (out, *torch.autograd.grad(out, (q, k, v), dout))
+
+    want = [[t.detach().clone() for t in step(i)] for i in layouts]
+    first, second = torch.cuda.CUDAGraph(), torch.cuda.CUDAGraph()
+    with torch.cuda.graph(first):
+        a = step(ids[0])
+    with torch.cuda.graph(second, pool=first.pool()):
+        b = step(ids[1])
+    for i, j in ((0, 1), (2, 0), (1, 2)):
+        ids[0].copy_(layouts[i])
+        first.replay()
+        got = [t.detach().clone() for t in a]
+        ids[1].copy_(layouts[j])
+        second.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(x, y) for x, y in zip(got, want[i])) and all(torch.equal(x, y) for x, y in zip(b, want[j]))
+    _lib.fetch_status()
