@@ -9,18 +9,23 @@
 // arithmetic is at one half, O += P V of the other and the other's next scores are formed. (With whole blocks a tile alternates
 // between 2600 cycles of arithmetic and 1800 of products and their waits, and the two tiles hide only part of that from one
 // another: 4400 cycles for the pair, of 2048 of UMMAs.) Halves of which no row sees a key are left out.
-// Measured (bf16, TFLOP/s of the visible pairs): 8192 rows, 32 / 8 heads of 128, window 1024 206 us / 628; 16384 rows, 8 / 2 heads,
-// window 4096 297 us / 814; the whole causal triangle of 8192 rows 616 us / 890; heads of 64 reach 352, since a product of half the
-// work leaves the same arithmetic. Bound by the tile's arithmetic between two products, by its instructions more than by the
-// exponentials: a quarter of them by polynomial on the multiply-add pipe costs 7 per cent here (the backward gains from that).
+// Measured (launches recorded into a graph, L2 flushed between them, median; TFLOP/s of the visible pairs): 8192 rows, 32 / 8 heads of
+// 128, window 1024 191 to 197 us / 679 to 658 (two boxes); 16384 rows, 8 / 2 heads, window 4096 297 us / 813; the whole causal triangle
+// of 8192 rows 610 us / 901; 32 / 8 heads of 64 176 us / 367, since a product of half the work leaves the same arithmetic. What takes
+// the time is the tile's arithmetic between two products, its instructions more than the exponentials (a quarter of them by
+// polynomial on the multiply-add pipe costs 7 per cent here, where the backward gains): a state of this code, not a limit of the GPU.
 // The two tiles are two query heads of one key/value head on the same rows where the group is even, else neighbouring rows of
 // one head. O is rescaled only when a row's maximum has grown by more than 2^8 since the last rescale: P then stays below 2^8
 // and its bf16 rounding is relative, so nothing is lost, and after the first blocks the rescale hardly ever happens.
 //
-// What P is relative to is a whole power of two, and O is divided by the sum of the ROUNDED P. The backward can then form the
-// very same rounded weights, for which the terms of dS cancel as they do in the exact softmax; with weights rounded in one
-// place only, a row whose keys have much in common (first tokens that take most of the weight) or that sees few keys loses
-// up to a few per cent of dq. For the same reason the forward of a training step keeps what the rounding of O left (out_lo).
+// Roundings. P is bf16 because the operands of a UMMA have one type, and V is bf16: a weight is off by up to half a step, at random
+// over the keys, which adds to the output less than its own rounding (relative error against 64 bits 0.0022 where fp32 weights give
+// 0.0017). P is relative to a whole power of two and O is divided by the sum of the ROUNDED P, so that the dQ kernel can round its
+// weights on the same grid (they differ by a step now and then: part of its exponentials come from a polynomial) and the terms of dS
+// cancel nearly as in the exact softmax. For the same reason the forward of a training step keeps what the rounding of O left
+// (out_lo): where nearly all weight is on one key, as trained models' is on the first, dS is a small difference, and with delta
+// from the rounded output alone dQ of such rows was 8 to 23 times as far off. dK and dV round the normalised weights on a grid of their
+// own: a key's sum over queries has no such cancellation.
 #include "host.h"
 #include "ptx.cuh"
 #include "window.cuh"

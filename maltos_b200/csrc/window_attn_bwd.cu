@@ -13,9 +13,13 @@
 // The keys of first tokens are seen by every later query, so a block that holds some has many times the work of the others; and
 // with few heads there are fewer blocks than SMs. Both are met by cutting a block's work into pieces. No atomics: the same bits
 // every time.
+// P and dS enter their products in bf16, since the operands of a UMMA have one type and Q, K and dO are bf16; sums are fp32. Each
+// rounding is up to half a step of one term, at random over a sum's terms: dQ, dK and dV are 0.0030 to 0.0035 off relative to 64 bits,
+// where their own rounding alone is 0.0017. delta is known to some 17 bits, from out and out_lo.
 // What bounds it: the UMMAs (7 products of 128 x 128 x D a tile pair, against 5 that the mathematics needs) and the waits
-// between them; see the notes at the two loops. Measured (8192 rows, 32 / 8 heads of 128, window 1024): 544 us, 595 TFLOP/s of the
-// five products (preparation 42, dK / dV 320, dQ 225 each by itself); 16384 rows, 8 / 2 heads, window 4096: 851 us, 709 TFLOP/s.
+// between them; see the notes at the two loops. Measured with the forward (launches in a graph, L2 flushed between): 8192 rows, 32 / 8
+// heads of 128, window 1024 746 to 760 us, 606 to 596 TFLOP/s of the seven products counted (two boxes; preparation 42, dK / dV 328, dQ
+// 236 each by itself under a profiler); 16384 rows, 8 / 2 heads, window 4096 1165 us, 725 TFLOP/s.
 #include "host.h"
 #include "ptx.cuh"
 #include "window.cuh"
@@ -820,8 +824,9 @@ window_bwd_dq_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
     if (static_cast<int>(blockIdx.x) < items) fetch(blockIdx.x);
     for (int item = blockIdx.x; item < items; item += gridDim.x) {
       const int n = t.count(), qi = q0 + row;
-      // The forward's own rounded weights, so that the terms of dS cancel as exactly as there: weights relative to a whole power
-      // of two (the forward's differ from it by another such factor), rounded to bf16, times what is left of 2^-lse2.
+      // Weights rounded on the forward's grid, so that the terms of dS cancel nearly as exactly as there: relative to a whole power of
+      // two (the forward's differ from it by another such factor), rounded to bf16, times what is left of 2^-lse2. They are the
+      // forward's but for a neighbouring bf16 value now and then, since a quarter comes from the polynomial.
       const float shift = floorf(my_lse);
       const float factor = my_lse != INFINITY ? wb_exp2(shift - my_lse) : 0.f;
       const uint64_t shift2 = f32x2(-shift, -shift), factor2 = f32x2(factor, factor), offset2 = f32x2(-my_delta * factor, -my_delta * factor);
