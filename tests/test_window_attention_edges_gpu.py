@@ -153,3 +153,26 @@ def test_documents_in_captured_graphs_that_share_a_pool():
         torch.cuda.synchronize()
         assert all(torch.equal(x, y) for x, y in zip(got, want[i])) and all(torch.equal(x, y) for x, y in zip(b, want[j]))
     _lib.fetch_status()
+
+
+@pytest.mark.parametrize("D", [64, 128])
+def test_weights_of_the_backward_over_their_whole_range(D):
+    """With unit vectors as the output's gradient, dV holds the backward's weights themselves, from near 1 to below the smallest normal
+    number, in every column of a tile (a quarter of the exponentials are a polynomial's)."""
+    Sk, Sq = 400, 64
+    g = torch.Generator(device=DEV).manual_seed(0)
+    q, k = torch.zeros(1, Sq, 1, D, device=DEV), torch.zeros(1, Sk, 1, D, device=DEV)
+    q[..., 0] = 1
+    k[..., 0] = -95 * torch.rand(1, Sk, 1, device=DEV, generator=g)
+    k[0, :40, 0, 0] = torch.linspace(-1, 0, 40, device=DEV)
+    q, k = q.bfloat16().requires_grad_(), k.bfloat16().requires_grad_()
+    v = torch.randn(1, Sk, 1, D, device=DEV, generator=g).bfloat16().requires_grad_()
+    dout = torch.eye(Sq, D, device=DEV).view(1, Sq, 1, D).bfloat16()
+    out = sliding_window_attention(q, k, v, window=Sk, scale=1.0)
+    dv = torch.autograd.grad(out, (q, k, v), dout)[2][0, :, 0, :Sq].double()
+    _lib.fetch_status()
+    seen = build_window_mask(Sq, Sk, Sk, 0, None, DEV)[0]
+    want = k.detach()[0, :, 0, 0].double().expand(Sq, Sk).masked_fill(~seen, -math.inf).softmax(-1).t()
+    assert (want[want > 0].min() < 2.0 ** -126) and want.max() > 0.02
+    # rounded to bf16, and over the sum of the forward's rounded weights; fp32's argument of the exponential (up to 140) is off by 2^-17
+    assert ((dv - want).abs() <= (2.1 * U + 2.0 ** -12) * want + 2.0 ** -126).all()
